@@ -262,6 +262,54 @@ int tbf16_attn_bwd(const void* q, const void* k, const void* v, const void* o16,
                    void* dq, void* dk, void* dv, int32_t* exps_out, int32_t* overflow, const int32_t* gate,
                    void* ws, int64_t ws_bytes, void* stream);
 
+/* Rows of bf16 as 8-bit integers with one scale each: with a = max_k |x[r, k]|,
+ * y8[r, k] = rint(127 x[r, k] / a) (ties to even, of the exact quotient), scale[r] = a / 127;
+ * zero codes for an all-zero row, zero codes and a NaN scale for a row with an infinity or
+ * a NaN. x bf16 (R, K), row stride ldx, any alignment; y8 int8, rows 16-byte aligned, ldy % 16
+ * == 0, written up to K rounded up to 16 (zeros). K <= TBF16_I8_MAX_K: the int32 sums of
+ * K products of codes cannot overflow. No counterpart in the reference. */
+#define TBF16_I8_MAX_K 131072
+int tbf16_quantize_rows_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, float* scale,
+                           void* stream);
+
+/* Linear in 8-bit integers: y[m, n] = bf16((sum_k qx[m, k] w8[n, k]) sx[m] ws[n] + bias[n]),
+ * x quantised per row inside the call as tbf16_quantize_rows_i8 does, int32 sums on the i8
+ * MFMA, the scales and the bias in fp32. w8 int8 (N, K) with scales ws fp32 (N,)
+ * (tbf16_quantize_rows_i8 of the weight): rows 16-byte aligned, ldw % 16 == 0, readable up
+ * to K rounded up to 16 (what is there does not matter). bias bf16 (N,) or NULL. y bf16,
+ * rows 16-byte aligned, ldy % 8 == 0; columns from N up to N rounded up to 8 are written with
+ * values to leave out. workspace: tbf16_linear_i8_ws_bytes(M, K, N) bytes, 16-byte aligned.
+ * No counterpart in the reference. */
+size_t tbf16_linear_i8_ws_bytes(int64_t M, int64_t K, int64_t N);
+int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx, const void* w8, int64_t N, int64_t ldw,
+                    const float* ws, const void* bias, void* y, int64_t ldy, void* workspace, int64_t ws_bytes,
+                    void* stream);
+
+/* Writes tokens' keys and values into a paged cache: for slots[t] = s with 0 <= s < pages *
+ * page, k_cache[s / page, h, s % page, :] = k[t, h, :], the same for v; other s leave the cache
+ * as it is. Of tokens with the same slot the last one's rows stay. k, v bf16 (T, Hkv, D),
+ * element strides (t, h); k_cache, v_cache bf16 (pages, Hkv, page, D), element strides
+ * (page, head, row), no two elements at one address; D contiguous, everything 16-byte aligned. No counterpart in the
+ * reference, which has no cache. */
+int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int64_t D, const int64_t* k_strides,
+                      const int64_t* v_strides, const int32_t* slots, void* k_cache, void* v_cache, int64_t pages,
+                      int64_t page, const int64_t* kc_strides, const int64_t* vc_strides, void* stream);
+
+/* Attention of one new token per sequence over a paged cache: o[b, h] = softmax(scale q[b, h] .
+ * k_j) v_j over positions j < lengths[b], position j in page table[b, j / page], row j % page,
+ * head h / (H / Hkv). fp32 logits, running maximum, sum and output, one rounding to bf16.
+ * Positions past max_pages * page and positions whose page lies outside [0, pages) are left
+ * out; a sequence with none gives zeros. q bf16 (B, H, D), element strides (b, h); caches as tbf16_paged_write's
+ * (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row stride
+ * table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. ws:
+ * tbf16_paged_attn_ws_bytes(B, H, Hkv, D) bytes, 16-byte aligned, for this call alone until
+ * it has run. Serves the calls the reference leaves to torch (tbf16/convert.py:29-30). */
+size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D);
+int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
+                     const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int64_t* kc_strides,
+                     const int64_t* vc_strides, const int32_t* table, int64_t table_stride, int64_t max_pages,
+                     const int32_t* lengths, float scale, void* o, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,10 +8,13 @@ __version__ = "0.1.0"
 
 from .attention import sdpa
 from . import autograd
-from .convert import Linear, TrainLinear, convert, install_sdpa, is_supported_gpu, uninstall_sdpa
+from .convert import Int8Linear, Linear, TrainLinear, convert, install_sdpa, is_supported_gpu, uninstall_sdpa
+from .int8 import int8_linear, prepare_weight_i8, quantize_rows_i8
 from .ops import prepare_weight, quantize_rows, scaled_linear
+from .paged import paged_sdpa, paged_write
 from .patch import TuringBF16Mode, patch
 
 __all__ = ["quantize_rows", "scaled_linear", "prepare_weight", "sdpa", "patch", "TuringBF16Mode", "convert",
            "Linear", "TrainLinear", "autograd", "install_sdpa", "uninstall_sdpa",
-           "is_supported_gpu"]
+           "is_supported_gpu", "paged_sdpa", "paged_write", "int8_linear", "prepare_weight_i8", "quantize_rows_i8",
+           "Int8Linear"]

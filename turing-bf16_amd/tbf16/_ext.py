@@ -63,6 +63,12 @@ _SIGS = {
     "tbf16_attn_bwd_ws_bytes": (SZ, [I64, I64, I64, I64, I64, I64]),
     "tbf16_attn_bwd": (I, [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, PI64, PI64, PI64, PI64, P, PI64, F,
                            I, I, F, U64, P, P, P, P, P, P, P, I64, P]),
+    "tbf16_quantize_rows_i8": (I, [P, I64, I64, I64, P, I64, P, P]),
+    "tbf16_linear_i8_ws_bytes": (SZ, [I64, I64, I64]),
+    "tbf16_linear_i8": (I, [P, I64, I64, I64, P, I64, I64, P, P, P, I64, P, I64, P]),
+    "tbf16_paged_write": (I, [P, P, I64, I64, I64, PI64, PI64, P, P, P, I64, I64, PI64, PI64, P]),
+    "tbf16_paged_attn_ws_bytes": (SZ, [I64, I64, I64, I64]),
+    "tbf16_paged_attn": (I, [P, I64, I64, I64, I64, PI64, P, P, I64, I64, PI64, PI64, P, I64, I64, P, F, P, P, I64, P]),
 }
 
 

@@ -2,13 +2,15 @@
 of the reference: same entry points, layer classes, buffer names and thresholds).
 
     tbf16.convert(model)               # inference
+    tbf16.convert(model, int8=True)    # inference, linears in 8-bit integers
     tbf16.convert(pipe)                # a diffusers-style pipeline: each nn.Module component
     tbf16.convert(model, train=True)   # training / fine-tuning (also after PEFT/LoRA wrapping)
 
 Inference: each bf16 nn.Linear on the GPU is replaced by a tbf16.Linear whose weight
 is stored as fp16 `weight16` plus one fp32 power-of-two inverse scale per output row,
 `weight_scale` (the bytes of the bf16 weight, the same values); bf16 Conv1d/2d/3d
-become scaled fp16 convolutions (tbf16.conv). Parameters shared between modules
+become scaled fp16 convolutions (tbf16.conv). With int8=True the linears become
+tbf16.Int8Linear instead: int8 `weight8` and its scales, half the bytes. Parameters shared between modules
 (tied embeddings) stay native, so nothing is stored twice.
 Training: each nn.Linear changes class to tbf16.TrainLinear, an nn.Linear subclass
 with the same parameters, hooks and wrappers, whose bf16 forward and backward run
@@ -28,6 +30,7 @@ import torch.nn.functional as F
 from . import autograd, routing
 from .attention import sdpa as _scaled_sdpa
 from .conv import convert_conv, convertible
+from .int8 import MAX_K, int8_linear, prepare_weight_i8
 from .ops import prepare_weight, scaled_linear
 
 # Training: layers with in or out features below this run in fp32 (tbf16/convert.py:26-27).
@@ -60,6 +63,37 @@ class Linear(nn.Module):
         wants_grad = torch.is_grad_enabled() and x.requires_grad
         if x.dtype == torch.bfloat16 and not wants_grad:
             return scaled_linear(x, self.weight16, self.weight_scale, self.bias)
+        # other dtypes, and inputs that need a gradient: the native op on the rebuilt weight
+        bias = None if self.bias is None else self.bias.to(x.dtype)
+        return F.linear(x, self.weight.to(x.dtype), bias)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+class Int8Linear(nn.Module):
+    """Inference stand-in for a bf16 nn.Linear in 8-bit integers (tbf16.int8_linear). Buffers
+    `weight8` (int8, N x K) and `weight_scale` (fp32, N) carry the weight, rounded to 8 bits
+    relative to each row's maximum; `bias` is the original parameter."""
+
+    def __init__(self, lin: nn.Linear):
+        super().__init__()
+        self.in_features = lin.in_features
+        self.out_features = lin.out_features
+        w8, ws = prepare_weight_i8(lin.weight.data)
+        self.register_buffer("weight8", w8)
+        self.register_buffer("weight_scale", ws)
+        self.bias = lin.bias
+
+    @property
+    def weight(self) -> torch.Tensor:
+        """The bf16 weight nearest to weight8 times weight_scale, rebuilt on each read."""
+        return (self.weight8.float() * self.weight_scale.unsqueeze(1)).to(torch.bfloat16)
+
+    def forward(self, x):
+        wants_grad = torch.is_grad_enabled() and x.requires_grad
+        if x.dtype == torch.bfloat16 and not wants_grad:
+            return int8_linear(x, self.weight8, self.weight_scale, self.bias)
         # other dtypes, and inputs that need a gradient: the native op on the rebuilt weight
         bias = None if self.bias is None else self.bias.to(x.dtype)
         return F.linear(x, self.weight.to(x.dtype), bias)
@@ -163,7 +197,7 @@ def _to_training(root: nn.Module) -> None:
             m.__class__ = TrainLinear
 
 
-def _to_inference(root: nn.Module, conv: bool) -> None:
+def _to_inference(root: nn.Module, conv: bool, int8: bool) -> None:
     shared = _shared_parameters(root)
     replaced = {}  # a module reachable from two parents is converted once
     for parent in list(root.modules()):
@@ -175,18 +209,22 @@ def _to_inference(root: nn.Module, conv: bool) -> None:
             if not isinstance(w, torch.Tensor) or id(w) in shared:
                 continue
             if type(child) is nn.Linear and w.dtype == torch.bfloat16 and w.is_cuda:
-                new = Linear(child)
-                child.weight = None  # drop the bf16 copy as soon as the fp16 one exists
+                new = Int8Linear(child) if int8 and child.in_features <= MAX_K else Linear(child)
+                child.weight = None  # drop the bf16 copy as soon as the converted one exists
                 replaced[id(child)] = new
                 setattr(parent, name, new)
             elif conv and convertible(child):
                 convert_conv(child)
 
 
-def convert(model, train: bool = False, sdpa: bool = True, force: bool = False, conv: bool = True):
+def convert(model, train: bool = False, sdpa: bool = True, force: bool = False, conv: bool = True,
+            int8: bool = False):
     """Convert `model` in place and return it (tbf16/convert.py:108-147). On GPUs other
     than gfx950 it warns and returns the model unchanged unless force=True.
-    conv: also convert bf16 Conv1d/2d/3d (inference only)."""
+    conv: also convert bf16 Conv1d/2d/3d (inference only). int8: linears in 8-bit integers
+    (inference only; layers of more than 131072 inputs stay with fp16)."""
+    if train and int8:
+        raise ValueError("tbf16.convert: int8 linears are for inference, not train=True")
     if not force and not is_supported_gpu():
         warnings.warn("tbf16.convert: this GPU is not an MI355X (gfx950); leaving the model unchanged. "
                       "Pass force=True to convert anyway.")
@@ -195,7 +233,7 @@ def convert(model, train: bool = False, sdpa: bool = True, force: bool = False, 
         if train:
             _to_training(root)
         else:
-            _to_inference(root, conv)
+            _to_inference(root, conv, int8)
     if not train and torch.cuda.is_available():
         torch.cuda.empty_cache()
     if sdpa:

@@ -44,67 +44,572 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
 }
 
 // ---- attention ----------------------------------------------------------------------
+//
+// o = sum_j p_j v_j / sum_j p_j, p_j = exp2(s_j - m), s_j = scale log2(e) q . k_j, with the
+// maximum m and both sums running over tiles of 32 keys.
+//
+// A unit is one sequence's key/value head with up to 16 RT of its query heads (rows). A tile's
+// logits are K Q^T on v_mfma_f32_16x16x32_bf16: K rows as they lie in memory (lane l: key l %
+// 16, chunks of 8 elements l / 16 + 4 i) against the rows' Q, so lane l gets, for row l % 16,
+// keys 4 (l / 16) .. + 3 of each half tile. Those are the lane's 8 k slots of the second
+// product O^T = V^T P^T, whose operand P so needs no exchange. V^T's operand holds, for the same
+// 8 keys, element dd of chunk l % 16 (chunks of CH = DP / 16): the lane loads its chunk of its
+// 8 keys' rows (whole rows per 16 lanes) and picks halves with v_perm_b32, DP / 16 MFMAs per 32
+// keys. O^T then has row l % 16's elements CH (4 (l / 16) + i) + dd in lane l: the softmax
+// factors of a lane belong to its own outputs. Nothing goes through LDS, every byte of K and V
+// is loaded once, by one wave. p goes in as the sum of two bf16 (its leading 8 bits and the
+// rest rounded, 2^-17 of p lost): one bf16 would add an error of the output's own rounding.
+//
+// Memory bounds it: 16 KB a tile of D = 128 against ~ 130 VALU instructions and 24 MFMAs.
+// K and V of the next tile are loaded as soon as this tile's registers are free, its page
+// entries one tile earlier, across the ends of units too.
+//
+// Tiles of all units form one list (by sequence, then head). Each wave takes an equal run of
+// it, so a batch of ragged lengths keeps every wave busy to the end. What a wave computes of a
+// unit that other waves share is joined through LDS inside a block, and through memory and a
+// second launch between blocks. Where the cache is so short that a block covers a unit, blocks
+// are units and the second launch is left out.
 
-// One block per (sequence, query head): 256 keys at a time, a thread per key for the
-// logits, a thread per output element for the weighted sum. Running maximum and sum in
-// fp32 (log2 domain).
-__global__ __launch_bounds__(256) void paged_attn_kernel(const uint16_t* __restrict__ q, int64_t q_sb, int64_t q_sh,
-                                                         const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                                                         CacheGeom kg, CacheGeom vg, int64_t pages, int page,
-                                                         const int32_t* __restrict__ table, int64_t t_sb, int max_pages,
-                                                         const int32_t* __restrict__ lengths, float scale_log2, int H,
-                                                         int G, int D, uint16_t* __restrict__ o) {
-  __shared__ float qs[256], w[256], red[4];
-  __shared__ int64_t row[256];
-  const int b = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
-  const int64_t cap = (int64_t)max_pages * page;
-  const int len = (int)min<int64_t>(max(lengths[b], 0), cap);
-  if (tid < D) qs[tid] = bf16_lo(q[b * q_sb + h * q_sh + tid]);
-  __syncthreads();
-  // the lowest finite value: infinite logits below it weigh nothing, and nothing is inf - inf
-  float m = -FLT_MAX, l = 0.f, acc = 0.f;
-  bool some = false;
-  for (int j0 = 0; j0 < len; j0 += 256) {
-    const int j = j0 + tid;
-    float s = -INFINITY;
-    int64_t at = -1;
-    if (j < len) {
-      const int p = table[b * t_sb + j / page];
-      if (p >= 0 && p < pages) {
-        at = p;
-        const uint16_t* kr = kc + p * kg.sp + (h / G) * kg.sh + (j % page) * kg.ss;
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(qs[d], bf16_lo(kr[d]), s);
-        s *= scale_log2;
-      }
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 32;
+// Running maxima start at kNone; a unit that had any key ends at kFew or above.
+constexpr float kNone = -FLT_MAX, kFew = -3.0e38f;
+
+struct AttnArgs {
+  const uint16_t *q, *kc, *vc;
+  int64_t q_sb, q_sh;
+  CacheGeom kg, vg;
+  const int32_t *table, *lengths;
+  int64_t t_sb, cap;  // positions a table row covers
+  uint32_t pages, page, magic, shift;  // j / page = (j magic) >> shift for j < 2^31
+  float scale_log2;
+  int B, H, Hkv, G, D, R, RG;  // R rows a unit, RG units a key/value head
+  uint16_t* o;
+  float *part, *stat;  // [block][2][R][D], [block][2][R][2]
+};
+
+__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
+  return (int)min<int64_t>(max(a.lengths[b], 0), a.cap);
+}
+__device__ __forceinline__ int64_t wave_sum_l(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, kWave);
+  return v;
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform_l(int64_t v) {
+  return (int64_t)(uint32_t)uniform((int)v) | (int64_t)uniform((int)(v >> 32)) << 32;
+}
+// Tiles of the whole batch, per unit of a sequence.
+__device__ __forceinline__ int64_t batch_tiles(const AttnArgs& a, int lane) {
+  int64_t n = 0;
+  for (int b = lane; b < a.B; b += kWave) n += (seq_len(a, b) + kTile - 1) / kTile;
+  return uniform_l(wave_sum_l(n));
+}
+// The list's split: tiles per wave, at least kMinTiles.
+constexpr int kMinTiles = 2;
+__device__ __forceinline__ int64_t tiles_per_wave(int64_t tiles, int64_t waves) {
+  return max<int64_t>(kMinTiles, (tiles + waves - 1) / waves);
+}
+
+// A place in the list.
+struct Cursor {
+  int b, unit, tile, nt, len;
+};
+__device__ __forceinline__ void enter(const AttnArgs& a, Cursor& c) {  // c.b set: its first tile, skipping empty ones
+  c.unit = c.tile = c.nt = c.len = 0;
+  while (c.b < a.B && (c.len = uniform(seq_len(a, c.b))) == 0) ++c.b;
+  c.nt = (c.len + kTile - 1) / kTile;
+}
+__device__ __forceinline__ void advance(const AttnArgs& a, Cursor& c, int units) {
+  if (++c.tile < c.nt) return;
+  c.tile = 0;
+  if (++c.unit < units) return;
+  ++c.b;
+  enter(a, c);
+}
+// Tile t of the list.
+__device__ __forceinline__ Cursor locate(const AttnArgs& a, int64_t t, int units, int lane) {
+  Cursor c{0, 0, 0, 0, 0};
+  for (int b0 = 0;; b0 += kWave) {
+    const int b = b0 + lane;
+    const int64_t n = b < a.B ? (int64_t)((seq_len(a, b) + kTile - 1) / kTile) * units : 0;
+    int64_t up = n;  // inclusive prefix sums
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int64_t v = __shfl_up((long long)up, o, kWave);
+      if (lane >= o) up += v;
     }
-    row[tid] = at;
-    float mt = wave_max(s);
-    if ((tid & 63) == 0) red[tid >> 6] = mt;
-    const bool here = __syncthreads_or(at >= 0);
-    if (here) {
-      some = true;
-      // a NaN logit has to reach the output: the maximum may leave it out, its weight is NaN
-      const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-      const float f = exp2f(m - mn);
-      w[tid] = at >= 0 ? exp2f(s - mn) : 0.f;
-      __syncthreads();
-      acc *= f;
-      l *= f;
-      for (int i = 0; i < 256; ++i)
-        if (row[i] >= 0) {
-          l += w[i];
-          if (tid < D)
-            acc = fmaf(w[i], bf16_lo(vc[row[i] * vg.sp + (h / G) * vg.sh + ((j0 + i) % page) * vg.ss + tid]), acc);
+    const uint64_t past = __ballot(up > t);
+    if (past == 0 && b0 + kWave < a.B) {
+      t -= uniform_l(__shfl((long long)up, kWave - 1, kWave));
+      continue;
+    }
+    const int l = past ? __builtin_ctzll(past) : kWave - 1;
+    c.b = b0 + l;
+    t -= uniform_l(__shfl((long long)(up - n), l, kWave));
+    break;
+  }
+  c.len = uniform(seq_len(a, c.b));
+  c.nt = (c.len + kTile - 1) / kTile;
+  c.unit = (int)(t / c.nt);
+  c.tile = (int)(t % c.nt);
+  return c;
+}
+
+// What a lane holds of a unit: for row l % 16 of each 16-row block, the maximum, its own
+// part of the sum, and DP / 4 outputs.
+template <int DP, int RT>
+struct Acc {
+  static constexpr int CH = DP / 16;
+  float m[RT], l[RT];
+  floatx4 o[RT][CH];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      m[r] = kNone;
+      l[r] = 0.f;
+#pragma unroll
+      for (int d = 0; d < CH; ++d) o[r][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __device__ __forceinline__ void scale(int r, float f) {
+    l[r] *= f;
+#pragma unroll
+    for (int d = 0; d < CH; ++d) o[r][d] *= f;
+  }
+  // the sum over the four lanes of a row, once, before the unit leaves its wave
+  __device__ __forceinline__ void total() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) l[r] = sum_xor32(sum_xor16(l[r]));
+  }
+  // put / take: rows of D floats at `rows` (stride ld), their (m, l) at `stat`
+  __device__ __forceinline__ void put(float* rows, int ld, float* stat, int R, int D, int lane) const {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = 16 * r + (lane & 15);
+      if (row >= R) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < CH; d += 4) {
+          const int at = CH * (4 * (lane >> 4) + i) + d;
+          if (at < D)
+            *reinterpret_cast<float4*>(rows + (int64_t)row * ld + at) =
+                make_float4(o[r][d][i], o[r][d + 1][i], o[r][d + 2][i], o[r][d + 3][i]);
         }
-      m = mn;
+      if (lane < 16) *reinterpret_cast<float2*>(stat + 2 * row) = make_float2(m[r], l[r]);
     }
-    __syncthreads();
   }
-  if (tid < D) {
-    const float y = some ? acc / l : 0.f;
-    o[((int64_t)b * H + h) * D + tid] = (uint16_t)pack_bf16(y, 0.f);
+  __device__ __forceinline__ void take(const float* rows, int ld, const float* stat, int R, int D, int lane) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = 16 * r + (lane & 15);
+      if (row >= R) continue;
+      const float2 s = *reinterpret_cast<const float2*>(stat + 2 * row);
+      const float mn = fmaxf(m[r], s.x), f = exp2f(s.x - mn);
+      scale(r, exp2f(m[r] - mn));
+      m[r] = mn;
+      l[r] = fmaf(f, s.y, l[r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < CH; d += 4) {
+          const int at = CH * (4 * (lane >> 4) + i) + d;
+          if (at < D) {
+            const float4 v = *reinterpret_cast<const float4*>(rows + (int64_t)row * ld + at);
+            o[r][d][i] = fmaf(f, v.x, o[r][d][i]);
+            o[r][d + 1][i] = fmaf(f, v.y, o[r][d + 1][i]);
+            o[r][d + 2][i] = fmaf(f, v.z, o[r][d + 2][i]);
+            o[r][d + 3][i] = fmaf(f, v.w, o[r][d + 3][i]);
+          }
+        }
+    }
   }
+  // the outputs: o points at the unit's first row
+  __device__ __forceinline__ void finish(uint16_t* out, int R, int D, int lane) const {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = 16 * r + (lane & 15);
+      if (row >= R) continue;
+      const float f = m[r] == kNone ? 0.f : 1.f / l[r];  // no key at all: zeros
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < CH; d += 4) {
+          const int at = CH * (4 * (lane >> 4) + i) + d;
+          if (at < D)
+            *reinterpret_cast<uint2*>(out + (int64_t)row * D + at) =
+                make_uint2(pack_bf16(o[r][d][i] * f, o[r][d + 1][i] * f), pack_bf16(o[r][d + 2][i] * f, o[r][d + 3][i] * f));
+        }
+    }
+  }
+};
+
+// A unit's first row in o, and how many it has.
+__device__ __forceinline__ uint16_t* unit_out(const AttnArgs& a, int b, int unit) {
+  return a.o + ((int64_t)b * a.H + unit / a.RG * a.G + unit % a.RG * a.R) * a.D;
+}
+__device__ __forceinline__ int unit_rows(const AttnArgs& a, int unit) { return min(a.R, a.G - unit % a.RG * a.R); }
+
+// DP: D rounded up to 64, 128 or 256 (D == DP unless PAD). WPB waves a block. UNIT: one block
+// per unit instead of equal runs of the list.
+template <int DP, int RT, int WPB, bool PAD, bool UNIT>
+__global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
+  constexpr int CH = DP / 16, KI = DP / 32, VW = CH / 2;  // V dwords a lane holds of a key
+  extern __shared__ __align__(16) float lds[];  // [wave][R][DP + 4], [wave][R][2]
+  __shared__ int flags[WPB];  // 1: the wave left a part of a unit begun before it, 2: its last
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
+  const int units = a.Hkv * a.RG;
+  const int ld = DP + 4;
+  float* const stat0 = lds + WPB * a.R * ld;
+
+  Cursor cur;
+  int64_t n;  // this wave's tiles
+  if constexpr (UNIT) {
+    cur.b = blockIdx.x / units;
+    cur.unit = blockIdx.x % units;
+    cur.len = uniform(seq_len(a, cur.b));
+    cur.nt = (cur.len + kTile - 1) / kTile;
+    const int c = (cur.nt + WPB - 1) / WPB;
+    cur.tile = min(wave * c, cur.nt);
+    n = min(c, cur.nt - cur.tile);
+    if (cur.nt == 0) {
+      const int rows = unit_rows(a, cur.unit) * a.D / 8;
+      for (int i = threadIdx.x; i < rows; i += WPB * 64)
+        stg16(unit_out(a, cur.b, cur.unit) + 8 * i, make_uint4(0, 0, 0, 0));
+      return;
+    }
+  } else {
+    const int64_t tiles = batch_tiles(a, lane) * units, c = tiles_per_wave(tiles, (int64_t)gridDim.x * WPB);
+    const int64_t t0 = ((int64_t)blockIdx.x * WPB + wave) * c;
+    n = max<int64_t>(0, min(c, tiles - t0));
+    if (n > 0) cur = locate(a, t0, units, lane);
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
+      if (seq_len(a, b) == 0)
+        for (int i = threadIdx.x; i < a.H * a.D / 8; i += WPB * 64)
+          stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
+  }
+  if (lane == 0) flags[wave] = 0;
+
+  Acc<DP, RT> acc;
+  bool tail = false;  // acc is the begin of a unit that goes on in the next wave
+  if (n > 0) {
+    struct Page {
+      int id, row;
+    };
+    // the page and row of the lane's key (l % 32) of a tile
+    auto page_of = [&](const Cursor& c) {
+      const uint32_t pos = c.tile * kTile + (lane & 31);
+      const uint32_t idx = (uint32_t)((uint64_t)pos * a.magic >> a.shift);
+      Page p{-1, (int)(pos - idx * a.page)};
+      if (pos < (uint32_t)c.len) p.id = a.table[c.b * a.t_sb + idx];
+      return p;
+    };
+    uint4 kr[2][KI];
+    uint32_t vr[8][VW];
+    uint32_t live;  // keys of the tile that there are
+    auto shfl_off = [&](int64_t off, int src) {
+      return (int64_t)(uint32_t)__shfl((int)off, src, kWave) | (int64_t)__shfl((int)(off >> 32), src, kWave) << 32;
+    };
+    auto load_k = [&](const Cursor& c, const Page& p) {
+      const bool ok = (uint32_t)p.id < a.pages;
+      const int64_t off = ok ? (int64_t)p.id * a.kg.sp + (int64_t)p.row * a.kg.ss : 0;
+      const uint16_t* base = a.kc + c.unit / a.RG * a.kg.sh;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint16_t* row = base + shfl_off(off, 16 * h + r16);
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+          const int e = 8 * (g + 4 * i);
+          kr[h][i] = ldg16(row + (PAD && e >= a.D ? 0 : e));
+        }
+      }
+    };
+    auto load_v = [&](const Cursor& c, const Page& p) {
+      const bool ok = (uint32_t)p.id < a.pages;
+      const int64_t off = ok ? (int64_t)p.id * a.vg.sp + (int64_t)p.row * a.vg.ss : 0;
+      const int e = PAD && CH * r16 >= a.D ? 0 : CH * r16;  // (what lies past D goes to outputs past D)
+      const uint16_t* base = a.vc + c.unit / a.RG * a.vg.sh + e;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(base + shfl_off(off, 16 * (j >> 2) + 4 * g + (j & 3)));
+#pragma unroll
+        for (int w = 0; w < VW; w += CH >= 8 ? 4 : 2) {
+          if constexpr (CH >= 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + w);
+            vr[j][w] = v.x; vr[j][w + 1] = v.y; vr[j][w + 2] = v.z; vr[j][w + 3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(row + w);
+            vr[j][w] = v.x; vr[j][w + 1] = v.y;
+          }
+        }
+      }
+    };
+    auto alive = [&](const Page& p) { return (uint32_t)__ballot((uint32_t)p.id < a.pages); };  // lanes l and l + 32 alike
+    bf16x8 qf[RT][KI];
+    auto load_q = [&](const Cursor& c) {
+      const int h0 = c.unit / a.RG * a.G + c.unit % a.RG * a.R, rows = unit_rows(a, c.unit);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int row = 16 * r + r16;
+        const uint16_t* src = a.q + c.b * a.q_sb + (h0 + min(row, rows - 1)) * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+          const int e = 8 * (g + 4 * i);
+          const bool in = row < rows && (!PAD || e < a.D);
+          const uint4 v = ldg16(src + (!PAD || e < a.D ? e : 0));
+          qf[r][i] = __builtin_bit_cast(bf16x8, in ? v : make_uint4(0, 0, 0, 0));
+        }
+      }
+    };
+
+    Cursor nx = cur;
+    Page pc = page_of(cur), pn{-1, 0};
+    if (n > 1) {
+      advance(a, nx, units);
+      pn = page_of(nx);
+    }
+    load_q(cur);
+    load_k(cur, pc);
+    load_v(cur, pc);
+    live = alive(pc);
+    acc.clear();
+    bool begun = cur.tile == 0;  // acc holds its unit from the first tile on
+    for (int64_t i = 0;; ++i) {
+      Cursor n2 = nx;
+      Page p2{-1, 0};
+      if (i + 2 < n) {
+        advance(a, n2, units);
+        p2 = page_of(n2);
+      }
+      // logits
+      floatx4 s[RT][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          s[r][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < KI; ++t) {
+            uint4 kv = kr[h][t];
+            if (PAD && 8 * (g + 4 * t) >= a.D) kv = make_uint4(0, 0, 0, 0);
+            s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv), qf[r][t], s[r][h], 0, 0, 0);
+          }
+        }
+      if (i + 1 < n) load_k(nx, pn);
+      const bool whole = live == 0xffffffffu;
+      bf16x8 ph[RT], pl[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = s[r][j >> 2][j & 3] * a.scale_log2;
+          if (!whole && !(live >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1)) x[j] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        mx = fmaxf(mx, live ? kFew : kNone);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        // rescaled only where a row's maximum grew by 2^8 (weights up to 2^8 lose nothing)
+        if (__any(mx > acc.m[r] + 8.f)) {
+          const float mn = fmaxf(acc.m[r], mx);
+          acc.scale(r, exp2f(acc.m[r] - mn));
+          acc.m[r] = mn;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p0 = exp2f(x[2 * j] - acc.m[r]), p1 = exp2f(x[2 * j + 1] - acc.m[r]);
+          acc.l[r] += p0 + p1;
+          const uint32_t b0 = __float_as_uint(p0) & 0xffff0000u, b1 = __float_as_uint(p1) & 0xffff0000u;
+          hi[j] = b0 >> 16 | b1;
+          lo[j] = pack_bf16(p0 - __uint_as_float(b0), p1 - __uint_as_float(b1));
+        }
+        ph[r] = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        pl[r] = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+      }
+      if (!whole) {  // a weight of zero times whatever lies there has to be zero
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(live >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1))
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[j][w] = 0;
+      }
+#pragma unroll
+      for (int d = 0; d < CH; ++d) {
+        uint32_t f[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          f[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d >> 1], vr[2 * t][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3]));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          acc.o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[r], acc.o[r][d], 0, 0, 0);
+          acc.o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[r], acc.o[r][d], 0, 0, 0);
+        }
+      }
+      const bool end = cur.tile + 1 == cur.nt;  // of the unit
+      if (i + 1 < n) {
+        load_v(nx, pn);
+        live = alive(pn);
+        if (end) load_q(nx);
+      }
+      if (end || i + 1 == n) {
+        const int rows = unit_rows(a, cur.unit);
+        acc.total();
+        if (begun && end) {
+          acc.finish(unit_out(a, cur.b, cur.unit), rows, a.D, lane);
+        } else if (!begun) {
+          acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, rows, a.D, lane);
+          if (lane == 0) flags[wave] = end ? 3 : 1;
+        } else {
+          tail = true;
+        }
+        if (i + 1 == n) break;
+        acc.clear();
+        begun = true;
+      }
+      cur = nx;
+      nx = n2;
+      pn = p2;
+    }
+  }
+  __syncthreads();
+  // joins inside the block: a wave that began a unit takes what the waves after it left
+  const int64_t slot = (int64_t)blockIdx.x * 2;
+  auto take = [&](int w) { acc.take(lds + w * a.R * ld, ld, stat0 + w * a.R * 2, a.R, a.D, lane); };
+  if (tail) {
+    bool ended = false;
+    for (int w = wave + 1; w < WPB && !ended; ++w) {
+      take(w);
+      ended = uniform(flags[w]) == 3;
+    }
+    if (ended) acc.finish(unit_out(a, cur.b, cur.unit), unit_rows(a, cur.unit), a.D, lane);
+    else if constexpr (!UNIT) acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
+  }
+  if constexpr (!UNIT) {
+    if (wave == 0 && uniform(flags[0]) != 0) {  // a unit begun in an earlier block
+      acc.clear();
+      bool ended = false;
+      for (int w = 0; w < WPB && !ended && uniform(flags[w]) != 0; ++w) {
+        take(w);
+        ended = uniform(flags[w]) == 3;
+      }
+      acc.put(a.part + slot * a.R * a.D, a.D, a.stat + slot * a.R * 2, a.R, a.D, lane);
+    }
+  }
+}
+
+// The join between blocks: one block per unit and 64 groups of 4 outputs; its waves take the
+// parts of the blocks that share the unit in turns and meet in LDS.
+constexpr int kJoinWaves = 8;
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a, int64_t blocks, int wpb, int groups) {
+  __shared__ float4 so[kJoinWaves][64];
+  __shared__ float2 ss[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int units = a.Hkv * a.RG;
+  const int64_t u = blockIdx.x / groups;
+  const int b = (int)(u / units), unit = (int)(u % units);
+  const int len = uniform(seq_len(a, b)), nt = (len + kTile - 1) / kTile;
+  if (nt == 0) return;
+  int64_t all = 0, before = 0;
+  for (int i = lane; i < a.B; i += kWave) {
+    const int t = (seq_len(a, i) + kTile - 1) / kTile;
+    all += t;
+    before += i < b ? t : 0;
+  }
+  const int64_t tiles = uniform_l(wave_sum_l(all)) * units, t0 = uniform_l(wave_sum_l(before)) * units + (int64_t)unit * nt;
+  const int64_t run = tiles_per_wave(tiles, blocks * wpb) * wpb;
+  const int64_t first = t0 / run, last = (t0 + nt - 1) / run;
+  if (first == last) return;
+  const int rows = unit_rows(a, unit), dg = a.D / 4;
+  const int e = (int)(blockIdx.x % groups) * 64 + lane;  // (row, group of 4)
+  const int row = min(e / dg, rows - 1), d = e % dg * 4;
+  float m = kNone, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t i = first + wave; i <= last; i += kJoinWaves) {
+    const int64_t slot = i * 2 + (i == first ? 1 : 0);
+    const float2 s = *reinterpret_cast<const float2*>(a.stat + (slot * a.R + row) * 2);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (slot * a.R + row) * a.D + d);
+    const float mn = fmaxf(m, s.x), f = exp2f(m - mn), h = exp2f(s.x - mn);
+    m = mn;
+    l = fmaf(l, f, s.y * h);
+    o.x = fmaf(o.x, f, v.x * h);
+    o.y = fmaf(o.y, f, v.y * h);
+    o.z = fmaf(o.z, f, v.z * h);
+    o.w = fmaf(o.w, f, v.w * h);
+  }
+  so[wave][lane] = o;
+  ss[wave][lane] = make_float2(m, l);
+  __syncthreads();
+  if (wave != 0 || e >= rows * dg) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) {
+    const float2 s = ss[w][lane];
+    const float4 v = so[w][lane];
+    const float mn = fmaxf(m, s.x), f = exp2f(m - mn), h = exp2f(s.x - mn);
+    m = mn;
+    l = fmaf(l, f, s.y * h);
+    o.x = fmaf(o.x, f, v.x * h);
+    o.y = fmaf(o.y, f, v.y * h);
+    o.z = fmaf(o.z, f, v.z * h);
+    o.w = fmaf(o.w, f, v.w * h);
+  }
+  const float f = m == kNone ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(unit_out(a, b, unit) + (int64_t)row * a.D + d) =
+      make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
+}
+
+int64_t num_cus() {
+  static int64_t cache[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cache[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
+
+// How a call is split: head dim DP, RT blocks of 16 rows a unit, wpb waves a block, blocks of
+// the list form, and the workspace for what they share.
+struct AttnPlan {
+  int DP, RT, wpb, R, RG;
+  int64_t blocks;
+  size_t stat, bytes;
+};
+AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D) {
+  AttnPlan p;
+  const int64_t G = H / Hkv;
+  p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  p.RT = G <= 16 ? 1 : G <= 32 || p.DP == 256 ? 2 : 4;
+  p.R = (int)std::min<int64_t>(G, 16 * p.RT);
+  p.RG = (int)cdiv(G, p.R);
+  p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
+  p.blocks = num_cus();
+  p.stat = align_up((size_t)p.blocks * 2 * p.R * (size_t)D * 4, 256);
+  p.bytes = p.stat + align_up((size_t)p.blocks * 2 * p.R * 2 * 4, 256);
+  return p;
+}
+
+template <int DP, int RT, int WPB>
+void launch_attn(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
+  const size_t lds = (size_t)WPB * a.R * (DP + 4 + 2) * 4;
+  const bool pad = a.D != DP;
+#define ATTN(PAD_, UNIT_) \
+  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_><<<(unsigned)blocks, WPB * 64, lds, st>>>(a)
+  if (unit) {
+    if (pad) ATTN(true, true);
+    else ATTN(false, true);
+  } else {
+    if (pad) ATTN(true, false);
+    else ATTN(false, false);
+  }
+#undef ATTN
 }
 
 int check_cache(const char* fn, const void* kc, const void* vc, int64_t pages, int64_t Hkv, int64_t page, int64_t D,
@@ -140,7 +645,7 @@ extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_
 }
 
 extern "C" size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D) {
-  return B > 0 && H > 0 && Hkv > 0 && D > 0 ? 16 : 0;
+  return B > 0 && H > 0 && Hkv > 0 && D > 0 && H % Hkv == 0 ? attn_plan(H, Hkv, D).bytes : 0;
 }
 
 extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
@@ -152,21 +657,71 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   if (int rc = check_cache("paged_attn", k_cache, v_cache, pages, Hkv, page, D, kc_strides, vc_strides)) return rc;
   TB_CHECK(H % Hkv == 0, "paged_attn: query heads must be a multiple of key/value heads");
   TB_CHECK(D <= 256, "paged_attn: head dim must be at most 256");
-  TB_CHECK(B * H < (int64_t)1 << 31 && max_pages >= 0 && max_pages < (int64_t)1 << 31, "paged_attn: shape too large");
+  TB_CHECK(max_pages >= 0 && max_pages < (int64_t)1 << 31, "paged_attn: table too wide");
   TB_CHECK(aligned16(q) && aligned16(o) && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
            "paged_attn: q must have 16-byte aligned rows");
   TB_CHECK(aligned4(table) && aligned4(lengths), "paged_attn: table and lengths must be 4-byte aligned");
   if (B == 0) return 0;
   TB_CHECK(aligned16(ws) && ws != nullptr, "paged_attn: workspace missing or misaligned");
-  if (ws_bytes < (int64_t)tbf16_paged_attn_ws_bytes(B, H, Hkv, D)) {
-    set_error("paged_attn: workspace too small");
+  const AttnPlan p = attn_plan(H, Hkv, D);
+  TB_CHECK(B * Hkv * p.RG * cdiv(p.R * D, 256) < (int64_t)1 << 31, "paged_attn: shape too large");
+  if (ws_bytes < (int64_t)p.bytes) {
+    set_error("paged_attn: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, p.bytes);
     return TBF16_EWS;
   }
-  paged_attn_kernel<<<(unsigned)(B * H), 256, 0, as_stream(stream)>>>(
-      (const uint16_t*)q, q_strides[0], q_strides[1], (const uint16_t*)k_cache, (const uint16_t*)v_cache,
-      CacheGeom{kc_strides[0], kc_strides[1], kc_strides[2]}, CacheGeom{vc_strides[0], vc_strides[1], vc_strides[2]}, pages,
-      (int)page, table, table_stride, (int)max_pages, lengths, scale * 1.4426950408889634f, (int)H, (int)(H / Hkv), (int)D,
-      (uint16_t*)o);
+  AttnArgs a;
+  a.q = (const uint16_t*)q;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.q_sb = q_strides[0];
+  a.q_sh = q_strides[1];
+  a.kg = CacheGeom{kc_strides[0], kc_strides[1], kc_strides[2]};
+  a.vg = CacheGeom{vc_strides[0], vc_strides[1], vc_strides[2]};
+  a.table = table;
+  a.lengths = lengths;
+  a.t_sb = table_stride;
+  a.cap = pages == 0 ? 0 : std::min<int64_t>(max_pages * page, ((int64_t)1 << 31) - 64);
+  a.pages = (uint32_t)pages;
+  a.page = (uint32_t)page;
+  // page <= 2^l: magic = ceil(2^(31 + l) / page) is off by less than 2^l / page of 2^-31
+  int l = 0;
+  while (((int64_t)1 << l) < page) ++l;
+  a.magic = (uint32_t)((((uint64_t)1 << (31 + l)) + page - 1) / page);
+  a.shift = 31 + l;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.B = (int)B;
+  a.H = (int)H;
+  a.Hkv = (int)Hkv;
+  a.G = (int)(H / Hkv);
+  a.D = (int)D;
+  a.R = p.R;
+  a.RG = p.RG;
+  a.o = (uint16_t*)o;
+  a.part = (float*)ws;
+  a.stat = (float*)((uint8_t*)ws + p.stat);
+  const hipStream_t st = as_stream(stream);
+  const int64_t units = B * Hkv * p.RG;
+  const bool unit = cdiv(a.cap, kTile) <= p.wpb * 4;
+  const int64_t blocks = unit ? units : p.blocks;
+#define ATTN(DP_, RT_, WPB_) launch_attn<DP_, RT_, WPB_>(a, unit, blocks, st)
+  if (p.DP == 64) {
+    if (p.RT == 1) ATTN(64, 1, 8);
+    else if (p.RT == 2) ATTN(64, 2, 4);
+    else ATTN(64, 4, 4);
+  } else if (p.DP == 128) {
+    if (p.RT == 1) ATTN(128, 1, 8);
+    else if (p.RT == 2) ATTN(128, 2, 4);
+    else ATTN(128, 4, 4);
+  } else {
+    if (p.RT == 1) ATTN(256, 1, 4);
+    else ATTN(256, 2, 4);
+  }
+#undef ATTN
   TB_LAUNCH_CHECK("paged_attn");
+  if (!unit) {
+    const int groups = (int)cdiv(p.R * D, 256);
+    paged_join_kernel<<<(unsigned)(units * groups), kJoinWaves * 64, 0, st>>>(a, blocks, p.wpb, groups);
+    TB_LAUNCH_CHECK("paged_attn join");
+  }
   return 0;
 }

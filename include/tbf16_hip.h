@@ -291,9 +291,10 @@ int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx, const void
  * element strides (t, h); k_cache, v_cache bf16 (pages, Hkv, page, D), element strides
  * (page, head, row), no two elements at one address; D contiguous, everything 16-byte aligned. No counterpart in the
  * reference, which has no cache. */
-int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int64_t D, const int64_t* k_strides,
-                      const int64_t* v_strides, const int32_t* slots, void* k_cache, void* v_cache, int64_t pages,
-                      int64_t page, const int64_t* kc_strides, const int64_t* vc_strides, void* stream);
+int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int64_t D, int64_t k_st, int64_t k_sh,
+                      int64_t v_st, int64_t v_sh, const int32_t* slots, void* k_cache, void* v_cache, int64_t pages,
+                      int64_t page, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh,
+                      int64_t vc_ss, void* stream);
 
 /* Attention of one new token per sequence over a paged cache: o[b, h] = softmax(scale q[b, h] .
  * k_j) v_j over positions j < lengths[b], position j in page table[b, j / page], row j % page,
@@ -302,13 +303,15 @@ int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int6
  * out; a sequence with none gives zeros. q bf16 (B, H, D), element strides (b, h); caches as tbf16_paged_write's
  * (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row stride
  * table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. ws:
- * tbf16_paged_attn_ws_bytes(B, H, Hkv, D) bytes, 16-byte aligned, for this call alone until
+ * tbf16_paged_attn_ws_bytes(H, Hkv, D, max_pages * page) bytes (asked with the stream's device
+ * current; 0 for short caches, ws may then be NULL), 16-byte aligned, this call's alone until
  * it has run. Serves the calls the reference leaves to torch (tbf16/convert.py:29-30). */
-size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D);
-int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
-                     const void* k_cache, const void* v_cache, int64_t pages, int64_t page, const int64_t* kc_strides,
-                     const int64_t* vc_strides, const int32_t* table, int64_t table_stride, int64_t max_pages,
-                     const int32_t* lengths, float scale, void* o, void* ws, int64_t ws_bytes, void* stream);
+size_t tbf16_paged_attn_ws_bytes(int64_t H, int64_t Hkv, int64_t D, int64_t positions);
+int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
+                     const void* k_cache, const void* v_cache, int64_t pages, int64_t page, int64_t kc_sp, int64_t kc_sh,
+                     int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, const int32_t* table,
+                     int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale, void* o, void* ws,
+                     int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -73,6 +73,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 32;
+#ifndef BLOCKS_MUL
+#define BLOCKS_MUL 1
+#endif
 // Running maxima start at kNone; a unit that had any key ends at kFew or above.
 constexpr float kNone = -FLT_MAX, kFew = -3.0e38f;
 
@@ -81,37 +84,19 @@ struct AttnArgs {
   int64_t q_sb, q_sh;
   CacheGeom kg, vg;
   const int32_t *table, *lengths;
-  int64_t t_sb, cap;  // positions a table row covers
+  int64_t t_sb;
+  int cap;  // positions a table row covers
   uint32_t pages, page, magic, shift;  // j / page = (j magic) >> shift for j < 2^31
   float scale_log2;
   int B, H, Hkv, G, D, R, RG;  // R rows a unit, RG units a key/value head
   uint16_t* o;
-  float *part, *stat;  // [block][2][R][D], [block][2][R][2]
+  float *part, *stat;  // [block][2][R][D], [block][2][R][2]: what a block leaves of units it shares
+  int4* desc;  // [block]: the unit it began and later blocks end (b, unit, last block, 1) or (.., 0)
 };
 
-__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
-  return (int)min<int64_t>(max(a.lengths[b], 0), a.cap);
-}
-__device__ __forceinline__ int64_t wave_sum_l(int64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, kWave);
-  return v;
-}
+__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.cap); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform_l(int64_t v) {
-  return (int64_t)(uint32_t)uniform((int)v) | (int64_t)uniform((int)(v >> 32)) << 32;
-}
-// Tiles of the whole batch, per unit of a sequence.
-__device__ __forceinline__ int64_t batch_tiles(const AttnArgs& a, int lane) {
-  int64_t n = 0;
-  for (int b = lane; b < a.B; b += kWave) n += (seq_len(a, b) + kTile - 1) / kTile;
-  return uniform_l(wave_sum_l(n));
-}
-// The list's split: tiles per wave, at least kMinTiles.
-constexpr int kMinTiles = 2;
-__device__ __forceinline__ int64_t tiles_per_wave(int64_t tiles, int64_t waves) {
-  return max<int64_t>(kMinTiles, (tiles + waves - 1) / waves);
-}
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A place in the list.
 struct Cursor {
@@ -129,33 +114,56 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Cursor& c, int units)
   ++c.b;
   enter(a, c);
 }
-// Tile t of the list.
-__device__ __forceinline__ Cursor locate(const AttnArgs& a, int64_t t, int units, int lane) {
-  Cursor c{0, 0, 0, 0, 0};
-  for (int b0 = 0;; b0 += kWave) {
-    const int b = b0 + lane;
-    const int64_t n = b < a.B ? (int64_t)((seq_len(a, b) + kTile - 1) / kTile) * units : 0;
-    int64_t up = n;  // inclusive prefix sums
+// The list's split into runs of c tiles, at least kMinTiles, run w from tile w c on (the host
+// has made sure that 32 bits count its tiles), and run w's length n and first place.
+constexpr int kMinTiles = 2;
+struct Run {
+  uint32_t c;
+  int n;
+  Cursor at;
+};
+__device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t w, uint32_t waves, int units, int lane) {
+  auto tiles = [&](int b) { return b < a.B ? (uint32_t)((seq_len(a, b) + kTile - 1) / kTile * units) : 0u; };
+  auto prefix = [&](uint32_t v) {  // inclusive
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
-      const int64_t v = __shfl_up((long long)up, o, kWave);
-      if (lane >= o) up += v;
+      const uint32_t u = __shfl_up((int)v, o, kWave);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  const uint32_t n0 = tiles(lane), up0 = prefix(n0);
+  uint32_t all = uniform(__shfl((int)up0, kWave - 1, kWave));
+  if (a.B > kWave) {
+    uint32_t more = 0;
+    for (int b = lane + kWave; b < a.B; b += kWave) more += tiles(b);
+    all += uniform(__shfl((int)prefix(more), kWave - 1, kWave));
+  }
+  Run r{max((uint32_t)kMinTiles, (all + waves - 1) / waves), 0, {0, 0, 0, 0, 0}};
+  const uint64_t first = (uint64_t)w * r.c;
+  if (first >= all) return r;
+  r.n = min(r.c, all - (uint32_t)first);
+  uint32_t t = (uint32_t)first, n = n0, up = up0;
+  for (int b0 = 0;; b0 += kWave) {
+    if (b0 > 0) {
+      n = tiles(b0 + lane);
+      up = prefix(n);
     }
     const uint64_t past = __ballot(up > t);
-    if (past == 0 && b0 + kWave < a.B) {
-      t -= uniform_l(__shfl((long long)up, kWave - 1, kWave));
+    if (past == 0) {
+      t -= uniform(__shfl((int)up, kWave - 1, kWave));
       continue;
     }
-    const int l = past ? __builtin_ctzll(past) : kWave - 1;
-    c.b = b0 + l;
-    t -= uniform_l(__shfl((long long)(up - n), l, kWave));
+    const int l = __builtin_ctzll(past);
+    r.at.b = b0 + l;
+    t -= uniform(__shfl((int)(up - n), l, kWave));
+    r.at.nt = uniform(__shfl((int)n, l, kWave)) / units;
     break;
   }
-  c.len = uniform(seq_len(a, c.b));
-  c.nt = (c.len + kTile - 1) / kTile;
-  c.unit = (int)(t / c.nt);
-  c.tile = (int)(t % c.nt);
-  return c;
+  r.at.len = uniform(seq_len(a, r.at.b));
+  r.at.unit = t / (uint32_t)r.at.nt;
+  r.at.tile = t % (uint32_t)r.at.nt;
+  return r;
 }
 
 // What a lane holds of a unit: for row l % 16 of each 16-row block, the maximum, its own
@@ -184,7 +192,7 @@ struct Acc {
 #pragma unroll
     for (int r = 0; r < RT; ++r) l[r] = sum_xor32(sum_xor16(l[r]));
   }
-  // put / take: rows of D floats at `rows` (stride ld), their (m, l) at `stat`
+  // rows of D floats at `rows` (stride ld), their (m, l) at `stat`
   __device__ __forceinline__ void put(float* rows, int ld, float* stat, int R, int D, int lane) const {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -202,29 +210,39 @@ struct Acc {
       if (lane < 16) *reinterpret_cast<float2*>(stat + 2 * row) = make_float2(m[r], l[r]);
     }
   }
-  __device__ __forceinline__ void take(const float* rows, int ld, const float* stat, int R, int D, int lane) {
+  // adds what n others put, part w at rows + w step and stat + w stat_step: the common maximum
+  // first, so that the parts' loads do not wait for each other
+  __device__ __forceinline__ void take(const float* rows, int step, int ld, const float* stat, int stat_step, int n, int R,
+                                       int D, int lane) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = 16 * r + (lane & 15);
       if (row >= R) continue;
-      const float2 s = *reinterpret_cast<const float2*>(stat + 2 * row);
-      const float mn = fmaxf(m[r], s.x), f = exp2f(s.x - mn);
-      scale(r, exp2f(m[r] - mn));
+      float mn = m[r];
+      for (int w = 0; w < n; ++w) mn = fmaxf(mn, stat[w * stat_step + 2 * row]);
+      scale(r, ex2(m[r] - mn));
       m[r] = mn;
-      l[r] = fmaf(f, s.y, l[r]);
+#pragma unroll 2
+      for (int w = 0; w < n; ++w) {
+        const float2 s = *reinterpret_cast<const float2*>(stat + w * stat_step + 2 * row);
+        const float f = ex2(s.x - mn);
+        l[r] = fmaf(f, s.y, l[r]);
+        float4 v[4][CH / 4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < CH; d += 4) {
-          const int at = CH * (4 * (lane >> 4) + i) + d;
-          if (at < D) {
-            const float4 v = *reinterpret_cast<const float4*>(rows + (int64_t)row * ld + at);
-            o[r][d][i] = fmaf(f, v.x, o[r][d][i]);
-            o[r][d + 1][i] = fmaf(f, v.y, o[r][d + 1][i]);
-            o[r][d + 2][i] = fmaf(f, v.z, o[r][d + 2][i]);
-            o[r][d + 3][i] = fmaf(f, v.w, o[r][d + 3][i]);
+          for (int d = 0; d < CH; d += 4)
+            v[i][d / 4] = *reinterpret_cast<const float4*>(rows + w * step + row * ld + CH * (4 * (lane >> 4) + i) + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < CH; d += 4) {
+            o[r][d][i] = fmaf(f, v[i][d / 4].x, o[r][d][i]);
+            o[r][d + 1][i] = fmaf(f, v[i][d / 4].y, o[r][d + 1][i]);
+            o[r][d + 2][i] = fmaf(f, v[i][d / 4].z, o[r][d + 2][i]);
+            o[r][d + 3][i] = fmaf(f, v[i][d / 4].w, o[r][d + 3][i]);
           }
-        }
+      }
     }
   }
   // the outputs: o points at the unit's first row
@@ -266,30 +284,22 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
   float* const stat0 = lds + WPB * a.R * ld;
 
   Cursor cur;
-  int64_t n;  // this wave's tiles
+  int n;  // this wave's tiles
+  uint32_t c = 0;
   if constexpr (UNIT) {
     cur.b = blockIdx.x / units;
     cur.unit = blockIdx.x % units;
     cur.len = uniform(seq_len(a, cur.b));
     cur.nt = (cur.len + kTile - 1) / kTile;
-    const int c = (cur.nt + WPB - 1) / WPB;
-    cur.tile = min(wave * c, cur.nt);
-    n = min(c, cur.nt - cur.tile);
-    if (cur.nt == 0) {
-      const int rows = unit_rows(a, cur.unit) * a.D / 8;
-      for (int i = threadIdx.x; i < rows; i += WPB * 64)
-        stg16(unit_out(a, cur.b, cur.unit) + 8 * i, make_uint4(0, 0, 0, 0));
-      return;
-    }
+    const int per = (cur.nt + WPB - 1) / WPB;
+    cur.tile = min(wave * per, cur.nt);
+    n = min(per, cur.nt - cur.tile);
   } else {
-    const int64_t tiles = batch_tiles(a, lane) * units, c = tiles_per_wave(tiles, (int64_t)gridDim.x * WPB);
-    const int64_t t0 = ((int64_t)blockIdx.x * WPB + wave) * c;
-    n = max<int64_t>(0, min(c, tiles - t0));
-    if (n > 0) cur = locate(a, t0, units, lane);
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
-      if (seq_len(a, b) == 0)
-        for (int i = threadIdx.x; i < a.H * a.D / 8; i += WPB * 64)
-          stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
+    const Run r = run_of(a, blockIdx.x * WPB + wave, gridDim.x * WPB, units, lane);
+    c = r.c;
+    n = r.n;
+    cur = r.at;
+    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   if (lane == 0) flags[wave] = 0;
 
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
     live = alive(pc);
     acc.clear();
     bool begun = cur.tile == 0;  // acc holds its unit from the first tile on
-    for (int64_t i = 0;; ++i) {
+    for (int i = 0;; ++i) {
       Cursor n2 = nx;
       Page p2{-1, 0};
       if (i + 2 < n) {
@@ -416,13 +426,13 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
         // rescaled only where a row's maximum grew by 2^8 (weights up to 2^8 lose nothing)
         if (__any(mx > acc.m[r] + 8.f)) {
           const float mn = fmaxf(acc.m[r], mx);
-          acc.scale(r, exp2f(acc.m[r] - mn));
+          acc.scale(r, ex2(acc.m[r] - mn));
           acc.m[r] = mn;
         }
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p0 = exp2f(x[2 * j] - acc.m[r]), p1 = exp2f(x[2 * j + 1] - acc.m[r]);
+          const float p0 = ex2(x[2 * j] - acc.m[r]), p1 = ex2(x[2 * j + 1] - acc.m[r]);
           acc.l[r] += p0 + p1;
           const uint32_t b0 = __float_as_uint(p0) & 0xffff0000u, b1 = __float_as_uint(p1) & 0xffff0000u;
           hi[j] = b0 >> 16 | b1;
@@ -478,88 +488,96 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
     }
   }
   __syncthreads();
-  // joins inside the block: a wave that began a unit takes what the waves after it left
+  // joins inside the block: a wave that began a unit takes what the waves after it left, the
+  // first wave what they left of a unit begun in an earlier block
   const int64_t slot = (int64_t)blockIdx.x * 2;
-  auto take = [&](int w) { acc.take(lds + w * a.R * ld, ld, stat0 + w * a.R * 2, a.R, a.D, lane); };
-  if (tail) {
-    bool ended = false;
-    for (int w = wave + 1; w < WPB && !ended; ++w) {
-      take(w);
-      ended = uniform(flags[w]) == 3;
+  int last;  // the last wave before the end of the unit that wave `from` - 1 goes on with, or of the block
+  auto span = [&](int from) {
+    for (last = from; last < WPB - 1 && uniform(flags[last]) == 1; ++last) {
     }
-    if (ended) acc.finish(unit_out(a, cur.b, cur.unit), unit_rows(a, cur.unit), a.D, lane);
-    else if constexpr (!UNIT) acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
+    return last < WPB && uniform(flags[last]) == 3;
+  };
+  auto take = [&](int from) {
+    acc.take(lds + from * a.R * ld, a.R * ld, ld, stat0 + from * a.R * 2, a.R * 2, last + 1 - from, a.R, a.D, lane);
+  };
+  if (tail) {
+    const bool ended = wave + 1 < WPB && span(wave + 1);
+    if (wave + 1 < WPB) take(wave + 1);
+    if (ended) {
+      acc.finish(unit_out(a, cur.b, cur.unit), unit_rows(a, cur.unit), a.D, lane);
+    } else if constexpr (!UNIT) {
+      acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
+      // the unit's last tile: this wave's last one is its tile cur.tile
+      const uint32_t end = (blockIdx.x * WPB + wave) * c + n - 1 - cur.tile + cur.nt - 1;
+      if (lane == 0) a.desc[blockIdx.x] = make_int4(cur.b, cur.unit, end / (c * WPB), 1);
+    }
   }
-  if constexpr (!UNIT) {
-    if (wave == 0 && uniform(flags[0]) != 0) {  // a unit begun in an earlier block
+  if constexpr (UNIT) {
+    if (cur.nt == 0) {  // a sequence without keys
+      const int chunks = unit_rows(a, cur.unit) * a.D / 8;
+      for (int i = threadIdx.x; i < chunks; i += WPB * 64)
+        stg16(unit_out(a, cur.b, cur.unit) + 8 * i, make_uint4(0, 0, 0, 0));
+    }
+  } else {
+    if (wave == 0 && uniform(flags[0]) != 0) {
       acc.clear();
-      bool ended = false;
-      for (int w = 0; w < WPB && !ended && uniform(flags[w]) != 0; ++w) {
-        take(w);
-        ended = uniform(flags[w]) == 3;
-      }
+      span(0);
+      take(0);
       acc.put(a.part + slot * a.R * a.D, a.D, a.stat + slot * a.R * 2, a.R, a.D, lane);
     }
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (uniform(seq_len(a, b)) == 0)
+        for (int i = threadIdx.x; i < a.H * a.D / 8; i += WPB * 64)
+          stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
   }
 }
 
-// The join between blocks: one block per unit and 64 groups of 4 outputs; its waves take the
-// parts of the blocks that share the unit in turns and meet in LDS.
+// The join between blocks: for the unit that block blockIdx.x of the list began and did not end,
+// 64 groups of 4 outputs a block; its waves take the parts in turns and meet in LDS.
 constexpr int kJoinWaves = 8;
-__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a, int64_t blocks, int wpb, int groups) {
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a) {
   __shared__ float4 so[kJoinWaves][64];
   __shared__ float2 ss[kJoinWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int units = a.Hkv * a.RG;
-  const int64_t u = blockIdx.x / groups;
-  const int b = (int)(u / units), unit = (int)(u % units);
-  const int len = uniform(seq_len(a, b)), nt = (len + kTile - 1) / kTile;
-  if (nt == 0) return;
-  int64_t all = 0, before = 0;
-  for (int i = lane; i < a.B; i += kWave) {
-    const int t = (seq_len(a, i) + kTile - 1) / kTile;
-    all += t;
-    before += i < b ? t : 0;
-  }
-  const int64_t tiles = uniform_l(wave_sum_l(all)) * units, t0 = uniform_l(wave_sum_l(before)) * units + (int64_t)unit * nt;
-  const int64_t run = tiles_per_wave(tiles, blocks * wpb) * wpb;
-  const int64_t first = t0 / run, last = (t0 + nt - 1) / run;
-  if (first == last) return;
-  const int rows = unit_rows(a, unit), dg = a.D / 4;
-  const int e = (int)(blockIdx.x % groups) * 64 + lane;  // (row, group of 4)
+  const int4 u = a.desc[blockIdx.x];
+  if (u.w == 0) return;
+  const int first = blockIdx.x, last = u.z, rows = unit_rows(a, u.y), dg = a.D / 4;
+  const int e = blockIdx.y * 64 + lane;  // (row, group of 4)
   const int row = min(e / dg, rows - 1), d = e % dg * 4;
   float m = kNone, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int64_t i = first + wave; i <= last; i += kJoinWaves) {
-    const int64_t slot = i * 2 + (i == first ? 1 : 0);
-    const float2 s = *reinterpret_cast<const float2*>(a.stat + (slot * a.R + row) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (slot * a.R + row) * a.D + d);
-    const float mn = fmaxf(m, s.x), f = exp2f(m - mn), h = exp2f(s.x - mn);
+  auto add = [&](float2 s, float4 v) {
+    const float mn = fmaxf(m, s.x), f = ex2(m - mn), h = ex2(s.x - mn);
     m = mn;
     l = fmaf(l, f, s.y * h);
     o.x = fmaf(o.x, f, v.x * h);
     o.y = fmaf(o.y, f, v.y * h);
     o.z = fmaf(o.z, f, v.z * h);
     o.w = fmaf(o.w, f, v.w * h);
+  };
+  constexpr int U = 4;  // parts in flight
+  for (int i0 = first + wave; i0 <= last; i0 += U * kJoinWaves) {
+    float2 s[U];
+    float4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = min(i0 + k * kJoinWaves, last);
+      const int64_t slot = (int64_t)i * 2 + (i == first ? 1 : 0);
+      s[k] = *reinterpret_cast<const float2*>(a.stat + (slot * a.R + row) * 2);
+      v[k] = *reinterpret_cast<const float4*>(a.part + (slot * a.R + row) * a.D + d);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (i0 + k * kJoinWaves <= last) add(s[k], v[k]);
   }
   so[wave][lane] = o;
   ss[wave][lane] = make_float2(m, l);
   __syncthreads();
   if (wave != 0 || e >= rows * dg) return;
 #pragma unroll
-  for (int w = 1; w < kJoinWaves; ++w) {
-    const float2 s = ss[w][lane];
-    const float4 v = so[w][lane];
-    const float mn = fmaxf(m, s.x), f = exp2f(m - mn), h = exp2f(s.x - mn);
-    m = mn;
-    l = fmaf(l, f, s.y * h);
-    o.x = fmaf(o.x, f, v.x * h);
-    o.y = fmaf(o.y, f, v.y * h);
-    o.z = fmaf(o.z, f, v.z * h);
-    o.w = fmaf(o.w, f, v.w * h);
-  }
+  for (int w = 1; w < kJoinWaves; ++w) add(ss[w][lane], so[w][lane]);
   const float f = m == kNone ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(unit_out(a, b, unit) + (int64_t)row * a.D + d) =
+  *reinterpret_cast<uint2*>(unit_out(a, u.x, u.y) + (int64_t)row * a.D + d) =
       make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
 }
 
@@ -579,20 +597,26 @@ int64_t num_cus() {
 // the list form, and the workspace for what they share.
 struct AttnPlan {
   int DP, RT, wpb, R, RG;
+  bool unit;  // one block per unit, nothing shared
   int64_t blocks;
-  size_t stat, bytes;
+  size_t stat, desc, bytes;
 };
-AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D) {
+AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   AttnPlan p;
   const int64_t G = H / Hkv;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  p.RT = G <= 16 ? 1 : G <= 32 || p.DP == 256 ? 2 : 4;
+  p.RT = G <= 16 || p.DP == 256 ? 1 : G <= 32 || p.DP == 128 ? 2 : 4;
   p.R = (int)std::min<int64_t>(G, 16 * p.RT);
   p.RG = (int)cdiv(G, p.R);
   p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
-  p.blocks = num_cus();
+  p.unit = cdiv(cap, kTile) <= p.wpb * 4;
+  p.stat = p.desc = p.bytes = 0;
+  p.blocks = 0;
+  if (p.unit) return p;
+  p.blocks = num_cus() * (8 / p.wpb) * BLOCKS_MUL;
   p.stat = align_up((size_t)p.blocks * 2 * p.R * (size_t)D * 4, 256);
-  p.bytes = p.stat + align_up((size_t)p.blocks * 2 * p.R * 2 * 4, 256);
+  p.desc = p.stat + align_up((size_t)p.blocks * 2 * p.R * 2 * 4, 256);
+  p.bytes = p.desc + align_up((size_t)p.blocks * 16, 256);
   return p;
 }
 
@@ -613,58 +637,59 @@ void launch_attn(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
 }
 
 int check_cache(const char* fn, const void* kc, const void* vc, int64_t pages, int64_t Hkv, int64_t page, int64_t D,
-                const int64_t* ks, const int64_t* vs) {
+                const CacheGeom& kg, const CacheGeom& vg) {
   TB_CHECK(pages >= 0 && Hkv > 0 && page > 0 && D > 0, "%s: bad cache shape", fn);
   TB_CHECK(pages < (int64_t)1 << 31 && page < (int64_t)1 << 31 && Hkv < (int64_t)1 << 20, "%s: cache too large", fn);
   TB_CHECK(D % 8 == 0, "%s: head dim must be a multiple of 8", fn);
   TB_CHECK(aligned16(kc) && aligned16(vc), "%s: cache must be 16-byte aligned", fn);
-  for (int i = 0; i < 3; ++i)
-    TB_CHECK(ks[i] % 8 == 0 && vs[i] % 8 == 0 && ks[i] >= 0 && vs[i] >= 0 && ks[i] < (int64_t)1 << 31 && vs[i] < (int64_t)1 << 31,
-             "%s: cache strides must be multiples of 8 below 2^31", fn);
+  for (const int64_t s : {kg.sp, kg.sh, kg.ss, vg.sp, vg.sh, vg.ss})
+    TB_CHECK(s % 8 == 0 && s >= 0 && s < (int64_t)1 << 31, "%s: cache strides must be multiples of 8 below 2^31", fn);
   return 0;
 }
 
 }  // namespace
 
-extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int64_t D, const int64_t* k_strides,
-                                 const int64_t* v_strides, const int32_t* slots, void* k_cache, void* v_cache,
-                                 int64_t pages, int64_t page, const int64_t* kc_strides, const int64_t* vc_strides,
-                                 void* stream) {
-  if (int rc = check_cache("paged_write", k_cache, v_cache, pages, Hkv, page, D, kc_strides, vc_strides)) return rc;
+extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int64_t D, int64_t k_st,
+                                 int64_t k_sh, int64_t v_st, int64_t v_sh, const int32_t* slots, void* k_cache,
+                                 void* v_cache, int64_t pages, int64_t page, int64_t kc_sp, int64_t kc_sh, int64_t kc_ss,
+                                 int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, void* stream) {
+  const CacheGeom kg{kc_sp, kc_sh, kc_ss}, vg{vc_sp, vc_sh, vc_ss};
+  if (int rc = check_cache("paged_write", k_cache, v_cache, pages, Hkv, page, D, kg, vg)) return rc;
   TB_CHECK(T >= 0 && T < (int64_t)1 << 31, "paged_write: bad number of tokens");
   TB_CHECK(aligned16(k) && aligned16(v) && aligned4(slots), "paged_write: k and v must be 16-byte aligned");
-  for (int i = 0; i < 2; ++i)
-    TB_CHECK(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0, "paged_write: strides must be multiples of 8");
+  TB_CHECK(k_st % 8 == 0 && k_sh % 8 == 0 && v_st % 8 == 0 && v_sh % 8 == 0, "paged_write: strides must be multiples of 8");
   if (T == 0 || pages == 0) return 0;
   paged_write_kernel<<<(unsigned)cdiv(T, 4), 256, 0, as_stream(stream)>>>(
-      (const uint16_t*)k, (const uint16_t*)v, k_strides[0], k_strides[1], v_strides[0], v_strides[1], slots, (int)T,
-      (int)Hkv, (int)(D / 8), (uint16_t*)k_cache, (uint16_t*)v_cache, CacheGeom{kc_strides[0], kc_strides[1], kc_strides[2]},
-      CacheGeom{vc_strides[0], vc_strides[1], vc_strides[2]}, pages * page, (int)page);
+      (const uint16_t*)k, (const uint16_t*)v, k_st, k_sh, v_st, v_sh, slots, (int)T, (int)Hkv, (int)(D / 8),
+      (uint16_t*)k_cache, (uint16_t*)v_cache, kg, vg, pages * page, (int)page);
   TB_LAUNCH_CHECK("paged_write");
   return 0;
 }
 
-extern "C" size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D) {
-  return B > 0 && H > 0 && Hkv > 0 && D > 0 && H % Hkv == 0 ? attn_plan(H, Hkv, D).bytes : 0;
+extern "C" size_t tbf16_paged_attn_ws_bytes(int64_t H, int64_t Hkv, int64_t D, int64_t positions) {
+  return H > 0 && Hkv > 0 && D > 0 && H % Hkv == 0 ? attn_plan(H, Hkv, D, positions).bytes : 0;
 }
 
-extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
-                                const void* k_cache, const void* v_cache, int64_t pages, int64_t page,
-                                const int64_t* kc_strides, const int64_t* vc_strides, const int32_t* table,
-                                int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale, void* o,
-                                void* ws, int64_t ws_bytes, void* stream) {
+extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
+                                const void* k_cache, const void* v_cache, int64_t pages, int64_t page, int64_t kc_sp,
+                                int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss,
+                                const int32_t* table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                float scale, void* o, void* ws, int64_t ws_bytes, void* stream) {
+  const CacheGeom kg{kc_sp, kc_sh, kc_ss}, vg{vc_sp, vc_sh, vc_ss};
   TB_CHECK(B >= 0 && H > 0, "paged_attn: bad shape");
-  if (int rc = check_cache("paged_attn", k_cache, v_cache, pages, Hkv, page, D, kc_strides, vc_strides)) return rc;
+  if (int rc = check_cache("paged_attn", k_cache, v_cache, pages, Hkv, page, D, kg, vg)) return rc;
   TB_CHECK(H % Hkv == 0, "paged_attn: query heads must be a multiple of key/value heads");
   TB_CHECK(D <= 256, "paged_attn: head dim must be at most 256");
   TB_CHECK(max_pages >= 0 && max_pages < (int64_t)1 << 31, "paged_attn: table too wide");
-  TB_CHECK(aligned16(q) && aligned16(o) && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
+  TB_CHECK(aligned16(q) && aligned16(o) && q_sb % 8 == 0 && q_sh % 8 == 0,
            "paged_attn: q must have 16-byte aligned rows");
   TB_CHECK(aligned4(table) && aligned4(lengths), "paged_attn: table and lengths must be 4-byte aligned");
   if (B == 0) return 0;
-  TB_CHECK(aligned16(ws) && ws != nullptr, "paged_attn: workspace missing or misaligned");
-  const AttnPlan p = attn_plan(H, Hkv, D);
-  TB_CHECK(B * Hkv * p.RG * cdiv(p.R * D, 256) < (int64_t)1 << 31, "paged_attn: shape too large");
+  const AttnPlan p = attn_plan(H, Hkv, D, max_pages * page);
+  TB_CHECK(aligned16(ws) && (ws != nullptr || p.bytes == 0), "paged_attn: workspace missing or misaligned");
+  TB_CHECK(B < (int64_t)1 << 31 && B * Hkv * p.RG < (int64_t)1 << 31 &&
+               (double)(B * Hkv * p.RG) * (double)cdiv(std::min<int64_t>(max_pages * page, (int64_t)1 << 31), kTile) < 2e9,
+           "paged_attn: shape too large");
   if (ws_bytes < (int64_t)p.bytes) {
     set_error("paged_attn: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, p.bytes);
     return TBF16_EWS;
@@ -673,14 +698,14 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   a.q = (const uint16_t*)q;
   a.kc = (const uint16_t*)k_cache;
   a.vc = (const uint16_t*)v_cache;
-  a.q_sb = q_strides[0];
-  a.q_sh = q_strides[1];
-  a.kg = CacheGeom{kc_strides[0], kc_strides[1], kc_strides[2]};
-  a.vg = CacheGeom{vc_strides[0], vc_strides[1], vc_strides[2]};
+  a.q_sb = q_sb;
+  a.q_sh = q_sh;
+  a.kg = kg;
+  a.vg = vg;
   a.table = table;
   a.lengths = lengths;
   a.t_sb = table_stride;
-  a.cap = pages == 0 ? 0 : std::min<int64_t>(max_pages * page, ((int64_t)1 << 31) - 64);
+  a.cap = pages == 0 ? 0 : (int)std::min<int64_t>(max_pages * page, ((int64_t)1 << 31) - 64);
   a.pages = (uint32_t)pages;
   a.page = (uint32_t)page;
   // page <= 2^l: magic = ceil(2^(31 + l) / page) is off by less than 2^l / page of 2^-31
@@ -699,28 +724,25 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   a.o = (uint16_t*)o;
   a.part = (float*)ws;
   a.stat = (float*)((uint8_t*)ws + p.stat);
+  a.desc = (int4*)((uint8_t*)ws + p.desc);
   const hipStream_t st = as_stream(stream);
   const int64_t units = B * Hkv * p.RG;
-  const bool unit = cdiv(a.cap, kTile) <= p.wpb * 4;
-  const int64_t blocks = unit ? units : p.blocks;
-#define ATTN(DP_, RT_, WPB_) launch_attn<DP_, RT_, WPB_>(a, unit, blocks, st)
+  const int64_t blocks = p.unit ? units : p.blocks;
+#define ATTN(DP_, RT_, WPB_) launch_attn<DP_, RT_, WPB_>(a, p.unit, blocks, st)
   if (p.DP == 64) {
     if (p.RT == 1) ATTN(64, 1, 8);
     else if (p.RT == 2) ATTN(64, 2, 4);
     else ATTN(64, 4, 4);
   } else if (p.DP == 128) {
     if (p.RT == 1) ATTN(128, 1, 8);
-    else if (p.RT == 2) ATTN(128, 2, 4);
-    else ATTN(128, 4, 4);
+    else ATTN(128, 2, 4);
   } else {
-    if (p.RT == 1) ATTN(256, 1, 4);
-    else ATTN(256, 2, 4);
+    ATTN(256, 1, 4);
   }
 #undef ATTN
   TB_LAUNCH_CHECK("paged_attn");
-  if (!unit) {
-    const int groups = (int)cdiv(p.R * D, 256);
-    paged_join_kernel<<<(unsigned)(units * groups), kJoinWaves * 64, 0, st>>>(a, blocks, p.wpb, groups);
+  if (!p.unit) {
+    paged_join_kernel<<<dim3((unsigned)blocks, (unsigned)cdiv(p.R * D, 256)), kJoinWaves * 64, 0, st>>>(a);
     TB_LAUNCH_CHECK("paged_attn join");
   }
   return 0;

@@ -19,45 +19,42 @@ power-of-two scales are needed and any bf16 magnitude is taken.
 """
 from __future__ import annotations
 
-import ctypes
-import math
-
 import torch
 
-from ._ext import launch, lib, ptr
+from ._ext import launch, lib
 
 MAX_HEAD_DIM = 256
 
 
-def _strides(t, n) -> ctypes.Array:
-    return (ctypes.c_int64 * n)(*t.stride()[:n])
-
-
-def _rows_ok(t) -> bool:
-    """Contiguous, 16-byte aligned rows along the last dimension."""
-    *outer, last = t.stride()
-    return last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in outer)
-
-
-def _check_cache(fn, k_cache, v_cache, *others):
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+def _cache(fn, k_cache, v_cache, *others):
+    """(shape, k_cache's strides, v_cache's) of a cache the kernels take, on the device of
+    `others` too; raises for any other."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"tbf16.{fn}: expected k_cache and v_cache of one shape (pages, Hkv, page, D), got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    _, Hkv, page, D = k_cache.shape
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
+    _, Hkv, page, D = shape
     if D % 8 or not 0 < D <= MAX_HEAD_DIM:
         raise ValueError(f"tbf16.{fn}: head dim {D} is not a multiple of 8 up to {MAX_HEAD_DIM}")
     if Hkv == 0 or page == 0:
-        raise ValueError(f"tbf16.{fn}: cache of shape {tuple(k_cache.shape)} holds nothing")
+        raise ValueError(f"tbf16.{fn}: cache of shape {tuple(shape)} holds nothing")
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise TypeError(f"tbf16.{fn}: expected a bf16 cache")
-    if not (_rows_ok(k_cache) and _rows_ok(v_cache)):
+    k_st, v_st = k_cache.stride(), v_cache.stride()
+    if (k_st[3] != 1 or v_st[3] != 1 or (k_st[0] | k_st[1] | k_st[2] | v_st[0] | v_st[1] | v_st[2]) & 7
+            or (k_cache.data_ptr() | v_cache.data_ptr()) & 15):
         raise ValueError(f"tbf16.{fn}: cache rows must be contiguous and 16-byte aligned (strides multiples of 8)")
-    dev = k_cache.device
-    if dev.type != "cuda":
+    _same_device(fn, k_cache, v_cache, *others)
+    return shape, k_st, v_st
+
+
+def _same_device(fn, first, *others):
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("tbf16: expected tensors on a ROCm (cuda) device")
-    for t in (v_cache, *others):
-        if t.device != dev:
-            raise ValueError(f"tbf16.{fn}: tensors on {t.device} and {dev}")
+    for t in others:
+        if t.get_device() != dev:
+            raise ValueError(f"tbf16.{fn}: tensors on {t.device} and {first.device}")
 
 
 def _index(fn, name, t, dim):
@@ -66,38 +63,65 @@ def _index(fn, name, t, dim):
     return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
 
 
+def _rows(t):
+    """(t, its strides) with contiguous, 16-byte aligned rows of its last of three dimensions: t
+    itself or a copy."""
+    st = t.stride()
+    if st[2] == 1 and not (st[0] | st[1]) & 7 and not t.data_ptr() & 15:
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
+
+
 def paged_write(k_cache, v_cache, k, v, slots) -> None:
     """k_cache[s // page, :, s % page] = k[t], v_cache likewise, for s = slots[t] of every
     token t. k, v bf16 (T, Hkv, D), any strides; slots int32 (T,). Slots outside the cache
     (negative: a padded batch) leave it as it is; where slots repeat, the last token's rows
     stay. In place; k and v must not lie in the cache's own storage."""
-    _check_cache("paged_write", k_cache, v_cache, k, v, slots)
-    pages, Hkv, page, D = k_cache.shape
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (Hkv, D):
-        raise ValueError(f"tbf16.paged_write: k {tuple(k.shape)} and v {tuple(v.shape)} are not (T, {Hkv}, {D})")
+    (pages, Hkv, page, D), kc_st, vc_st = _cache("paged_write", k_cache, v_cache, k, v, slots)
+    shape = k.shape
+    T = shape[0] if len(shape) else 0
+    if v.shape != shape or shape != (T, Hkv, D):
+        raise ValueError(f"tbf16.paged_write: k {tuple(shape)} and v {tuple(v.shape)} are not (T, {Hkv}, {D})")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise TypeError("tbf16.paged_write: expected bf16 k and v")
     slots = _index("paged_write", "slots", slots, 1)
-    T = k.shape[0]
     if slots.shape[0] != T:
         raise ValueError(f"tbf16.paged_write: {slots.shape[0]} slots for {T} tokens")
     if pages * page >= 2 ** 31:
         raise ValueError("tbf16.paged_write: the cache has more slots than int32 counts")
-    for c in (k_cache, v_cache):
-        if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
-            raise ValueError("tbf16.paged_write: the cache is an expanded view")
-    if k_cache.data_ptr() == v_cache.data_ptr() and pages:
+    if 0 in kc_st or 0 in vc_st:
+        for c in (k_cache, v_cache):
+            if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+                raise ValueError("tbf16.paged_write: the cache is an expanded view")
+    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+    if kc == vc and pages:
         raise ValueError("tbf16.paged_write: k_cache and v_cache are the same memory")
-    held = {c.untyped_storage().data_ptr() for c in (k_cache, v_cache)}
+    held = k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr()
     if T and (k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held):
         raise ValueError("tbf16.paged_write: k and v lie in the cache's storage")
     torch.autograd.graph.increment_version((k_cache, v_cache))
     if T == 0 or pages == 0:
         return
-    k, v = (t if _rows_ok(t) else t.contiguous() for t in (k, v))
-    k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (k, v))
-    launch("tbf16_paged_write", k_cache, ptr(k), ptr(v), T, Hkv, D, _strides(k, 2), _strides(v, 2), ptr(slots),
-           ptr(k_cache), ptr(v_cache), pages, page, _strides(k_cache, 3), _strides(v_cache, 3))
+    (k, k_st), (v, v_st) = _rows(k), _rows(v)
+    launch("tbf16_paged_write", k_cache, k.data_ptr(), v.data_ptr(), T, Hkv, D, k_st[0], k_st[1], v_st[0], v_st[1],
+           slots.data_ptr(), kc, vc, pages, page, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
+
+
+# tbf16_paged_attn's workspace bytes per (device, H, Hkv, D, positions a table row covers): its
+# blocks are counted by the device's CUs, so it is asked on the tensors' device, once
+_WS_BYTES: dict = {}
+
+
+def _ws_bytes(dev: int, H: int, Hkv: int, D: int, cap: int) -> int:
+    key = (dev, H, Hkv, D, cap)
+    n = _WS_BYTES.get(key)
+    if n is None:
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        with torch.cuda.device(dev):
+            n = _WS_BYTES[key] = int(lib().tbf16_paged_attn_ws_bytes(H, Hkv, D, cap))
+    return n
 
 
 def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
@@ -108,28 +132,27 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     gives zeros. Entries of page_table outside [0, pages) hold no keys: their positions are
     left out. scale: 1 / sqrt(D) if None. Logits, softmax statistics and sums in fp32, one
     rounding to bf16."""
-    _check_cache("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
-    pages, Hkv, page, D = k_cache.shape
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"tbf16.paged_sdpa: q {tuple(q.shape)} is not (B, H, {D})")
+    (pages, Hkv, page, D), k_st, v_st = _cache("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"tbf16.paged_sdpa: q {tuple(shape)} is not (B, H, {D})")
     if q.dtype != torch.bfloat16:
         raise TypeError("tbf16.paged_sdpa: expected bf16 q")
-    B, H, _ = q.shape
+    B, H, _ = shape
     if H == 0 or H % Hkv:
         raise ValueError(f"tbf16.paged_sdpa: {H} query heads over {Hkv} key/value heads")
     page_table = _index("paged_sdpa", "page_table", page_table, 2)
     lengths = _index("paged_sdpa", "lengths", lengths, 1)
-    if page_table.shape[0] != B or lengths.shape[0] != B:
-        raise ValueError(f"tbf16.paged_sdpa: page_table for {page_table.shape[0]} and lengths for {lengths.shape[0]} "
-                         f"sequences, q has {B}")
-    if not _rows_ok(q):
-        q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-    o = torch.empty((B, H, D), device=q.device, dtype=torch.bfloat16)
+    rows, n = page_table.shape
+    if rows != B or lengths.shape[0] != B:
+        raise ValueError(f"tbf16.paged_sdpa: page_table for {rows} and lengths for {lengths.shape[0]} sequences, q has {B}")
+    q, q_st = _rows(q)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return o
-    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    ws = torch.empty((max(lib().tbf16_paged_attn_ws_bytes(B, H, Hkv, D), 16),), device=q.device, dtype=torch.uint8)
-    launch("tbf16_paged_attn", q, ptr(q), B, H, Hkv, D, _strides(q, 2), ptr(k_cache), ptr(v_cache), pages, page,
-           _strides(k_cache, 3), _strides(v_cache, 3), ptr(page_table), page_table.stride(0), page_table.shape[1],
-           ptr(lengths), sc, ptr(o), ptr(ws), ws.numel())
+    wsb = _ws_bytes(q.get_device(), H, Hkv, D, n * page)
+    ws = q.new_empty(wsb, dtype=torch.uint8) if wsb else o  # (o: nothing is written there)
+    launch("tbf16_paged_attn", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], k_cache.data_ptr(), v_cache.data_ptr(),
+           pages, page, k_st[0], k_st[1], k_st[2], v_st[0], v_st[1], v_st[2], page_table.data_ptr(), page_table.stride(0), n,
+           lengths.data_ptr(), D ** -0.5 if scale is None else float(scale), o.data_ptr(), ws.data_ptr(), wsb)
     return o

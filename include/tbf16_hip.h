@@ -275,11 +275,12 @@ int tbf16_quantize_rows_i8(const void* x, int64_t R, int64_t K, int64_t ldx, voi
 /* Linear in 8-bit integers: y[m, n] = bf16((sum_k qx[m, k] w8[n, k]) sx[m] ws[n] + bias[n]),
  * x quantised per row inside the call as tbf16_quantize_rows_i8 does, int32 sums on the i8
  * MFMA, the scales and the bias in fp32. w8 int8 (N, K) with scales ws fp32 (N,)
- * (tbf16_quantize_rows_i8 of the weight): rows 16-byte aligned, ldw % 16 == 0, readable up
- * to K rounded up to 16 (what is there does not matter). bias bf16 (N,) or NULL. y bf16,
+ * (tbf16_quantize_rows_i8 of the weight): rows 16-byte aligned, ldw % 16 == 0 and at
+ * least K rounded up to 16, the last row readable up to min(ldw, K rounded up to 128) (what is
+ * there does not matter). bias bf16 (N,) or NULL. y bf16,
  * rows 16-byte aligned, ldy % 8 == 0; columns from N up to N rounded up to 8 are written with
- * values to leave out. workspace: tbf16_linear_i8_ws_bytes(M, K, N) bytes, 16-byte aligned.
- * No counterpart in the reference. */
+ * values to leave out. workspace: tbf16_linear_i8_ws_bytes(M, K, N) bytes (asked with the
+ * stream's device current), 16-byte aligned. No counterpart in the reference. */
 size_t tbf16_linear_i8_ws_bytes(int64_t M, int64_t K, int64_t N);
 int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx, const void* w8, int64_t N, int64_t ldw,
                     const float* ws, const void* bias, void* y, int64_t ldy, void* workspace, int64_t ws_bytes,
@@ -303,10 +304,10 @@ int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int6
  * out; a sequence with none gives zeros. q bf16 (B, H, D), element strides (b, h); caches as tbf16_paged_write's
  * (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row stride
  * table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. ws:
- * tbf16_paged_attn_ws_bytes(H, Hkv, D, max_pages * page) bytes (asked with the stream's device
- * current; 0 for short caches, ws may then be NULL), 16-byte aligned, this call's alone until
+ * tbf16_paged_attn_ws_bytes(B, H, Hkv, D, max_pages * page) bytes (asked with the stream's
+ * device current; 0 for few short sequences, ws may then be NULL), 16-byte aligned, this call's alone until
  * it has run. Serves the calls the reference leaves to torch (tbf16/convert.py:29-30). */
-size_t tbf16_paged_attn_ws_bytes(int64_t H, int64_t Hkv, int64_t D, int64_t positions);
+size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t positions);
 int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
                      const void* k_cache, const void* v_cache, int64_t pages, int64_t page, int64_t kc_sp, int64_t kc_sh,
                      int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss, const int32_t* table,

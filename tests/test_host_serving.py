@@ -26,7 +26,7 @@ def wargs(T=5, Hkv=2, D=64):
 def host(monkeypatch):
     """The operators' checks with the one for the device left out (tensors here are on the CPU)."""
     monkeypatch.setattr(paged, "_same_device", lambda *a: None)
-    monkeypatch.setattr(int8, "_dev_check", lambda *a: None)
+    monkeypatch.setattr(int8, "_device", lambda *a: 0)
 
 
 CACHE = [  # what is wrong, the error, part of its text
@@ -137,7 +137,7 @@ def test_abi_refusals():
         assert text in err(), (bad, err())
     assert attn(B=64, H=64, Hkv=2, D=128, wsb=0) == -3 and "workspace" in err()
     assert attn(B=0) == 0
-    assert L.tbf16_paged_attn_ws_bytes(64, 2, 128, 100) == 0 < L.tbf16_paged_attn_ws_bytes(64, 2, 128, 3200)
+    assert L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 100) == 0 < L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 3200)
 
     def write(T=2, ks=s2, kc=16, cs=s3, D=64, k=16, pages=4):
         return L.tbf16_paged_write(k, 16, T, 2, D, *ks, *s2, 16, kc, 16, pages, 16, *cs, *s3, None)
@@ -153,10 +153,10 @@ def test_abi_refusals():
 
     for bad, text in [(dict(K=131073, ldx=131073), "131072"), (dict(ldx=31), "row stride"), (dict(w=8), "weight rows"),
                       (dict(ldw=40), "weight rows"), (dict(K=33, ldx=33), "weight rows"), (dict(ldy=4), "rows of y"),
-                      (dict(N=9), "rows of y"), (dict(y=8), "rows of y"), (dict(ws=None), "workspace"), (dict(M=-1), "bad shape")]:
+                      (dict(N=9), "rows of y"), (dict(y=8), "rows of y"), (dict(ws=None, M=100), "workspace"), (dict(ws=24), "workspace"), (dict(M=-1), "bad shape")]:
         assert linear(**bad) == -1, bad
         assert text in err(), (bad, err())
-    assert linear(wsb=0) == -3 and "workspace" in err()
+    assert linear(wsb=0, M=100) == -3 and "workspace" in err()
     assert linear(M=0) == 0 and linear(N=0) == 0
     assert L.tbf16_linear_i8_ws_bytes(0, 32, 8) == 0 and L.tbf16_linear_i8_ws_bytes(5, 33, 8) >= 5 * 48 + 20
     assert L.tbf16_quantize_rows_i8(16, 2, 33, 33, 16, 32, 16, None) == -1 and "padded" in err()

@@ -7,12 +7,11 @@
 
 #include "abi_util.h"
 #include "common.h"
+#include "gemm_tiles.h"
 
 using namespace tbf16;
 
 namespace {
-
-typedef int int4i __attribute__((ext_vector_type(4)));
 
 // ---- quantisation ---------------------------------------------------------------------
 
@@ -46,65 +45,339 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, kWave));
   return v;
 }
+// The larger magnitude's bits of two or eight bf16: as integers, so that a NaN counts as larger
+// than an infinity and no value is lost.
+__device__ __forceinline__ uint32_t mag2(uint32_t v) { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); }
+__device__ __forceinline__ uint32_t mag8(uint4 v) { return max(max(mag2(v.x), mag2(v.y)), max(mag2(v.z), mag2(v.w))); }
+// The codes of two or eight bf16, packed.
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, const RowCode& rc) {
+  const uint32_t lo = __builtin_amdgcn_perm(code_of(bf16_hi(a), rc), code_of(bf16_lo(a), rc), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(code_of(bf16_hi(b), rc), code_of(bf16_lo(b), rc), 0x04000c0cu);
+  return lo | hi;
+}
+__device__ __forceinline__ uint2 codes8(uint4 v, const RowCode& rc) {
+  return make_uint2(codes4(v.x, v.y, rc), codes4(v.z, v.w, rc));
+}
+// Rows whose maximum is not finite (an infinity or a NaN among their values: integers hold
+// neither) get zero codes and a NaN scale, so every product with them is NaN.
+__device__ __forceinline__ float row_max(uint32_t bits) { return bits < 0x7f80u ? __uint_as_float(bits << 16) : 0.f; }
+__device__ __forceinline__ float row_scale(uint32_t bits) {
+  return bits < 0x7f80u ? __uint_as_float(bits << 16) / 127.f : NAN;
+}
 
-// One wave per row. Rows whose maximum is not finite (an infinity or a NaN among their
-// values: integers hold neither) get zero codes and a NaN scale, so every product with
-// them is NaN.
-__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int64_t R, int64_t K,
-                                                               int64_t ldx, uint8_t* __restrict__ y, int64_t ldy,
+// One wave per row. VEC: rows of 16-byte chunks (K % 8 == 0), up to kChunks x 512 values held in
+// registers between the maximum and the codes (one read of x); otherwise value by value. Codes are
+// written up to Kp (zeros past K).
+constexpr int kChunks = 16;
+template <bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int64_t R, int K, int64_t ldx,
+                                                               uint8_t* __restrict__ y, int64_t ldy, int Kp,
                                                                float* __restrict__ scale) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (row >= R) return;
   const uint16_t* xr = x + row * ldx;
+  uint8_t* yr = y + row * ldy;
   uint32_t bits = 0;
-  for (int64_t i = lane; i < K; i += 64) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
-  bits = wave_max_u(bits);
-  const bool finite = bits < 0x7f80u;
-  const float amax = finite ? __uint_as_float(bits << 16) : 0.f;
-  const RowCode rc = row_code(amax);
-  for (int64_t i = lane; i < (K + 15) / 16 * 16; i += 64)
-    y[row * ldy + i] = i < K && finite ? (uint8_t)code_of(bf16_lo(xr[i]), rc) : (uint8_t)0;
-  if (lane == 0) scale[row] = finite ? amax / 127.f : NAN;
+  if constexpr (VEC) {
+    const uint4* src = reinterpret_cast<const uint4*>(xr);
+    uint2* dst = reinterpret_cast<uint2*>(yr);
+    const int K8 = K >> 3, Kp8 = Kp >> 3;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    if (Kp8 <= kWave * kChunks) {
+      uint4 v[kChunks];
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        v[c] = zero;
+        if (c * kWave < K8 && lane + c * kWave < K8) v[c] = src[lane + c * kWave];
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (c * kWave < K8) bits = max(bits, mag8(v[c]));
+      bits = wave_max_u(bits);
+      const RowCode rc = row_code(row_max(bits));
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (c * kWave < Kp8 && lane + c * kWave < Kp8)
+          dst[lane + c * kWave] = bits < 0x7f80u ? codes8(v[c], rc) : make_uint2(0, 0);
+    } else {
+      constexpr int U = 4;
+      for (int i = lane; i < K8; i += U * kWave) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = i + u * kWave < K8 ? src[i + u * kWave] : zero;
+#pragma unroll
+        for (int u = 0; u < U; ++u) bits = max(bits, mag8(v[u]));
+      }
+      bits = wave_max_u(bits);
+      const RowCode rc = row_code(row_max(bits));
+      for (int i = lane; i < Kp8; i += U * kWave) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = i + u * kWave < K8 ? src[i + u * kWave] : zero;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i + u * kWave < Kp8) dst[i + u * kWave] = bits < 0x7f80u ? codes8(v[u], rc) : make_uint2(0, 0);
+      }
+    }
+  } else {
+    for (int i = lane; i < K; i += kWave) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
+    bits = wave_max_u(bits);
+    const RowCode rc = row_code(row_max(bits));
+    for (int i = lane; i < Kp; i += kWave)
+      yr[i] = i < K && bits < 0x7f80u ? (uint8_t)code_of(bf16_lo(xr[i]), rc) : (uint8_t)0;
+  }
+  if (lane == 0) scale[row] = row_scale(bits);
 }
 
-// ---- product ----------------------------------------------------------------------------
+// ---- product of few rows (decoding) -------------------------------------------------------
+//
+// The weight stream bounds it: N K bytes. A block of 8 waves owns 16 T weight rows, its waves take
+// K in turns of 128 bytes (two MFMAs of 64 a row), weights straight from memory into registers, PF
+// turns of a wave in flight; the int32 sums of the waves meet in LDS. A lane's fragment is 16 bytes
+// of weight row l % 16, and the same k of token l % 16 (of MT groups of 16).
+// FUSED: at most kFusedRows tokens, which every block quantises into LDS for itself, while its
+// first weights are on their way: one launch, no workspace. Otherwise the codes come from a pass
+// of their own (padded with zeros to a multiple of 128, so that what lies behind a weight row
+// does not matter).
+constexpr int kFusedRows = 4, kFusedBytes = 1 << 16;
+template <int T, int MT, bool FUSED>
+__global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restrict__ x, int64_t ldx,
+                                                        const uint8_t* __restrict__ x8, const float* __restrict__ sx,
+                                                        const uint8_t* __restrict__ W, int64_t ldw,
+                                                        const float* __restrict__ sw, const uint16_t* __restrict__ bias,
+                                                        uint16_t* __restrict__ y, int64_t ldy, int M, int N, int K) {
+  constexpr int WAVES = 8, PF = T == 1 ? 8 : T == 2 ? 4 : 3;
+  extern __shared__ __align__(16) uint8_t xl[];  // FUSED: [M][Kp + 16] codes
+  __shared__ intx4 red[WAVES][T * MT][64];
+  __shared__ uint32_t amax[kFusedRows][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * T;
+  const int turns = (K + 127) / 128, Kp = turns * 128;
+  const BufRes wres = make_res(W + (int64_t)n0 * ldw, min<int64_t>((int64_t)(N - n0) * ldw, 0x7fffffff));
+  int woff[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) woff[t] = (16 * t + fr) * (int)ldw + 16 * g;
+  uint4 w[PF][T][2];
+  auto load = [&](uint4 (&w)[T][2], int turn) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) w[t][s] = buf_load16(wres, woff[t] + 64 * s, turn * 128);
+  };
+#pragma unroll
+  for (int u = 0; u < PF; ++u)
+    if (wave + u * WAVES < turns) load(w[u], wave + u * WAVES);
 
-// One wave per 16 x 16 outputs, fragments straight from memory: lane l holds 16 codes of
-// row l % 16, k = 16 (l / 16) of a 64-wide step.
-__global__ __launch_bounds__(64) void gemm_i8_kernel(const uint8_t* __restrict__ A, int64_t lda,
-                                                     const float* __restrict__ sa, const uint8_t* __restrict__ B,
-                                                     int64_t ldb, const float* __restrict__ sb,
-                                                     const uint16_t* __restrict__ bias, uint16_t* __restrict__ C,
-                                                     int64_t ldc, int M, int N, int K16) {
-  const int tiles_n = (N + 15) / 16;
-  const int m0 = blockIdx.x / tiles_n * 16, n0 = blockIdx.x % tiles_n * 16;
-  const int lane = threadIdx.x, fr = lane & 15, fk = lane >> 4;
-  const uint8_t* ar = A + (int64_t)min(m0 + fr, M - 1) * lda;
-  const uint8_t* br = B + (int64_t)min(n0 + fr, N - 1) * ldb;
-  int4i acc = {0, 0, 0, 0};
-  for (int k = 0; k < K16; k += 64) {
-    const int kk = k + 16 * fk;
-    int4i a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-    if (kk < K16) {
-      a = *reinterpret_cast<const int4i*>(ar + kk);
-      b = *reinterpret_cast<const int4i*>(br + kk);
+  if constexpr (FUSED) {
+    for (int m = 0; m < M; ++m) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
+      uint32_t bits = 0;
+      for (int i = tid; i < K >> 3; i += WAVES * 64) bits = max(bits, mag8(src[i]));
+      bits = wave_max_u(bits);
+      if (lane == 0) amax[m][wave] = bits;
     }
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, acc, 0, 0, 0);
+    __syncthreads();
+    for (int m = 0; m < M; ++m) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
+      uint32_t bits = amax[m][0];
+#pragma unroll
+      for (int i = 1; i < WAVES; ++i) bits = max(bits, amax[m][i]);
+      const RowCode rc = row_code(row_max(bits));
+      for (int i = tid; i < Kp >> 3; i += WAVES * 64) {
+        uint2 c = make_uint2(0, 0);
+        if (i < K >> 3 && bits < 0x7f80u) c = codes8(src[i], rc);
+        *reinterpret_cast<uint2*>(xl + m * (Kp + 16) + 8 * i) = c;
+      }
+    }
+    __syncthreads();
   }
-  const int m = m0 + fr;
-  for (int i = 0; i < 4; ++i) {
-    const int n = n0 + 4 * fk + i;
-    if (m < M && n < N) {
-      const float y = (float)acc[i] * (sa[m] * 0x1p-24f) * (sb[n] * 0x1p24f) + (bias ? bf16_lo(bias[n]) : 0.f);
-      C[(int64_t)m * ldc + n] = (uint16_t)pack_bf16(y, 0.f);
+  // tokens past M take the last one's codes and are not stored
+  const uint8_t* xr[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = min(16 * j + fr, M - 1);
+    xr[j] = (FUSED ? xl + m * (Kp + 16) : x8 + (int64_t)m * Kp) + 16 * g;
+  }
+  intx4 acc[T][MT];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[t][j] = intx4{0, 0, 0, 0};
+  for (int t0 = wave; t0 < turns; t0 += PF * WAVES) {
+#pragma unroll
+    for (int u = 0; u < PF; ++u) {
+      const int turn = t0 + u * WAVES;
+      if (turn >= turns) break;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const intx4 xf = *reinterpret_cast<const intx4*>(xr[j] + turn * 128 + 64 * s);
+#pragma unroll
+          for (int t = 0; t < T; ++t) acc[t][j] = I8Op::mma(__builtin_bit_cast(intx4, w[u][t][s]), xf, acc[t][j]);
+        }
+      if (turn + PF * WAVES < turns) load(w[u], turn + PF * WAVES);
     }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[wave][t * MT + j][lane] = acc[t][j];
+  __syncthreads();
+  const int Np = (N + 7) / 8 * 8;
+  for (int i = tid; i < T * MT * 64; i += WAVES * 64) {
+    const int blk = i >> 6, ln = i & 63;
+    const int m = 16 * (blk % MT) + (ln & 15), n = n0 + 16 * (blk / MT) + 4 * (ln >> 4);
+    if (m >= M || n >= Np) continue;
+    intx4 v = red[0][blk][ln];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) v += red[k][blk][ln];
+    float sa;
+    if constexpr (FUSED) {
+      uint32_t bits = amax[m][0];
+#pragma unroll
+      for (int k = 1; k < WAVES; ++k) bits = max(bits, amax[m][k]);
+      sa = row_scale(bits) * I8Op::kA;
+    } else {
+      sa = sx[m] * I8Op::kA;
+    }
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = min(n + e, N - 1);
+      f[e] = fmaf((float)v[e] * sa, sw[c] * I8Op::kB, bias ? bf16_lo(bias[c]) : 0.f);
+    }
+    *reinterpret_cast<uint2*>(y + (int64_t)m * ldy + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
   }
 }
 
-int launch_quantize_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, float* scale,
+// ---- product of many rows -------------------------------------------------------------------
+
+// Split K: the sum of the tile kernels' int32 partial sums (splits x M x Np) and the epilogue.
+// One thread per 8 columns of a row.
+__global__ __launch_bounds__(256) void splitk_i8_kernel(const intx4* __restrict__ part, int splits,
+                                                        const float* __restrict__ sx, const float* __restrict__ sw,
+                                                        const uint16_t* __restrict__ bias, uint16_t* __restrict__ y,
+                                                        int64_t ldy, int M, int N, int Np) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)M * (Np / 8)) return;
+  const int m = (int)(i / (Np / 8)), n = (int)(i % (Np / 8)) * 8;
+  const int64_t step = (int64_t)M * (Np / 4);
+  intx4 lo = part[2 * i], hi = part[2 * i + 1];
+  for (int k = 1; k < splits; ++k) {
+    lo += part[2 * i + k * step];
+    hi += part[2 * i + 1 + k * step];
+  }
+  const float sa = sx[m] * I8Op::kA;
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int c = min(n + e, N - 1);
+    f[e] = fmaf((float)(e < 4 ? lo[e & 3] : hi[e & 3]) * sa, sw[c] * I8Op::kB, bias ? bf16_lo(bias[c]) : 0.f);
+  }
+  stg16(y + (int64_t)m * ldy + n, make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
+                                             pack_bf16(f[6], f[7])));
+}
+
+int64_t num_cus() {
+  static int64_t cache[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cache[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
+
+// The tile kernels (gemm_tiles.h), and the estimate of their times: a round of at most CU-count
+// blocks takes c1 + k tiles x slope us, the slope from `light` (few blocks) to `full`.
+struct Tile {
+  int bm, bn;
+  bool ksplit;
+  float c1, light, full;
+};
+constexpr Tile kTiles[] = {{256, 256, false, 7.6f, 0.97f, 1.40f}, {192, 256, false, 7.4f, 0.82f, 1.04f},
+                           {128, 256, false, 5.8f, 0.75f, 0.87f}, {256, 128, false, 5.8f, 0.66f, 0.87f},
+                           {128, 128, false, 4.1f, 0.51f, 0.56f}, {256, 128, true, 6.6f, 0.62f, 0.83f},
+                           {192, 128, true, 5.6f, 0.46f, 0.635f}, {128, 128, true, 3.9f, 0.44f, 0.52f},
+                           {128, 64, true, 2.7f, 0.36f, 0.37f},   {64, 128, true, 2.7f, 0.36f, 0.37f},
+                           {64, 64, true, 2.0f, 0.25f, 0.26f}};
+constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+constexpr size_t kSplitBytes = (size_t)16 << 20;
+
+// How a call runs.
+struct Plan {
+  enum Form { kFused, kDecode, kTiled } form;
+  int T, MT;          // decode kernel
+  int tile, splits;   // tile kernels
+  size_t scale, x8, part, bytes;  // workspace
+};
+
+Plan plan_of(int64_t M, int64_t K, int64_t N, bool vec) {
+  Plan p{Plan::kTiled, 1, 1, 0, 1, 0, 0, 0, 0};
+  const int64_t Kp = (int64_t)align_up((size_t)K, 128), Np = (int64_t)align_up((size_t)N, 8), cus = num_cus();
+  if (M <= 64) {
+    p.MT = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    p.T = (int)std::min<int64_t>(p.MT == 4 ? 2 : 4, std::max<int64_t>(1, cdiv(cdiv(N, 16), cus)));
+    p.form = Plan::kDecode;
+    if (vec && M <= kFusedRows && M * (Kp + 16) <= kFusedBytes) {
+      p.form = Plan::kFused;
+      return p;
+    }
+  }
+  p.x8 = align_up((size_t)M * 4, 256);
+  p.bytes = p.part = align_up(p.x8 + (size_t)M * Kp, 256);
+  if (p.form == Plan::kDecode) return p;
+  const int64_t KT = std::max<int64_t>(1, Kp / 128);
+  float best = INFINITY;
+  for (int i = 0; i < kNumTiles; ++i) {
+    const Tile& t = kTiles[i];
+    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+    if (tiles >= (int64_t)1 << 31) continue;
+    for (int s = 1; s <= 8; s *= 2) {
+      const int64_t kt = cdiv(KT, s);
+      if (s > 1 && (kt < 8 || (s - 1) * kt >= KT || (size_t)s * M * Np * 4 > kSplitBytes)) break;
+      const float load = std::min(1.f, (float)(tiles * s) / (float)cus);
+      float us = (float)cdiv(tiles * s, cus) * (t.c1 + (float)kt * (t.light + (t.full - t.light) * load));
+      if (s > 1) us += 4.5f + (float)s * (float)M * (float)Np * 8.f / 2e6f;
+      if (us < best) {
+        best = us;
+        p.tile = i;
+        p.splits = s;
+      }
+    }
+  }
+  if (p.splits > 1) p.bytes = p.part + (size_t)p.splits * M * Np * 4;
+  return p;
+}
+// The last plans of this thread by shape (the search costs as much host time as a launch).
+const Plan& plan(int64_t M, int64_t K, int64_t N, bool vec) {
+  struct Entry {
+    int64_t M, K, N, cus;
+    bool vec;
+    Plan plan;
+  };
+  constexpr int kEntries = 64;
+  static thread_local Entry cache[kEntries] = {};  // M = 0: empty
+  Entry& e = cache[(uint64_t)(M * 31 + N * 7 + K) % kEntries];
+  const int64_t cus = num_cus();
+  if (e.M != M || e.K != K || e.N != N || e.cus != cus || e.vec != vec) e = Entry{M, K, N, cus, vec, plan_of(M, K, N, vec)};
+  return e.plan;
+}
+
+bool rows_vec(const void* x, int64_t K, int64_t ldx) { return K % 8 == 0 && ldx % 8 == 0 && aligned16(x); }
+
+int launch_quantize_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, int64_t Kp, float* scale,
                        hipStream_t st) {
-  quantize_rows_i8_kernel<<<(unsigned)cdiv(R, 4), 256, 0, st>>>((const uint16_t*)x, R, K, ldx, (uint8_t*)y8, ldy, scale);
+  const unsigned blocks = (unsigned)cdiv(R, 4);
+  if (rows_vec(x, K, ldx))
+    quantize_rows_i8_kernel<true><<<blocks, 256, 0, st>>>((const uint16_t*)x, R, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
+  else
+    quantize_rows_i8_kernel<false><<<blocks, 256, 0, st>>>((const uint16_t*)x, R, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
   TB_LAUNCH_CHECK("quantize_rows_i8");
   return 0;
 }
@@ -116,15 +389,6 @@ int check_rows_i8(const char* fn, const void* x, int64_t R, int64_t K, int64_t l
   return 0;
 }
 
-struct LinearI8Ws {
-  size_t scale, x8, bytes;
-};
-LinearI8Ws linear_i8_ws(int64_t M, int64_t K, int64_t N) {
-  LinearI8Ws w{0, align_up((size_t)M * 4, 256), 0};
-  w.bytes = align_up(w.x8 + (size_t)M * align_up((size_t)K, 16), 256);
-  return w;
-}
-
 }  // namespace
 
 extern "C" int tbf16_quantize_rows_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, float* scale,
@@ -133,40 +397,103 @@ extern "C" int tbf16_quantize_rows_i8(const void* x, int64_t R, int64_t K, int64
   TB_CHECK(aligned16(y8) && ldy % 16 == 0 && ldy >= (int64_t)align_up((size_t)K, 16) && aligned4(scale),
            "quantize_rows_i8: rows of codes must be 16-byte aligned and padded to 16");
   if (R == 0) return 0;
-  return launch_quantize_i8(x, R, K, ldx, y8, ldy, scale, as_stream(stream));
+  return launch_quantize_i8(x, R, K, ldx, y8, ldy, (int64_t)align_up((size_t)K, 16), scale, as_stream(stream));
 }
 
 extern "C" size_t tbf16_linear_i8_ws_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= 0 || K < 0 || N <= 0) return 0;
-  return linear_i8_ws(M, K, N).bytes;
+  return plan(M, K, N, false).bytes;  // (enough for the forms that need none)
 }
 
 extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx, const void* w8, int64_t N, int64_t ldw,
                                const float* ws, const void* bias, void* y, int64_t ldy, void* workspace, int64_t ws_bytes,
                                void* stream) {
   if (int rc = check_rows_i8("linear_i8", x, M, K, ldx)) return rc;
-  const int64_t K16 = (int64_t)align_up((size_t)K, 16);
-  TB_CHECK(N >= 0 && N < (int64_t)1 << 31, "linear_i8: bad shape");
+  const int64_t K16 = (int64_t)align_up((size_t)K, 16), Np = (int64_t)align_up((size_t)N, 8);
+  TB_CHECK(N >= 0 && N < ((int64_t)1 << 31) - 512 && M < ((int64_t)1 << 31) - 512, "linear_i8: bad shape");
   TB_CHECK(aligned16(w8) && ldw % 16 == 0 && ldw >= K16 && ldw < (int64_t)1 << 23,
            "linear_i8: weight rows must be 16-byte aligned and padded to 16");
-  TB_CHECK(aligned16(y) && ldy % 8 == 0 && ldy >= (int64_t)align_up((size_t)N, 8),
-           "linear_i8: rows of y must be 16-byte aligned and padded to 8");
+  TB_CHECK(aligned16(y) && ldy % 8 == 0 && ldy >= Np, "linear_i8: rows of y must be 16-byte aligned and padded to 8");
   TB_CHECK(aligned4(ws) && (reinterpret_cast<uintptr_t>(bias) & 1) == 0, "linear_i8: scales or bias misaligned");
   if (M == 0 || N == 0) return 0;
-  const LinearI8Ws w = linear_i8_ws(M, K, N);
-  TB_CHECK(aligned16(workspace) && workspace != nullptr, "linear_i8: workspace missing or misaligned");
-  if (ws_bytes < (int64_t)w.bytes) {
-    set_error("linear_i8: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, w.bytes);
+  const Plan& p = plan(M, K, N, rows_vec(x, K, ldx));
+  TB_CHECK(aligned16(workspace) && (workspace != nullptr || p.bytes == 0), "linear_i8: workspace missing or misaligned");
+  if (ws_bytes < (int64_t)p.bytes) {
+    set_error("linear_i8: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, p.bytes);
     return TBF16_EWS;
   }
   const hipStream_t st = as_stream(stream);
   uint8_t* wsp = static_cast<uint8_t*>(workspace);
-  float* sx = reinterpret_cast<float*>(wsp + w.scale);
-  if (int rc = launch_quantize_i8(x, M, K, ldx, wsp + w.x8, K16, sx, st)) return rc;
-  const int64_t blocks = cdiv(M, 16) * cdiv(N, 16);
-  TB_CHECK(blocks < (int64_t)1 << 31, "linear_i8: grid too large");
-  gemm_i8_kernel<<<(unsigned)blocks, 64, 0, st>>>(wsp + w.x8, K16, sx, (const uint8_t*)w8, ldw, ws, (const uint16_t*)bias,
-                                                  (uint16_t*)y, ldy, (int)M, (int)N, (int)K16);
+  float* sx = reinterpret_cast<float*>(wsp + p.scale);
+  uint8_t* x8 = wsp + p.x8;
+  const int64_t Kp = (int64_t)align_up((size_t)K, 128);
+  const uint16_t* bi = (const uint16_t*)bias;
+  uint16_t* yo = (uint16_t*)y;
+  if (p.form != Plan::kFused)
+    if (int rc = launch_quantize_i8(x, M, K, ldx, x8, Kp, Kp, sx, st)) return rc;
+  if (p.form != Plan::kTiled) {
+    const unsigned blocks = (unsigned)cdiv(N, 16 * p.T);
+#define DECODE(T_, MT_, FUSED_)                                                                                       \
+  decode_i8_kernel<T_, MT_, FUSED_><<<blocks, 512, FUSED_ ? (size_t)(M * (Kp + 16)) : 0, st>>>(                             \
+      (const uint16_t*)x, ldx, x8, sx, (const uint8_t*)w8, ldw, ws, bi, yo, ldy, (int)M, (int)N, (int)K)
+#define DECODE_T(MT_, FUSED_)                \
+  switch (p.T) {                             \
+    case 1: DECODE(1, MT_, FUSED_); break;   \
+    case 2: DECODE(2, MT_, FUSED_); break;   \
+    case 3: DECODE(3, MT_, FUSED_); break;   \
+    default: DECODE(4, MT_, FUSED_); break;  \
+  }
+    if (p.form == Plan::kFused) {
+      DECODE_T(1, true)
+    } else if (p.MT == 1) {
+      DECODE_T(1, false)
+    } else if (p.MT == 2) {
+      DECODE_T(2, false)
+    } else if (p.T == 1) {
+      DECODE(1, 4, false);
+    } else {
+      DECODE(2, 4, false);
+    }
+#undef DECODE_T
+#undef DECODE
+    TB_LAUNCH_CHECK("linear_i8");
+    return 0;
+  }
+  // operand rows in units of 2 bytes
+  const auto a = (const uint16_t*)x8, b = (const uint16_t*)w8;
+  const Tile& t = kTiles[p.tile];
+  float* part = p.splits > 1 ? reinterpret_cast<float*>(wsp + p.part) : nullptr;
+  int rows = t.bn;  // weight rows per block: fewer where a single row of tiles would leave CUs idle
+  if (t.ksplit && M <= t.bm && p.splits == 1 && cdiv(N, t.bn) < num_cus())
+    rows = (int)std::min<int64_t>(t.bn, std::max<int64_t>(8, cdiv(cdiv(N, num_cus()), 8) * 8));
+  const int kt_per = (int)cdiv(Kp / 128, p.splits);
+  const dim3 grid((unsigned)(cdiv(M, t.bm) * cdiv(Np, rows)), (unsigned)p.splits);
+#define PINGPONG(HA_, FB_, S_)                                                                                   \
+  pingpong_kernel<I8Op, HA_, FB_, S_, true><<<grid, 512, 0, st>>>(a, Kp / 2, sx, b, ldw / 2, ws, bi, yo, ldy, (int)M, (int)Np, \
+                                                                  (int)(Kp / 2), part, kt_per, (int)N)
+#define KSPLIT(RM_, RN_, S_)                                                                                             \
+  ksplit_kernel<I8Op, RM_, RN_, S_, true><<<grid, 512, 0, st>>>(a, Kp / 2, sx, b, ldw / 2, ws, bi, yo, ldy, (int)M, (int)Np, \
+                                                                (int)(Kp / 2), part, kt_per, rows, (int)N, ConvGeom{})
+  switch (p.tile) {
+    case 0: PINGPONG(4, 2, 2); break;
+    case 1: PINGPONG(3, 2, 2); break;
+    case 2: PINGPONG(2, 2, 3); break;
+    case 3: PINGPONG(4, 1, 3); break;
+    case 4: PINGPONG(2, 1, 3); break;
+    case 5: KSPLIT(8, 4, 3); break;
+    case 6: KSPLIT(6, 4, 3); break;
+    case 7: KSPLIT(4, 4, 4); break;
+    case 8: KSPLIT(4, 2, 6); break;
+    case 9: KSPLIT(2, 4, 6); break;
+    default: KSPLIT(2, 2, 6); break;
+  }
+#undef PINGPONG
+#undef KSPLIT
   TB_LAUNCH_CHECK("linear_i8");
+  if (part) {
+    splitk_i8_kernel<<<(unsigned)cdiv(M * (Np / 8), 256), 256, 0, st>>>((const intx4*)part, p.splits, sx, ws, bi, yo, ldy, (int)M,
+                                                                        (int)N, (int)Np);
+    TB_LAUNCH_CHECK("linear_i8 split-K sum");
+  }
   return 0;
 }

@@ -73,9 +73,6 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 32;
-#ifndef BLOCKS_MUL
-#define BLOCKS_MUL 1
-#endif
 // Running maxima start at kNone; a unit that had any key ends at kFew or above.
 constexpr float kNone = -FLT_MAX, kFew = -3.0e38f;
 
@@ -91,39 +88,45 @@ struct AttnArgs {
   int B, H, Hkv, G, D, R, RG;  // R rows a unit, RG units a key/value head
   uint16_t* o;
   float *part, *stat;  // [block][2][R][D], [block][2][R][2]: what a block leaves of units it shares
-  int4* desc;  // [block]: the unit it began and later blocks end (b, unit, last block, 1) or (.., 0)
+  int4* desc;  // [block]: the unit it began and later blocks end (b, head, last block, grp + 1), else w = 0
 };
 
 __device__ __forceinline__ int seq_len(const AttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.cap); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A place in the list.
+// A place in the list: tile `tile` of nt of a unit, the grp-th group of R rows of key/value head
+// `head` of sequence b.
 struct Cursor {
-  int b, unit, tile, nt, len;
+  int b, head, grp, tile, nt, len;
 };
-__device__ __forceinline__ void enter(const AttnArgs& a, Cursor& c) {  // c.b set: its first tile, skipping empty ones
-  c.unit = c.tile = c.nt = c.len = 0;
-  while (c.b < a.B && (c.len = uniform(seq_len(a, c.b))) == 0) ++c.b;
-  c.nt = (c.len + kTile - 1) / kTile;
-}
-__device__ __forceinline__ void advance(const AttnArgs& a, Cursor& c, int units) {
+__device__ __forceinline__ void advance(const AttnArgs& a, Cursor& c) {
   if (++c.tile < c.nt) return;
   c.tile = 0;
-  if (++c.unit < units) return;
-  ++c.b;
-  enter(a, c);
+  if (++c.grp < a.RG) return;
+  c.grp = 0;
+  if (++c.head < a.Hkv) return;
+  c.head = 0;
+  do c.len = uniform(seq_len(a, ++c.b));  // (the caller knows that there is a tile ahead)
+  while (c.len == 0);
+  c.nt = (c.len + kTile - 1) / kTile;
 }
-// The list's split into runs of c tiles, at least kMinTiles, run w from tile w c on (the host
-// has made sure that 32 bits count its tiles), and run w's length n and first place.
-constexpr int kMinTiles = 2;
+// The list's split: `act` waves of each block (fewer than WPB where the list is so short that the
+// CUs would not all get some) take runs of c tiles, run w from tile w c on. This run's length n and
+// first place. 32 bits count the list's tiles (the host has made sure).
 struct Run {
-  uint32_t c;
+  uint32_t c, act;
   int n;
   Cursor at;
 };
-__device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t w, uint32_t waves, int units, int lane) {
-  auto tiles = [&](int b) { return b < a.B ? (uint32_t)((seq_len(a, b) + kTile - 1) / kTile * units) : 0u; };
+__device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t block, uint32_t wave, uint32_t blocks, uint32_t wpb,
+                                      int units, int lane) {
+  constexpr int PF = 4;  // groups of 64 sequences whose lengths are loaded at once
+  int len[PF];
+  uint32_t up[PF];  // tiles of the group's sequences up to the lane's own
+#pragma unroll
+  for (int k = 0; k < PF; ++k) len[k] = lane + k * kWave < a.B ? seq_len(a, lane + k * kWave) : 0;
+  auto tiles = [&](int l) { return (uint32_t)((l + kTile - 1) / kTile); };
   auto prefix = [&](uint32_t v) {  // inclusive
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
@@ -132,37 +135,60 @@ __device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t w, uint32_t wa
     }
     return v;
   };
-  const uint32_t n0 = tiles(lane), up0 = prefix(n0);
-  uint32_t all = uniform(__shfl((int)up0, kWave - 1, kWave));
-  if (a.B > kWave) {
-    uint32_t more = 0;
-    for (int b = lane + kWave; b < a.B; b += kWave) more += tiles(b);
-    all += uniform(__shfl((int)prefix(more), kWave - 1, kWave));
-  }
-  Run r{max((uint32_t)kMinTiles, (all + waves - 1) / waves), 0, {0, 0, 0, 0, 0}};
-  const uint64_t first = (uint64_t)w * r.c;
-  if (first >= all) return r;
-  r.n = min(r.c, all - (uint32_t)first);
-  uint32_t t = (uint32_t)first, n = n0, up = up0;
-  for (int b0 = 0;; b0 += kWave) {
-    if (b0 > 0) {
-      n = tiles(b0 + lane);
-      up = prefix(n);
+  auto last = [&](uint32_t v) { return (uint32_t)uniform(__builtin_amdgcn_readlane((int)v, kWave - 1)); };
+  uint32_t all = 0;
+#pragma unroll
+  for (int k = 0; k < PF; ++k) {
+    up[k] = 0;
+    if (k * kWave < a.B) {
+      up[k] = prefix(tiles(len[k]));
+      all += last(up[k]);
     }
-    const uint64_t past = __ballot(up > t);
+  }
+  if (a.B > PF * kWave) {
+    uint32_t more = 0;
+    for (int b = lane + PF * kWave; b < a.B; b += kWave) more += tiles(seq_len(a, b));
+    all += last(prefix(more));
+  }
+  all *= units;
+  Run r{1, 1, 0, {0, 0, 0, 0, 0, 0}};
+  r.act = min(wpb, max(1u, (all + blocks - 1) / blocks));
+  r.c = max(1u, (all + blocks * r.act - 1) / (blocks * r.act));
+  const uint64_t first = ((uint64_t)block * r.act + wave) * r.c;
+  if (wave >= r.act || first >= all) return r;
+  r.n = min(r.c, all - (uint32_t)first);
+  // the sequence: the first one that ends behind tile `first`
+  uint32_t t = (uint32_t)first / units, rest = (uint32_t)first % units;  // in tiles of one unit
+  for (int k = 0;; ++k) {
+    int l = 0;
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+      if (k == i) {
+        l = len[i];
+        u = up[i];
+      }
+    if (k >= PF) {
+      const int b = k * kWave + lane;
+      l = b < a.B ? seq_len(a, b) : 0;
+      u = prefix(tiles(l));
+    }
+    const uint64_t past = __ballot(u > t);
     if (past == 0) {
-      t -= uniform(__shfl((int)up, kWave - 1, kWave));
+      t -= last(u);
       continue;
     }
-    const int l = __builtin_ctzll(past);
-    r.at.b = b0 + l;
-    t -= uniform(__shfl((int)(up - n), l, kWave));
-    r.at.nt = uniform(__shfl((int)n, l, kWave)) / units;
+    const int w = __builtin_ctzll(past);
+    r.at.b = k * kWave + w;
+    r.at.len = __builtin_amdgcn_readlane(l, w);
+    r.at.nt = (r.at.len + kTile - 1) / kTile;
+    t = (t - (__builtin_amdgcn_readlane((int)u, w) - r.at.nt)) * units + rest;  // in the sequence's own tiles
     break;
   }
-  r.at.len = uniform(seq_len(a, r.at.b));
-  r.at.unit = t / (uint32_t)r.at.nt;
-  r.at.tile = t % (uint32_t)r.at.nt;
+  const uint32_t unit = t / (uint32_t)r.at.nt;
+  r.at.tile = t - unit * r.at.nt;
+  r.at.head = unit / (uint32_t)a.RG;
+  r.at.grp = unit - r.at.head * a.RG;
   return r;
 }
 
@@ -266,37 +292,38 @@ struct Acc {
 };
 
 // A unit's first row in o, and how many it has.
-__device__ __forceinline__ uint16_t* unit_out(const AttnArgs& a, int b, int unit) {
-  return a.o + ((int64_t)b * a.H + unit / a.RG * a.G + unit % a.RG * a.R) * a.D;
+__device__ __forceinline__ uint16_t* unit_out(const AttnArgs& a, int b, int head, int grp) {
+  return a.o + ((int64_t)b * a.H + head * a.G + grp * a.R) * a.D;
 }
-__device__ __forceinline__ int unit_rows(const AttnArgs& a, int unit) { return min(a.R, a.G - unit % a.RG * a.R); }
+__device__ __forceinline__ int unit_rows(const AttnArgs& a, int grp) { return min(a.R, a.G - grp * a.R); }
 
 // DP: D rounded up to 64, 128 or 256 (D == DP unless PAD). WPB waves a block. UNIT: one block
 // per unit instead of equal runs of the list.
 template <int DP, int RT, int WPB, bool PAD, bool UNIT>
-__global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 : 2) void paged_attn_kernel(AttnArgs a) {
   constexpr int CH = DP / 16, KI = DP / 32, VW = CH / 2;  // V dwords a lane holds of a key
   extern __shared__ __align__(16) float lds[];  // [wave][R][DP + 4], [wave][R][2]
   __shared__ int flags[WPB];  // 1: the wave left a part of a unit begun before it, 2: its last
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
-  const int units = a.Hkv * a.RG;
-  const int ld = DP + 4;
+  constexpr int ld = DP + 4;
   float* const stat0 = lds + WPB * a.R * ld;
 
   Cursor cur;
   int n;  // this wave's tiles
-  uint32_t c = 0;
+  uint32_t c = 0, act = WPB;
   if constexpr (UNIT) {
-    cur.b = blockIdx.x / units;
-    cur.unit = blockIdx.x % units;
+    cur.b = blockIdx.x;
+    cur.head = blockIdx.y;
+    cur.grp = blockIdx.z;
     cur.len = uniform(seq_len(a, cur.b));
     cur.nt = (cur.len + kTile - 1) / kTile;
     const int per = (cur.nt + WPB - 1) / WPB;
     cur.tile = min(wave * per, cur.nt);
     n = min(per, cur.nt - cur.tile);
   } else {
-    const Run r = run_of(a, blockIdx.x * WPB + wave, gridDim.x * WPB, units, lane);
+    const Run r = run_of(a, blockIdx.x, wave, gridDim.x, WPB, a.Hkv * a.RG, lane);
     c = r.c;
+    act = r.act;
     n = r.n;
     cur = r.at;
     if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -307,13 +334,13 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
   bool tail = false;  // acc is the begin of a unit that goes on in the next wave
   if (n > 0) {
     struct Page {
-      int id, row;
+      int id, row, head;
     };
     // the page and row of the lane's key (l % 32) of a tile
     auto page_of = [&](const Cursor& c) {
       const uint32_t pos = c.tile * kTile + (lane & 31);
       const uint32_t idx = (uint32_t)((uint64_t)pos * a.magic >> a.shift);
-      Page p{-1, (int)(pos - idx * a.page)};
+      Page p{-1, (int)(pos - idx * a.page), c.head};
       if (pos < (uint32_t)c.len) p.id = a.table[c.b * a.t_sb + idx];
       return p;
     };
@@ -323,10 +350,10 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
     auto shfl_off = [&](int64_t off, int src) {
       return (int64_t)(uint32_t)__shfl((int)off, src, kWave) | (int64_t)__shfl((int)(off >> 32), src, kWave) << 32;
     };
-    auto load_k = [&](const Cursor& c, const Page& p) {
+    auto load_k = [&](const Page& p) {
       const bool ok = (uint32_t)p.id < a.pages;
       const int64_t off = ok ? (int64_t)p.id * a.kg.sp + (int64_t)p.row * a.kg.ss : 0;
-      const uint16_t* base = a.kc + c.unit / a.RG * a.kg.sh;
+      const uint16_t* base = a.kc + p.head * a.kg.sh;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint16_t* row = base + shfl_off(off, 16 * h + r16);
@@ -337,11 +364,11 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
         }
       }
     };
-    auto load_v = [&](const Cursor& c, const Page& p) {
+    auto load_v = [&](const Page& p) {
       const bool ok = (uint32_t)p.id < a.pages;
       const int64_t off = ok ? (int64_t)p.id * a.vg.sp + (int64_t)p.row * a.vg.ss : 0;
       const int e = PAD && CH * r16 >= a.D ? 0 : CH * r16;  // (what lies past D goes to outputs past D)
-      const uint16_t* base = a.vc + c.unit / a.RG * a.vg.sh + e;
+      const uint16_t* base = a.vc + p.head * a.vg.sh + e;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t* row = reinterpret_cast<const uint32_t*>(base + shfl_off(off, 16 * (j >> 2) + 4 * g + (j & 3)));
@@ -360,7 +387,7 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
     auto alive = [&](const Page& p) { return (uint32_t)__ballot((uint32_t)p.id < a.pages); };  // lanes l and l + 32 alike
     bf16x8 qf[RT][KI];
     auto load_q = [&](const Cursor& c) {
-      const int h0 = c.unit / a.RG * a.G + c.unit % a.RG * a.R, rows = unit_rows(a, c.unit);
+      const int h0 = c.head * a.G + c.grp * a.R, rows = unit_rows(a, c.grp);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const int row = 16 * r + r16;
@@ -375,24 +402,24 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
       }
     };
 
-    Cursor nx = cur;
-    Page pc = page_of(cur), pn{-1, 0};
-    if (n > 1) {
-      advance(a, nx, units);
-      pn = page_of(nx);
-    }
+    Page next = page_of(cur);
     load_q(cur);
-    load_k(cur, pc);
-    load_v(cur, pc);
-    live = alive(pc);
+    load_k(next);
+    load_v(next);
+    live = alive(next);
+    Cursor ahead = cur;
+    if (n > 1) {
+      advance(a, ahead);
+      next = page_of(ahead);
+    }
     acc.clear();
     bool begun = cur.tile == 0;  // acc holds its unit from the first tile on
     for (int i = 0;; ++i) {
-      Cursor n2 = nx;
-      Page p2{-1, 0};
+      const bool more = i + 1 < n;
+      Page next2 = next;
       if (i + 2 < n) {
-        advance(a, n2, units);
-        p2 = page_of(n2);
+        advance(a, ahead);
+        next2 = page_of(ahead);
       }
       // logits
       floatx4 s[RT][2];
@@ -408,7 +435,7 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
             s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv), qf[r][t], s[r][h], 0, 0, 0);
           }
         }
-      if (i + 1 < n) load_k(nx, pn);
+      if (more) load_k(next);
       const bool whole = live == 0xffffffffu;
       bf16x8 ph[RT], pl[RT];
 #pragma unroll
@@ -461,30 +488,33 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
           acc.o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[r], acc.o[r][d], 0, 0, 0);
         }
       }
+      if (more) {
+        load_v(next);
+        live = alive(next);
+        next = next2;
+      }
       const bool end = cur.tile + 1 == cur.nt;  // of the unit
-      if (i + 1 < n) {
-        load_v(nx, pn);
-        live = alive(pn);
-        if (end) load_q(nx);
+      if (more && (UNIT || !end)) {
+        ++cur.tile;
+        continue;
       }
-      if (end || i + 1 == n) {
-        const int rows = unit_rows(a, cur.unit);
-        acc.total();
-        if (begun && end) {
-          acc.finish(unit_out(a, cur.b, cur.unit), rows, a.D, lane);
-        } else if (!begun) {
-          acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, rows, a.D, lane);
-          if (lane == 0) flags[wave] = end ? 3 : 1;
-        } else {
-          tail = true;
-        }
-        if (i + 1 == n) break;
-        acc.clear();
-        begun = true;
+      const Cursor done = cur;
+      if (more) {  // the next unit's q is on its way while this unit leaves
+        advance(a, cur);
+        load_q(cur);
       }
-      cur = nx;
-      nx = n2;
-      pn = p2;
+      acc.total();
+      if (begun && end) {
+        acc.finish(unit_out(a, done.b, done.head, done.grp), unit_rows(a, done.grp), a.D, lane);
+      } else if (!begun) {
+        acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, unit_rows(a, done.grp), a.D, lane);
+        if (lane == 0) flags[wave] = end ? 3 : 1;
+      } else {
+        tail = true;
+      }
+      if (!more) break;
+      acc.clear();
+      begun = true;
     }
   }
   __syncthreads();
@@ -493,30 +523,30 @@ __global__ __launch_bounds__(WPB * 64) void paged_attn_kernel(AttnArgs a) {
   const int64_t slot = (int64_t)blockIdx.x * 2;
   int last;  // the last wave before the end of the unit that wave `from` - 1 goes on with, or of the block
   auto span = [&](int from) {
-    for (last = from; last < WPB - 1 && uniform(flags[last]) == 1; ++last) {
+    for (last = from; last < (int)act - 1 && uniform(flags[last]) == 1; ++last) {
     }
-    return last < WPB && uniform(flags[last]) == 3;
+    return uniform(flags[last]) == 3;
   };
   auto take = [&](int from) {
     acc.take(lds + from * a.R * ld, a.R * ld, ld, stat0 + from * a.R * 2, a.R * 2, last + 1 - from, a.R, a.D, lane);
   };
   if (tail) {
-    const bool ended = wave + 1 < WPB && span(wave + 1);
-    if (wave + 1 < WPB) take(wave + 1);
+    const bool ended = wave + 1 < (int)act && span(wave + 1);
+    if (wave + 1 < (int)act) take(wave + 1);
     if (ended) {
-      acc.finish(unit_out(a, cur.b, cur.unit), unit_rows(a, cur.unit), a.D, lane);
+      acc.finish(unit_out(a, cur.b, cur.head, cur.grp), unit_rows(a, cur.grp), a.D, lane);
     } else if constexpr (!UNIT) {
       acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
       // the unit's last tile: this wave's last one is its tile cur.tile
-      const uint32_t end = (blockIdx.x * WPB + wave) * c + n - 1 - cur.tile + cur.nt - 1;
-      if (lane == 0) a.desc[blockIdx.x] = make_int4(cur.b, cur.unit, end / (c * WPB), 1);
+      const uint32_t end = (blockIdx.x * act + wave) * c + n - 1 - cur.tile + cur.nt - 1;
+      if (lane == 0) a.desc[blockIdx.x] = make_int4(cur.b, cur.head, end / (c * act), cur.grp + 1);
     }
   }
   if constexpr (UNIT) {
     if (cur.nt == 0) {  // a sequence without keys
-      const int chunks = unit_rows(a, cur.unit) * a.D / 8;
+      const int chunks = unit_rows(a, cur.grp) * a.D / 8;
       for (int i = threadIdx.x; i < chunks; i += WPB * 64)
-        stg16(unit_out(a, cur.b, cur.unit) + 8 * i, make_uint4(0, 0, 0, 0));
+        stg16(unit_out(a, cur.b, cur.head, cur.grp) + 8 * i, make_uint4(0, 0, 0, 0));
     }
   } else {
     if (wave == 0 && uniform(flags[0]) != 0) {
@@ -541,7 +571,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a)
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int4 u = a.desc[blockIdx.x];
   if (u.w == 0) return;
-  const int first = blockIdx.x, last = u.z, rows = unit_rows(a, u.y), dg = a.D / 4;
+  const int first = blockIdx.x, last = u.z, rows = unit_rows(a, u.w - 1), dg = a.D / 4;
   const int e = blockIdx.y * 64 + lane;  // (row, group of 4)
   const int row = min(e / dg, rows - 1), d = e % dg * 4;
   float m = kNone, l = 0.f;
@@ -577,7 +607,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a)
 #pragma unroll
   for (int w = 1; w < kJoinWaves; ++w) add(ss[w][lane], so[w][lane]);
   const float f = m == kNone ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(unit_out(a, u.x, u.y) + (int64_t)row * a.D + d) =
+  *reinterpret_cast<uint2*>(unit_out(a, u.x, u.y, u.w - 1) + (int64_t)row * a.D + d) =
       make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
 }
 
@@ -601,7 +631,7 @@ struct AttnPlan {
   int64_t blocks;
   size_t stat, desc, bytes;
 };
-AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
+AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   AttnPlan p;
   const int64_t G = H / Hkv;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
@@ -609,11 +639,12 @@ AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   p.R = (int)std::min<int64_t>(G, 16 * p.RT);
   p.RG = (int)cdiv(G, p.R);
   p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
-  p.unit = cdiv(cap, kTile) <= p.wpb * 4;
+  p.unit = cdiv(cap, kTile) <= 2 * p.wpb && B * Hkv * p.RG <= num_cus();
   p.stat = p.desc = p.bytes = 0;
   p.blocks = 0;
   if (p.unit) return p;
-  p.blocks = num_cus() * (8 / p.wpb) * BLOCKS_MUL;
+  // as many as run at once: by registers, 4 waves a SIMD of D = 64, 2 of D = 128, 1 of D = 256
+  p.blocks = num_cus() * (p.DP == 64 || (p.wpb == 4 && p.DP < 256) ? 2 : 1);
   p.stat = align_up((size_t)p.blocks * 2 * p.R * (size_t)D * 4, 256);
   p.desc = p.stat + align_up((size_t)p.blocks * 2 * p.R * 2 * 4, 256);
   p.bytes = p.desc + align_up((size_t)p.blocks * 16, 256);
@@ -622,10 +653,11 @@ AttnPlan attn_plan(int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
 
 template <int DP, int RT, int WPB>
 void launch_attn(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
+  const dim3 grid = unit ? dim3((unsigned)a.B, (unsigned)a.Hkv, (unsigned)a.RG) : dim3((unsigned)blocks);
   const size_t lds = (size_t)WPB * a.R * (DP + 4 + 2) * 4;
   const bool pad = a.D != DP;
 #define ATTN(PAD_, UNIT_) \
-  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_><<<(unsigned)blocks, WPB * 64, lds, st>>>(a)
+  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_><<<grid, WPB * 64, lds, st>>>(a)
   if (unit) {
     if (pad) ATTN(true, true);
     else ATTN(false, true);
@@ -666,8 +698,8 @@ extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_
   return 0;
 }
 
-extern "C" size_t tbf16_paged_attn_ws_bytes(int64_t H, int64_t Hkv, int64_t D, int64_t positions) {
-  return H > 0 && Hkv > 0 && D > 0 && H % Hkv == 0 ? attn_plan(H, Hkv, D, positions).bytes : 0;
+extern "C" size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t positions) {
+  return B > 0 && H > 0 && Hkv > 0 && D > 0 && H % Hkv == 0 ? attn_plan(B, H, Hkv, D, positions).bytes : 0;
 }
 
 extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
@@ -685,7 +717,7 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
            "paged_attn: q must have 16-byte aligned rows");
   TB_CHECK(aligned4(table) && aligned4(lengths), "paged_attn: table and lengths must be 4-byte aligned");
   if (B == 0) return 0;
-  const AttnPlan p = attn_plan(H, Hkv, D, max_pages * page);
+  const AttnPlan p = attn_plan(B, H, Hkv, D, max_pages * page);
   TB_CHECK(aligned16(ws) && (ws != nullptr || p.bytes == 0), "paged_attn: workspace missing or misaligned");
   TB_CHECK(B < (int64_t)1 << 31 && B * Hkv * p.RG < (int64_t)1 << 31 &&
                (double)(B * Hkv * p.RG) * (double)cdiv(std::min<int64_t>(max_pages * page, (int64_t)1 << 31), kTile) < 2e9,
@@ -726,9 +758,7 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   a.stat = (float*)((uint8_t*)ws + p.stat);
   a.desc = (int4*)((uint8_t*)ws + p.desc);
   const hipStream_t st = as_stream(stream);
-  const int64_t units = B * Hkv * p.RG;
-  const int64_t blocks = p.unit ? units : p.blocks;
-#define ATTN(DP_, RT_, WPB_) launch_attn<DP_, RT_, WPB_>(a, p.unit, blocks, st)
+#define ATTN(DP_, RT_, WPB_) launch_attn<DP_, RT_, WPB_>(a, p.unit, p.blocks, st)
   if (p.DP == 64) {
     if (p.RT == 1) ATTN(64, 1, 8);
     else if (p.RT == 2) ATTN(64, 2, 4);
@@ -742,7 +772,7 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
 #undef ATTN
   TB_LAUNCH_CHECK("paged_attn");
   if (!p.unit) {
-    paged_join_kernel<<<dim3((unsigned)blocks, (unsigned)cdiv(p.R * D, 256)), kJoinWaves * 64, 0, st>>>(a);
+    paged_join_kernel<<<dim3((unsigned)p.blocks, (unsigned)cdiv(p.R * D, 256)), kJoinWaves * 64, 0, st>>>(a);
     TB_LAUNCH_CHECK("paged_attn join");
   }
   return 0;

@@ -67,7 +67,7 @@ _SIGS = {
     "tbf16_linear_i8_ws_bytes": (SZ, [I64, I64, I64]),
     "tbf16_linear_i8": (I, [P, I64, I64, I64, P, I64, I64, P, P, P, I64, P, I64, P]),
     "tbf16_paged_write": (I, [P, P] + [I64] * 7 + [P, P, P] + [I64] * 8 + [P]),
-    "tbf16_paged_attn_ws_bytes": (SZ, [I64, I64, I64, I64]),
+    "tbf16_paged_attn_ws_bytes": (SZ, [I64] * 5),
     "tbf16_paged_attn": (I, [P] + [I64] * 6 + [P, P] + [I64] * 8 + [P, I64, I64, P, F, P, P, I64, P]),
 }
 

@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from ._ext import launch, lib, ptr
-from .ops import _bias_bf16, _dev_check
+from .ops import _bias_bf16
 
 # int32 sums of K products of two codes of magnitude at most 127 (TBF16_I8_MAX_K)
 MAX_K = 131072
@@ -27,6 +27,17 @@ MAX_K = 131072
 
 def _up(n, mult):
     return n + (-n) % mult
+
+
+def _device(x, *others) -> int:
+    """The device of x (its index), which the others have to be on too."""
+    dev = x.get_device()
+    if dev < 0:
+        raise ValueError("tbf16: expected tensors on a ROCm (cuda) device")
+    for t in others:
+        if t.get_device() != dev:
+            raise ValueError(f"tbf16.int8_linear: tensors on {t.device} and {x.device}")
+    return dev
 
 
 def _rows(x):
@@ -39,11 +50,11 @@ def quantize_rows_i8(x: torch.Tensor):
     row's max |x|. The exact quotient decides, ties go to even. A row of zeros has scale 0; a
     row with an infinity or a NaN, which 8 bits cannot hold, zero codes and a NaN scale. The
     codes are a view of rows padded with zeros to a multiple of 16."""
-    _dev_check(x)
     if x.dim() != 2:
         raise ValueError(f"tbf16.quantize_rows_i8: expected (R, K), got {tuple(x.shape)}")
     if x.dtype != torch.bfloat16:
         raise TypeError("tbf16.quantize_rows_i8: expected bf16")
+    _device(x)
     R, K = x.shape
     if K > MAX_K:
         raise ValueError(f"tbf16.quantize_rows_i8: K = {K} is above {MAX_K}, int32 sums could overflow")
@@ -62,47 +73,66 @@ def prepare_weight_i8(w: torch.Tensor):
 
 
 def _weight_rows(w8, K):
-    """w8 with rows the kernels read in place: 16-byte aligned and padded to a multiple of
-    16 inside their storage (what prepare_weight_i8 returns); else a padded copy."""
-    N, Kp = w8.shape[0], _up(K, 16)
-    ld = w8.stride(0)
-    if (w8.stride(1) == 1 or K == 1) and ld % 16 == 0 and Kp <= ld < 1 << 23 and w8.data_ptr() % 16 == 0:
-        if Kp == K or w8.untyped_storage().nbytes() >= w8.storage_offset() + (N - 1) * ld + Kp:
+    """w8 with rows the kernels read in place: 16-byte aligned, apart by a multiple of 16 and
+    readable up to K rounded up to 128 or to the next row (what prepare_weight_i8 returns);
+    else a padded copy."""
+    N, ld = w8.shape[0], w8.stride(0)
+    if (w8.stride(1) == 1 or K == 1) and ld % 16 == 0 and K <= ld < 1 << 23 and w8.data_ptr() % 16 == 0:
+        if ld == K or w8.untyped_storage().nbytes() >= w8.storage_offset() + (N - 1) * ld + min(ld, _up(K, 128)):
             return w8
-    return F.pad(w8, (0, Kp - K)) if Kp != K else w8.clone(memory_format=torch.contiguous_format)
+    return F.pad(w8, (0, -K % 16)) if K % 16 else w8.clone(memory_format=torch.contiguous_format)
+
+
+# tbf16_linear_i8's workspace bytes per (device, M, K, N): its choice of kernel counts the
+# device's CUs, so it is asked on the tensors' device, once
+_WS_BYTES: dict = {}
+
+
+def _ws_bytes(dev: int, *sizes: int) -> int:
+    key = (dev, sizes)
+    n = _WS_BYTES.get(key)
+    if n is None:
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        with torch.cuda.device(dev):
+            n = _WS_BYTES[key] = int(lib().tbf16_linear_i8_ws_bytes(*sizes))
+    return n
 
 
 def int8_linear(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias=None):
     """y = x @ W^T + b for bf16 x (..., K), with W given by prepare_weight_i8. Returns bf16
     (..., N). Rows of x with an infinity or a NaN give NaN. Inference only."""
-    _dev_check(x, w8, w_scale)
     if x.dtype != torch.bfloat16:
         raise TypeError("tbf16.int8_linear: expected bf16 x")
     if w8.dtype != torch.int8 or w8.dim() != 2:
         raise TypeError("tbf16.int8_linear: expected an int8 weight (N, K)")
-    K, (N, Kw) = x.shape[-1], w8.shape
+    shape = x.shape
+    if len(shape) == 0:
+        raise ValueError("tbf16.int8_linear: x has no dimension")
+    K, (N, Kw) = shape[-1], w8.shape
     if Kw != K:
         raise ValueError(f"tbf16.int8_linear: x has K={K}, weight has K={Kw}")
     if K > MAX_K:
         raise ValueError(f"tbf16.int8_linear: K = {K} is above {MAX_K}, int32 sums could overflow")
     if w_scale.numel() != N:
         raise ValueError(f"tbf16.int8_linear: {w_scale.numel()} scales for {N} channels")
-    if w8.device != x.device or w_scale.device != x.device:
-        raise ValueError(f"tbf16.int8_linear: x on {x.device}, weight on {w8.device}, scales on {w_scale.device}")
-    shape = x.shape[:-1]
-    b = _bias_bf16(bias, N, x.device)
-    M = math.prod(shape)
+    dev = _device(x, w8, w_scale)
+    b = None if bias is None else _bias_bf16(bias, N, x.device)
+    x2 = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), K)
+    M = x2.shape[0]
     if K == 0:
         y = torch.zeros((M, N), device=x.device, dtype=torch.bfloat16)
-        return (y if b is None else y + b).reshape(*shape, N)
-    x2 = x.reshape(M, K)
+        return (y if b is None else y + b).reshape(*shape[:-1], N)
     Np = _up(N, 8)
-    y = torch.empty((M, Np), device=x.device, dtype=torch.bfloat16)
+    y = x.new_empty((M, Np))
     if M and N:
         x2 = _rows(x2)
-        w8, ws = _weight_rows(w8, K), w_scale.float().contiguous()
-        wsb = lib().tbf16_linear_i8_ws_bytes(M, K, N)
-        work = torch.empty((wsb,), device=x.device, dtype=torch.uint8)
-        launch("tbf16_linear_i8", x2, ptr(x2), M, K, max(x2.stride(0), K), ptr(w8), N, w8.stride(0), ptr(ws), ptr(b), ptr(y),
-               Np, ptr(work), wsb)
-    return (y if Np == N else y[:, :N]).reshape(*shape, N)
+        w8 = _weight_rows(w8, K)
+        ws = w_scale if w_scale.dtype == torch.float32 and w_scale.is_contiguous() else w_scale.float().contiguous()
+        wsb = _ws_bytes(dev, M, K, N)
+        work = x.new_empty(wsb, dtype=torch.uint8) if wsb else None
+        launch("tbf16_linear_i8", x2, x2.data_ptr(), M, K, max(x2.stride(0), K), w8.data_ptr(), N, max(w8.stride(0), K + -K % 16),
+               ws.data_ptr(), ptr(b), y.data_ptr(), Np, ptr(work), wsb)
+    if Np != N:
+        y = y[:, :N]
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], N)

@@ -108,19 +108,19 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
            slots.data_ptr(), kc, vc, pages, page, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
 
 
-# tbf16_paged_attn's workspace bytes per (device, H, Hkv, D, positions a table row covers): its
+# tbf16_paged_attn's workspace bytes per (device, B, H, Hkv, D, positions a table row covers): its
 # blocks are counted by the device's CUs, so it is asked on the tensors' device, once
 _WS_BYTES: dict = {}
 
 
-def _ws_bytes(dev: int, H: int, Hkv: int, D: int, cap: int) -> int:
-    key = (dev, H, Hkv, D, cap)
+def _ws_bytes(dev: int, *sizes: int) -> int:
+    key = (dev, sizes)
     n = _WS_BYTES.get(key)
     if n is None:
         if len(_WS_BYTES) > 4096:
             _WS_BYTES.clear()
         with torch.cuda.device(dev):
-            n = _WS_BYTES[key] = int(lib().tbf16_paged_attn_ws_bytes(H, Hkv, D, cap))
+            n = _WS_BYTES[key] = int(lib().tbf16_paged_attn_ws_bytes(*sizes))
     return n
 
 
@@ -150,7 +150,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return o
-    wsb = _ws_bytes(q.get_device(), H, Hkv, D, n * page)
+    wsb = _ws_bytes(q.get_device(), B, H, Hkv, D, n * page)
     ws = q.new_empty(wsb, dtype=torch.uint8) if wsb else o  # (o: nothing is written there)
     launch("tbf16_paged_attn", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], k_cache.data_ptr(), v_cache.data_ptr(),
            pages, page, k_st[0], k_st[1], k_st[2], v_st[0], v_st[1], v_st[2], page_table.data_ptr(), page_table.stride(0), n,

@@ -278,7 +278,7 @@ int tbf16_quantize_rows_i8(const void* x, int64_t R, int64_t K, int64_t ldx, voi
  * (tbf16_quantize_rows_i8 of the weight): rows 16-byte aligned, ldw % 16 == 0 and at
  * least K rounded up to 16, the last row readable up to min(ldw, K rounded up to 128) (what is
  * there does not matter). bias bf16 (N,) or NULL. y bf16,
- * rows 16-byte aligned, ldy % 8 == 0; columns from N up to N rounded up to 8 are written with
+ * rows 16-byte aligned, ldy % 8 == 0; columns from N up to N rounded up to 8 may be written with
  * values to leave out. workspace: tbf16_linear_i8_ws_bytes(M, K, N) bytes (asked with the
  * stream's device current), 16-byte aligned. No counterpart in the reference. */
 size_t tbf16_linear_i8_ws_bytes(int64_t M, int64_t K, int64_t N);

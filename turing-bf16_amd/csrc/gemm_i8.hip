@@ -65,97 +65,95 @@ __device__ __forceinline__ float row_scale(uint32_t bits) {
   return bits < 0x7f80u ? __uint_as_float(bits << 16) / 127.f : NAN;
 }
 
-// One wave per row. VEC: rows of 16-byte chunks (K % 8 == 0), up to kChunks x 512 values held in
-// registers between the maximum and the codes (one read of x); otherwise value by value. Codes are
-// written up to Kp (zeros past K).
-constexpr int kChunks = 16;
+// One block of 4 waves per row: the row's latency is what a call of few rows waits for (256 x 4096:
+// 6.2 us with a wave per row, Q_BLK us so). VEC: rows of 16-byte chunks (K % 8 == 0), up to 8192
+// values held in registers between the maximum and the codes (one read of x), longer ones read
+// twice; otherwise value by value. Codes are written up to Kp (zeros past K).
+constexpr int kQThreads = 256, kQChunks = 4;
 template <bool VEC>
-__global__ __launch_bounds__(256) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int64_t R, int K, int64_t ldx,
-                                                               uint8_t* __restrict__ y, int64_t ldy, int Kp,
-                                                               float* __restrict__ scale) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= R) return;
-  const uint16_t* xr = x + row * ldx;
-  uint8_t* yr = y + row * ldy;
+__global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int K, int64_t ldx,
+                                                                     uint8_t* __restrict__ y, int64_t ldy, int Kp,
+                                                                     float* __restrict__ scale) {
+  __shared__ uint32_t amax[kQThreads / kWave];
+  const int tid = threadIdx.x;
+  const uint16_t* xr = x + blockIdx.x * ldx;
+  uint8_t* yr = y + blockIdx.x * ldy;
+  auto reduce = [&](uint32_t bits) {
+    bits = wave_max_u(bits);
+    if ((tid & 63) == 0) amax[tid >> 6] = bits;
+    __syncthreads();
+    bits = max(max(amax[0], amax[1]), max(amax[2], amax[3]));
+    if (tid == 0) scale[blockIdx.x] = row_scale(bits);
+    return bits;
+  };
   uint32_t bits = 0;
   if constexpr (VEC) {
     const uint4* src = reinterpret_cast<const uint4*>(xr);
     uint2* dst = reinterpret_cast<uint2*>(yr);
     const int K8 = K >> 3, Kp8 = Kp >> 3;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    if (Kp8 <= kWave * kChunks) {
-      uint4 v[kChunks];
+    constexpr int STEP = kQThreads * kQChunks;
+    uint4 v[kQChunks];
+    auto load = [&](int i0) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        v[c] = zero;
-        if (c * kWave < K8 && lane + c * kWave < K8) v[c] = src[lane + c * kWave];
+      for (int c = 0; c < kQChunks; ++c) {
+        const int i = i0 + tid + c * kQThreads;
+        v[c] = make_uint4(0, 0, 0, 0);
+        if (i < K8) v[c] = src[i];
       }
+    };
+    for (int i = 0; i < K8; i += STEP) {
+      load(i);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        if (c * kWave < K8) bits = max(bits, mag8(v[c]));
-      bits = wave_max_u(bits);
-      const RowCode rc = row_code(row_max(bits));
+      for (int c = 0; c < kQChunks; ++c) bits = max(bits, mag8(v[c]));
+    }
+    bits = reduce(bits);
+    const RowCode rc = row_code(row_max(bits));
+    for (int i0 = 0; i0 < Kp8; i0 += STEP) {
+      if (Kp8 > STEP) load(i0);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        if (c * kWave < Kp8 && lane + c * kWave < Kp8)
-          dst[lane + c * kWave] = bits < 0x7f80u ? codes8(v[c], rc) : make_uint2(0, 0);
-    } else {
-      constexpr int U = 4;
-      for (int i = lane; i < K8; i += U * kWave) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = i + u * kWave < K8 ? src[i + u * kWave] : zero;
-#pragma unroll
-        for (int u = 0; u < U; ++u) bits = max(bits, mag8(v[u]));
-      }
-      bits = wave_max_u(bits);
-      const RowCode rc = row_code(row_max(bits));
-      for (int i = lane; i < Kp8; i += U * kWave) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = i + u * kWave < K8 ? src[i + u * kWave] : zero;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (i + u * kWave < Kp8) dst[i + u * kWave] = bits < 0x7f80u ? codes8(v[u], rc) : make_uint2(0, 0);
+      for (int c = 0; c < kQChunks; ++c) {
+        const int i = i0 + tid + c * kQThreads;
+        if (i < Kp8) dst[i] = bits < 0x7f80u ? codes8(v[c], rc) : make_uint2(0, 0);
       }
     }
   } else {
-    for (int i = lane; i < K; i += kWave) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
-    bits = wave_max_u(bits);
+    for (int i = tid; i < K; i += kQThreads) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
+    bits = reduce(bits);
     const RowCode rc = row_code(row_max(bits));
-    for (int i = lane; i < Kp; i += kWave)
+    for (int i = tid; i < Kp; i += kQThreads)
       yr[i] = i < K && bits < 0x7f80u ? (uint8_t)code_of(bf16_lo(xr[i]), rc) : (uint8_t)0;
   }
-  if (lane == 0) scale[row] = row_scale(bits);
 }
 
 // ---- product of few rows (decoding) -------------------------------------------------------
 //
-// The weight stream bounds it: N K bytes. A block of 8 waves owns 16 T weight rows, its waves take
-// K in turns of 128 bytes (two MFMAs of 64 a row), weights straight from memory into registers, PF
-// turns of a wave in flight; the int32 sums of the waves meet in LDS. A lane's fragment is 16 bytes
-// of weight row l % 16, and the same k of token l % 16 (of MT groups of 16).
-// FUSED: at most kFusedRows tokens, which every block quantises into LDS for itself, while its
-// first weights are on their way: one launch, no workspace. Otherwise the codes come from a pass
-// of their own (padded with zeros to a multiple of 128, so that what lies behind a weight row
-// does not matter).
-constexpr int kFusedRows = 4, kFusedBytes = 1 << 16;
-template <int T, int MT, bool FUSED>
+// At most 16 rows: the weight stream bounds it, N K bytes. A block of 8 waves owns R weight rows, as
+// many as spread the weight over every CU (R <= 16 T; the rest of its last tile loads as zeros,
+// without memory traffic). Its waves take K in turns of 128 bytes (two MFMAs of 64 a row),
+// weights straight from memory into registers, PF turns of a wave in flight; the int32 sums of
+// the waves meet in LDS. A lane's fragment is 16 bytes of weight row l % 16, and the same k of
+// token l % 16.
+// FUSED (1: of a single token, 2): every block quantises the tokens into LDS for itself, while its first weights are on their
+// way: one launch, no workspace (16 x 2560 x 10240: DEC_F us, DEC_S with a pass of its own).
+// Otherwise the codes come from a pass of their own (padded with zeros to a multiple of 128, so
+// that what lies behind a weight row does not matter).
+constexpr int kDecodeRows = 16, kFusedCodes = 16384;
+template <int T, int FUSED>
 __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restrict__ x, int64_t ldx,
                                                         const uint8_t* __restrict__ x8, const float* __restrict__ sx,
                                                         const uint8_t* __restrict__ W, int64_t ldw,
                                                         const float* __restrict__ sw, const uint16_t* __restrict__ bias,
-                                                        uint16_t* __restrict__ y, int64_t ldy, int M, int N, int K) {
+                                                        uint16_t* __restrict__ y, int64_t ldy, int M, int N, int K, int R) {
   constexpr int WAVES = 8, PF = T == 1 ? 8 : T == 2 ? 4 : 3;
   extern __shared__ __align__(16) uint8_t xl[];  // FUSED: [M][Kp + 16] codes
-  __shared__ intx4 red[WAVES][T * MT][64];
-  __shared__ uint32_t amax[kFusedRows][WAVES];
+  __shared__ intx4 red[WAVES][T][64];
+  __shared__ uint32_t amax[WAVES][kDecodeRows];
+  __shared__ float scale[kDecodeRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * T;
+  const int n0 = blockIdx.x * R, nend = min(N, n0 + R);
   const int turns = (K + 127) / 128, Kp = turns * 128;
-  const BufRes wres = make_res(W + (int64_t)n0 * ldw, min<int64_t>((int64_t)(N - n0) * ldw, 0x7fffffff));
+  const BufRes wres = make_res(W + (int64_t)n0 * ldw, (int64_t)(nend - n0) * ldw);  // (below 2^29)
   int woff[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) woff[t] = (16 * t + fr) * (int)ldw + 16 * g;
@@ -170,87 +168,73 @@ __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restri
   for (int u = 0; u < PF; ++u)
     if (wave + u * WAVES < turns) load(w[u], wave + u * WAVES);
 
-  if constexpr (FUSED) {
-    for (int m = 0; m < M; ++m) {
+  if constexpr (FUSED != 0) {
+    const int K8 = K >> 3, Kp8 = Kp >> 3;
+    // `per` waves on a row, 8 / per rows at once
+    const int lg = FUSED == 1 ? 3 : M == 2 ? 2 : M <= 4 ? 1 : 0, per = 1 << lg;
+    const int first = wave >> lg, part = wave & (per - 1), step = per * 64, i0 = part * 64 + lane;
+    for (int m = first; m < (FUSED == 1 ? 1 : M); m += WAVES >> lg) {
       const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
       uint32_t bits = 0;
-      for (int i = tid; i < K >> 3; i += WAVES * 64) bits = max(bits, mag8(src[i]));
+#pragma unroll 4
+      for (int i = i0; i < K8; i += step) bits = max(bits, mag8(src[i]));
       bits = wave_max_u(bits);
-      if (lane == 0) amax[m][wave] = bits;
+      if (lane == 0) amax[part][m] = bits;
     }
     __syncthreads();
-    for (int m = 0; m < M; ++m) {
+    for (int m = first; m < (FUSED == 1 ? 1 : M); m += WAVES >> lg) {
       const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
-      uint32_t bits = amax[m][0];
+      uint32_t bits = amax[0][m];
 #pragma unroll
-      for (int i = 1; i < WAVES; ++i) bits = max(bits, amax[m][i]);
+      for (int i = 1; i < WAVES; ++i) bits = max(bits, i < per ? amax[i][m] : 0u);
       const RowCode rc = row_code(row_max(bits));
-      for (int i = tid; i < Kp >> 3; i += WAVES * 64) {
+#pragma unroll 4
+      for (int i = i0; i < Kp8; i += step) {
         uint2 c = make_uint2(0, 0);
-        if (i < K >> 3 && bits < 0x7f80u) c = codes8(src[i], rc);
+        if (i < K8 && bits < 0x7f80u) c = codes8(src[i], rc);
         *reinterpret_cast<uint2*>(xl + m * (Kp + 16) + 8 * i) = c;
       }
+      if (i0 == 0) scale[m] = row_scale(bits);
     }
     __syncthreads();
   }
   // tokens past M take the last one's codes and are not stored
-  const uint8_t* xr[MT];
+  const int mr = FUSED == 1 ? 0 : min(fr, M - 1);
+  const uint8_t* xr = (FUSED ? xl + mr * (Kp + 16) : x8 + (int64_t)mr * Kp) + 16 * g;
+  intx4 acc[T];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int m = min(16 * j + fr, M - 1);
-    xr[j] = (FUSED ? xl + m * (Kp + 16) : x8 + (int64_t)m * Kp) + 16 * g;
-  }
-  intx4 acc[T][MT];
-#pragma unroll
-  for (int t = 0; t < T; ++t)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[t][j] = intx4{0, 0, 0, 0};
+  for (int t = 0; t < T; ++t) acc[t] = intx4{0, 0, 0, 0};
   for (int t0 = wave; t0 < turns; t0 += PF * WAVES) {
 #pragma unroll
     for (int u = 0; u < PF; ++u) {
       const int turn = t0 + u * WAVES;
       if (turn >= turns) break;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        const intx4 xf = *reinterpret_cast<const intx4*>(xr + turn * 128 + 64 * s);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const intx4 xf = *reinterpret_cast<const intx4*>(xr[j] + turn * 128 + 64 * s);
-#pragma unroll
-          for (int t = 0; t < T; ++t) acc[t][j] = I8Op::mma(__builtin_bit_cast(intx4, w[u][t][s]), xf, acc[t][j]);
-        }
+        for (int t = 0; t < T; ++t) acc[t] = I8Op::mma(__builtin_bit_cast(intx4, w[u][t][s]), xf, acc[t]);
+      }
       if (turn + PF * WAVES < turns) load(w[u], turn + PF * WAVES);
     }
   }
 #pragma unroll
-  for (int t = 0; t < T; ++t)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) red[wave][t * MT + j][lane] = acc[t][j];
+  for (int t = 0; t < T; ++t) red[wave][t][lane] = acc[t];
   __syncthreads();
-  const int Np = (N + 7) / 8 * 8;
-  for (int i = tid; i < T * MT * 64; i += WAVES * 64) {
-    const int blk = i >> 6, ln = i & 63;
-    const int m = 16 * (blk % MT) + (ln & 15), n = n0 + 16 * (blk / MT) + 4 * (ln >> 4);
-    if (m >= M || n >= Np) continue;
-    intx4 v = red[0][blk][ln];
+  if (tid >= T * 64) return;
+  const int t = tid >> 6, m = lane & 15, n = n0 + 16 * t + 4 * g;
+  if (m >= M || n >= (nend + 3) / 4 * 4) return;
+  intx4 v = red[0][t][lane];
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) v += red[k][blk][ln];
-    float sa;
-    if constexpr (FUSED) {
-      uint32_t bits = amax[m][0];
+  for (int k = 1; k < WAVES; ++k) v += red[k][t][lane];
+  const float sa = (FUSED ? scale[m] : sx[m]) * I8Op::kA;
+  float f[4];
 #pragma unroll
-      for (int k = 1; k < WAVES; ++k) bits = max(bits, amax[m][k]);
-      sa = row_scale(bits) * I8Op::kA;
-    } else {
-      sa = sx[m] * I8Op::kA;
-    }
-    float f[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = min(n + e, N - 1);
-      f[e] = fmaf((float)v[e] * sa, sw[c] * I8Op::kB, bias ? bf16_lo(bias[c]) : 0.f);
-    }
-    *reinterpret_cast<uint2*>(y + (int64_t)m * ldy + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+  for (int e = 0; e < 4; ++e) {
+    const int c = min(n + e, N - 1);
+    f[e] = fmaf((float)v[e] * sa, sw[c] * I8Op::kB, bias ? bf16_lo(bias[c]) : 0.f);
   }
+  *reinterpret_cast<uint2*>(y + (int64_t)m * ldy + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
 }
 
 // ---- product of many rows -------------------------------------------------------------------
@@ -312,7 +296,7 @@ constexpr size_t kSplitBytes = (size_t)16 << 20;
 // How a call runs.
 struct Plan {
   enum Form { kFused, kDecode, kTiled } form;
-  int T, MT;          // decode kernel
+  int T, R;           // decode kernel: R weight rows a block in T tiles of 16
   int tile, splits;   // tile kernels
   size_t scale, x8, part, bytes;  // workspace
 };
@@ -320,11 +304,11 @@ struct Plan {
 Plan plan_of(int64_t M, int64_t K, int64_t N, bool vec) {
   Plan p{Plan::kTiled, 1, 1, 0, 1, 0, 0, 0, 0};
   const int64_t Kp = (int64_t)align_up((size_t)K, 128), Np = (int64_t)align_up((size_t)N, 8), cus = num_cus();
-  if (M <= 64) {
-    p.MT = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    p.T = (int)std::min<int64_t>(p.MT == 4 ? 2 : 4, std::max<int64_t>(1, cdiv(cdiv(N, 16), cus)));
+  if (M <= kDecodeRows) {
+    p.R = (int)std::min<int64_t>(64, std::max<int64_t>(8, cdiv(cdiv(N, cus), 8) * 8));
+    p.T = (int)cdiv(p.R, 16);
     p.form = Plan::kDecode;
-    if (vec && M <= kFusedRows && M * (Kp + 16) <= kFusedBytes) {
+    if (vec && M * Kp <= (M <= 2 ? 4 : 1) * kFusedCodes) {
       p.form = Plan::kFused;
       return p;
     }
@@ -373,11 +357,11 @@ bool rows_vec(const void* x, int64_t K, int64_t ldx) { return K % 8 == 0 && ldx 
 
 int launch_quantize_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, int64_t Kp, float* scale,
                        hipStream_t st) {
-  const unsigned blocks = (unsigned)cdiv(R, 4);
+  const unsigned rows = (unsigned)R;
   if (rows_vec(x, K, ldx))
-    quantize_rows_i8_kernel<true><<<blocks, 256, 0, st>>>((const uint16_t*)x, R, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
+    quantize_rows_i8_kernel<true><<<rows, kQThreads, 0, st>>>((const uint16_t*)x, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
   else
-    quantize_rows_i8_kernel<false><<<blocks, 256, 0, st>>>((const uint16_t*)x, R, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
+    quantize_rows_i8_kernel<false><<<rows, kQThreads, 0, st>>>((const uint16_t*)x, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
   TB_LAUNCH_CHECK("quantize_rows_i8");
   return 0;
 }
@@ -432,27 +416,23 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
   if (p.form != Plan::kFused)
     if (int rc = launch_quantize_i8(x, M, K, ldx, x8, Kp, Kp, sx, st)) return rc;
   if (p.form != Plan::kTiled) {
-    const unsigned blocks = (unsigned)cdiv(N, 16 * p.T);
-#define DECODE(T_, MT_, FUSED_)                                                                                       \
-  decode_i8_kernel<T_, MT_, FUSED_><<<blocks, 512, FUSED_ ? (size_t)(M * (Kp + 16)) : 0, st>>>(                             \
-      (const uint16_t*)x, ldx, x8, sx, (const uint8_t*)w8, ldw, ws, bi, yo, ldy, (int)M, (int)N, (int)K)
-#define DECODE_T(MT_, FUSED_)                \
-  switch (p.T) {                             \
-    case 1: DECODE(1, MT_, FUSED_); break;   \
-    case 2: DECODE(2, MT_, FUSED_); break;   \
-    case 3: DECODE(3, MT_, FUSED_); break;   \
-    default: DECODE(4, MT_, FUSED_); break;  \
+    const unsigned blocks = (unsigned)cdiv(N, p.R);
+#define DECODE(T_, FUSED_)                                                                                   \
+  decode_i8_kernel<T_, FUSED_><<<blocks, 512, FUSED_ ? (size_t)(M * (Kp + 16)) : 0, st>>>(                   \
+      (const uint16_t*)x, ldx, x8, sx, (const uint8_t*)w8, ldw, ws, bi, yo, ldy, (int)M, (int)N, (int)K, p.R)
+#define DECODE_T(FUSED_)                \
+  switch (p.T) {                        \
+    case 1: DECODE(1, FUSED_); break;   \
+    case 2: DECODE(2, FUSED_); break;   \
+    case 3: DECODE(3, FUSED_); break;   \
+    default: DECODE(4, FUSED_); break;  \
   }
-    if (p.form == Plan::kFused) {
-      DECODE_T(1, true)
-    } else if (p.MT == 1) {
-      DECODE_T(1, false)
-    } else if (p.MT == 2) {
-      DECODE_T(2, false)
-    } else if (p.T == 1) {
-      DECODE(1, 4, false);
+    if (p.form == Plan::kDecode) {
+      DECODE_T(0)
+    } else if (M == 1) {
+      DECODE_T(1)
     } else {
-      DECODE(2, 4, false);
+      DECODE_T(2)
     }
 #undef DECODE_T
 #undef DECODE

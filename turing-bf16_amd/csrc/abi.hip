@@ -14,6 +14,18 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+int64_t num_cus() {
+  static int64_t cache[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cache[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
+
 }  // namespace tbf16
 
 extern "C" int tbf16_abi_version(void) { return TBF16_ABI_VERSION; }

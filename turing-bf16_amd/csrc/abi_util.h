@@ -12,6 +12,9 @@ namespace tbf16 {
 
 void set_error(const char* fmt, ...);
 
+// Compute units of the current device (cached per device).
+int64_t num_cus();
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }

@@ -1039,19 +1039,6 @@ constexpr TileCfg kCfgs[] = {{256, 256, 32}, {128, 128, 64}, {64, 64, 64},      
 constexpr int kNumCfgs = 31;
 constexpr int64_t kMaxRowTiles = 65536;  // fewer tiles than this along M
 
-// Compute units of the current device (cached per device).
-int64_t num_cus() {
-  static int64_t cache[64] = {};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cache[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev] = n;
-  }
-  return cache[dev];
-}
-
 // Split K in two for a pinned tile configuration that converts x in the GEMM or takes
 // x16 (workspace entry points): where it leaves at least half the CUs without a tile,
 // K >= 2048 and the fp32 partial sums take at most kSplitPartBytes, two blocks per

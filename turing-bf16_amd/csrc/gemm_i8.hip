@@ -265,18 +265,6 @@ __global__ __launch_bounds__(256) void splitk_i8_kernel(const intx4* __restrict_
                                              pack_bf16(f[6], f[7])));
 }
 
-int64_t num_cus() {
-  static int64_t cache[64] = {};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cache[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev] = n;
-  }
-  return cache[dev];
-}
-
 // The tile kernels (gemm_tiles.h), and the estimate of their times: a round of at most CU-count
 // blocks takes c1 + k tiles x slope us, the slope from `light` (few blocks) to `full`.
 struct Tile {

@@ -21,25 +21,64 @@ struct CacheGeom {
 
 // ---- write ------------------------------------------------------------------------
 
-// One wave per token: its 16-byte chunks of all heads, keys then values. A slot that a
-// later token names too is left to that token, so a repeated slot holds the last one's
-// whole row whatever the order of the waves.
+// A copy, bound by memory. A block takes TB tokens: a thread one 16-byte chunk of the keys' or values'
+// heads, over the block's tokens (W threads a token, so 256 / W tokens at once).
+// A slot that a later token names too is left to that token, so a repeated slot holds the last one's
+// whole rows whatever the order of the blocks: the block marks its slots in a small table of bits and
+// looks up every later token's slot there, those that hit it in full. Longer lists than kWriteTokens
+// are written by launches in turn, which keeps that search short.
+constexpr int kWriteBlock = 16, kWriteTokens = 16384;
 __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                           int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
-                                                          const int32_t* __restrict__ slots, int T, int Hkv, int D8,
-                                                          uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
-                                                          CacheGeom kg, CacheGeom vg, int64_t n_slots, int page) {
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (t >= T) return;
-  const int slot = slots[t];
-  if (slot < 0 || slot >= n_slots) return;
-  for (int u = t + 1 + lane; __any(u < T); u += 64)
-    if (__any(u < T && slots[u] == slot)) return;
-  const int64_t p = slot / page, r = slot % page;
-  for (int i = lane; i < Hkv * D8; i += 64) {
-    const int h = i / D8, c = i % D8 * 8;
-    stg16(kc + p * kg.sp + h * kg.sh + r * kg.ss + c, ldg16(k + t * k_st + h * k_sh + c));
-    stg16(vc + p * vg.sp + h * vg.sh + r * vg.ss + c, ldg16(v + t * v_st + h * v_sh + c));
+                                                          const int32_t* __restrict__ slots, int T, int TB, int C, int D8,
+                                                          int W, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc,
+                                                          CacheGeom kg, CacheGeom vg, int n_slots, int page) {
+  __shared__ int mine[kWriteBlock];  // the block's slots, -1: nowhere
+  __shared__ int64_t koff[kWriteBlock], voff[kWriteBlock];
+  __shared__ uint32_t named[64];
+  const int tid = threadIdx.x, t0 = blockIdx.x * TB, nt = min(TB, T - t0);
+  if (tid < 64) named[tid] = 0;
+  int slot = -1;
+  if (tid < nt) {
+    slot = slots[t0 + tid];
+    if (slot >= n_slots) slot = -1;
+    const int p = slot / page, r = slot % page;
+    mine[tid] = slot;
+    koff[tid] = p * kg.sp + r * kg.ss;
+    voff[tid] = p * vg.sp + r * vg.ss;
+  }
+  __syncthreads();
+  if (slot >= 0) atomicOr(&named[(slot >> 5) & 63], 1u << (slot & 31));
+  __syncthreads();
+  constexpr int U = 4;
+  for (int u0 = t0 + 1 + tid; u0 < T; u0 += 256 * U) {
+    int s[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) s[i] = u0 + 256 * i < T ? slots[u0 + 256 * i] : -1;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (s[i] >= 0 && (named[(s[i] >> 5) & 63] >> (s[i] & 31) & 1))
+        for (int t = 0; t < nt; ++t)
+          if (mine[t] == s[i] && t0 + t < u0 + 256 * i) mine[t] = -1;  // (every thread that writes it writes this)
+  }
+  __syncthreads();
+  for (int j = tid & (W - 1); j < 2 * C; j += W) {
+    const bool is_v = j >= C;
+    const int e = is_v ? j - C : j, h = e / D8, c = (e - h * D8) * 8;
+    const uint16_t* src = (is_v ? v + t0 * v_st + h * v_sh : k + t0 * k_st + h * k_sh) + c;
+    uint16_t* dst = (is_v ? vc + h * vg.sh : kc + h * kg.sh) + c;
+    const int64_t st = is_v ? v_st : k_st;
+    const int64_t* off = is_v ? voff : koff;
+    const int step = 256 / W;
+    for (int t = tid / W; t < nt; t += U * step) {
+      uint4 x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (t + i * step < nt && mine[t + i * step] >= 0) x[i] = ldg16(src + (t + i * step) * st);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (t + i * step < nt && mine[t + i * step] >= 0) stg16(dst + off[t + i * step], x[i]);
+    }
   }
 }
 
@@ -611,18 +650,6 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a)
       make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
 }
 
-int64_t num_cus() {
-  static int64_t cache[64] = {};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cache[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev] = n;
-  }
-  return cache[dev];
-}
-
 // How a call is split: head dim DP, RT blocks of 16 rows a unit, wpb waves a block, blocks of
 // the list form, and the workspace for what they share.
 struct AttnPlan {
@@ -690,11 +717,20 @@ extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_
   TB_CHECK(T >= 0 && T < (int64_t)1 << 31, "paged_write: bad number of tokens");
   TB_CHECK(aligned16(k) && aligned16(v) && aligned4(slots), "paged_write: k and v must be 16-byte aligned");
   TB_CHECK(k_st % 8 == 0 && k_sh % 8 == 0 && v_st % 8 == 0 && v_sh % 8 == 0, "paged_write: strides must be multiples of 8");
+  TB_CHECK(pages * page < (int64_t)1 << 31, "paged_write: more slots than int32 counts");
   if (T == 0 || pages == 0) return 0;
-  paged_write_kernel<<<(unsigned)cdiv(T, 4), 256, 0, as_stream(stream)>>>(
-      (const uint16_t*)k, (const uint16_t*)v, k_st, k_sh, v_st, v_sh, slots, (int)T, (int)Hkv, (int)(D / 8),
-      (uint16_t*)k_cache, (uint16_t*)v_cache, kg, vg, pages * page, (int)page);
-  TB_LAUNCH_CHECK("paged_write");
+  const int C = (int)(Hkv * (D / 8));
+  int W = 1;
+  while (W < 256 && W < 2 * C) W *= 2;
+  for (int64_t t = 0; t < T; t += kWriteTokens) {
+    const int n = (int)std::min<int64_t>(kWriteTokens, T - t);
+    // at least 4 blocks a CU as long as there are tokens
+    const int TB = (int)std::min<int64_t>(kWriteBlock, std::max<int64_t>(256 / W, n / (4 * num_cus())));
+    paged_write_kernel<<<(unsigned)cdiv(n, TB), 256, 0, as_stream(stream)>>>(
+        (const uint16_t*)k + t * k_st, (const uint16_t*)v + t * v_st, k_st, k_sh, v_st, v_sh, slots + t, n, TB, C, (int)(D / 8),
+        W, (uint16_t*)k_cache, (uint16_t*)v_cache, kg, vg, (int)(pages * page), (int)page);
+    TB_LAUNCH_CHECK("paged_write");
+  }
   return 0;
 }
 

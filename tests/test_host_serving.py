@@ -127,7 +127,7 @@ def test_abi_refusals():
     def attn(B=1, H=2, Hkv=2, D=64, qs=s2, kc=16, vc=16, pages=4, page=16, ks=s3, vs=s3, ws=16, wsb=None, q=16):
         if wsb is None:
             wsb = 1 << 40
-        return L.tbf16_paged_attn(q, B, H, Hkv, D, *qs, kc, vc, pages, page, *ks, *vs, 16, 200, 200, 16, 1.0, 16, ws, wsb, None)
+        return L.tbf16_paged_attn(q, B, H, Hkv, D, *qs, kc, vc, pages, page, *ks, *vs, 16, 400, 400, 16, 1.0, 16, ws, wsb, None)
 
     for bad, text in [(dict(H=3), "multiple of key/value heads"), (dict(D=60), "multiple of 8"), (dict(D=264), "256"),
                       (dict(kc=18), "aligned"), (dict(ks=odd3), "strides"), (dict(qs=odd2), "q must"), (dict(q=24), "q must"),
@@ -137,7 +137,7 @@ def test_abi_refusals():
         assert text in err(), (bad, err())
     assert attn(B=64, H=64, Hkv=2, D=128, wsb=0) == -3 and "workspace" in err()
     assert attn(B=0) == 0
-    assert L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 100) == 0 < L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 3200)
+    assert L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 100) == 0 < L.tbf16_paged_attn_ws_bytes(1, 64, 2, 128, 6400)
 
     def write(T=2, ks=s2, kc=16, cs=s3, D=64, k=16, pages=4):
         return L.tbf16_paged_write(k, 16, T, 2, D, *ks, *s2, 16, kc, 16, pages, 16, *cs, *s3, None)

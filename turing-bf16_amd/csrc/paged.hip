@@ -349,6 +349,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
 
   Cursor cur;
   int n;  // this wave's tiles
+  int per = 0;  // UNIT: tiles of a wave
   uint32_t c = 0, act = WPB;
   if constexpr (UNIT) {
     cur.b = blockIdx.x;
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     cur.grp = blockIdx.z;
     cur.len = uniform(seq_len(a, cur.b));
     cur.nt = (cur.len + kTile - 1) / kTile;
-    const int per = (cur.nt + WPB - 1) / WPB;
+    per = (cur.nt + WPB - 1) / WPB;
     cur.tile = min(wave * per, cur.nt);
     n = min(per, cur.nt - cur.tile);
   } else {
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     cur = r.at;
     if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
-  if (lane == 0) flags[wave] = 0;
+  if (!UNIT && lane == 0) flags[wave] = 0;
 
   Acc<DP, RT> acc;
   bool tail = false;  // acc is the begin of a unit that goes on in the next wave
@@ -537,12 +538,16 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
         ++cur.tile;
         continue;
       }
+      acc.total();
+      if constexpr (UNIT) {
+        acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, unit_rows(a, cur.grp), a.D, lane);
+        break;
+      }
       const Cursor done = cur;
       if (more) {  // the next unit's q is on its way while this unit leaves
         advance(a, cur);
         load_q(cur);
       }
-      acc.total();
       if (begun && end) {
         acc.finish(unit_out(a, done.b, done.head, done.grp), unit_rows(a, done.grp), a.D, lane);
       } else if (!begun) {
@@ -557,6 +562,33 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     }
   }
   __syncthreads();
+  if constexpr (UNIT) {
+    // the waves' parts, a thread 4 outputs of a row
+    const int rows = unit_rows(a, cur.grp), dg = a.D / 4;
+    const int parts = cur.nt ? (cur.nt + per - 1) / per : 0;
+    uint16_t* out = unit_out(a, cur.b, cur.head, cur.grp);
+    for (int e = threadIdx.x; e < rows * dg; e += WPB * 64) {
+      const int row = e / dg, d = (e - row * dg) * 4;
+      float2 st[WPB];
+      float m = kNone, l = 0.f;
+      floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WPB; ++w) {
+        st[w] = w < parts ? *reinterpret_cast<const float2*>(stat0 + (w * a.R + row) * 2) : make_float2(kNone, 0.f);
+        m = fmaxf(m, st[w].x);
+      }
+#pragma unroll
+      for (int w = 0; w < WPB; ++w)
+        if (w < parts) {
+          const float f = ex2(st[w].x - m);
+          l = fmaf(f, st[w].y, l);
+          o += f * *reinterpret_cast<const floatx4*>(lds + (w * a.R + row) * ld + d);
+        }
+      const float f = m == kNone ? 0.f : 1.f / l;  // no key at all: zeros
+      *reinterpret_cast<uint2*>(out + (int64_t)row * a.D + d) = make_uint2(pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f));
+    }
+    return;
+  }
   // joins inside the block: a wave that began a unit takes what the waves after it left, the
   // first wave what they left of a unit begun in an earlier block
   const int64_t slot = (int64_t)blockIdx.x * 2;
@@ -574,31 +606,23 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     if (wave + 1 < (int)act) take(wave + 1);
     if (ended) {
       acc.finish(unit_out(a, cur.b, cur.head, cur.grp), unit_rows(a, cur.grp), a.D, lane);
-    } else if constexpr (!UNIT) {
+    } else {
       acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
       // the unit's last tile: this wave's last one is its tile cur.tile
       const uint32_t end = (blockIdx.x * act + wave) * c + n - 1 - cur.tile + cur.nt - 1;
       if (lane == 0) a.desc[blockIdx.x] = make_int4(cur.b, cur.head, end / (c * act), cur.grp + 1);
     }
   }
-  if constexpr (UNIT) {
-    if (cur.nt == 0) {  // a sequence without keys
-      const int chunks = unit_rows(a, cur.grp) * a.D / 8;
-      for (int i = threadIdx.x; i < chunks; i += WPB * 64)
-        stg16(unit_out(a, cur.b, cur.head, cur.grp) + 8 * i, make_uint4(0, 0, 0, 0));
-    }
-  } else {
-    if (wave == 0 && uniform(flags[0]) != 0) {
-      acc.clear();
-      span(0);
-      take(0);
-      acc.put(a.part + slot * a.R * a.D, a.D, a.stat + slot * a.R * 2, a.R, a.D, lane);
-    }
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-      if (uniform(seq_len(a, b)) == 0)
-        for (int i = threadIdx.x; i < a.H * a.D / 8; i += WPB * 64)
-          stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
+  if (wave == 0 && uniform(flags[0]) != 0) {
+    acc.clear();
+    span(0);
+    take(0);
+    acc.put(a.part + slot * a.R * a.D, a.D, a.stat + slot * a.R * 2, a.R, a.D, lane);
   }
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
+    if (uniform(seq_len(a, b)) == 0)
+      for (int i = threadIdx.x; i < a.H * a.D / 8; i += WPB * 64)
+        stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
 }
 
 // The join between blocks: for the unit that block blockIdx.x of the list began and did not end,
@@ -666,7 +690,10 @@ AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   p.R = (int)std::min<int64_t>(G, 16 * p.RT);
   p.RG = (int)cdiv(G, p.R);
   p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
-  p.unit = cdiv(cap, kTile) <= 2 * p.wpb && B * Hkv * p.RG <= num_cus();
+  // Few short units: a launch less on the host and on the device (1 x 32 heads, 100 keys: 5.2 us, the
+  // list and its join 8.7); with more tiles a wave the list's finer split wins (700 keys of 16 heads, 3
+  // tiles a wave: 10.9 and 9.6 us on the device, 14 and 17 with the host; 1000 keys, 4 tiles: 15.4 and 13.1)
+  p.unit = cdiv(cap, kTile) <= 3 * p.wpb && B * Hkv * p.RG <= num_cus();
   p.stat = p.desc = p.bytes = 0;
   p.blocks = 0;
   if (p.unit) return p;

@@ -76,6 +76,13 @@ ATTEND = [  # H, Hkv, D, page, lengths
     (32, 8, 128, 16, [4096, 1, 2000, 3]),
     (4, 1, 128, 128, [20000]),
     (16, 8, 24, 3, [50] * 70),
+    # rows of heads in several units, in both forms of the split
+    (130, 2, 64, 16, [2000, 7]),
+    (24, 1, 128, 32, [90, 300]),
+    (80, 2, 128, 16, [1200, 31]),
+    (40, 1, 256, 16, [900, 45]),
+    (3, 1, 200, 16, [100, 7]),
+    (8, 4, 200, 16, [3000, 7, 0, 900]),
 ]
 
 
@@ -92,6 +99,35 @@ def test_attend_many_short(dev, B, lengths_of):
     k, v, table, ln = make_cache(dev, lengths, 2, 64, 16, seed=B)
     q = torch.randn(B, 4, 64, generator=gen(2)).to(BF).to(dev)
     check_attend(q, k, v, table, ln)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_attend_random_batches(dev, seed):
+    """Where the runs of the waves and blocks begin and end in the batch."""
+    r = __import__("random").Random(seed)
+    B = r.choice((1, 2, 3, 9, 40, 150))
+    Hkv, D, page = r.choice((1, 2, 5)), r.choice((8, 64, 72, 128)), r.choice((1, 5, 16, 33, 64))
+    top = r.choice((33, 200, 1500)) if B > 9 else r.choice((40, 700, 6000))
+    lengths = [r.choice((0, 1, r.randrange(top), r.randrange(top), 32 * r.randrange(1, top // 32 + 1))) for _ in range(B)]
+    H = Hkv * r.choice((1, 3, 4, 8, 17))
+    k, v, table, ln = make_cache(dev, lengths, Hkv, D, page, seed=seed)
+    q = torch.randn(B, H, D, generator=gen(seed)).to(BF).to(dev)
+    check_attend(q, k, v, table, ln)
+    wide = torch.full((B, table.shape[1] + 5000 // page), -1, dtype=torch.int32, device=dev)  # room for long ones
+    wide[:, :table.shape[1]] = table
+    check_attend(q, k, v, wide, ln)
+
+
+def test_attend_very_many_sequences(dev):
+    B = 70000
+    k = torch.randn(50, 1, 4, 8, generator=gen(1)).to(BF).to(dev)
+    table = torch.randint(0, 50, (B, 2), generator=gen(2), dtype=torch.int32).to(dev)
+    ln = torch.randint(0, 9, (B,), generator=gen(3), dtype=torch.int32).to(dev)
+    q = torch.randn(B, 2, 8, generator=gen(4)).to(BF).to(dev)
+    o = tbf16.paged_sdpa(q, k, k, table, ln)
+    at = torch.cat((torch.arange(40), torch.randint(0, B, (100,), generator=gen(5)), torch.arange(B - 40, B)))
+    ref, bound = paged_sdpa64(q[at], k, k, table[at], ln[at])
+    assert ((o[at].cpu().double() - ref).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.5, 3.0, 1e-3])
@@ -474,6 +510,28 @@ def test_linear_rows_alone(dev):
     y = tbf16.int8_linear(x, w8, ws)
     for n in (1, 2, 3, 16, 17, 64, 100, 128, 300):
         assert torch.equal(y[:n], tbf16.int8_linear(x[:n], w8, ws)), n
+
+
+def test_linear_far_offsets(dev):
+    """Outputs and weights past 2^31 elements and bytes."""
+    g = gen(10)
+    x = torch.randn(40000, 64, generator=g).to(BF).to(dev)
+    w = torch.randn(65536, 64, generator=g).to(BF).to(dev)
+    y = tbf16.int8_linear(x, *tbf16.prepare_weight_i8(w))
+    m, n = torch.tensor([0, 1, 20000, 32767, 32768, 39999]), torch.tensor([0, 7, 255, 256, 40000, 65535])
+    ref, bound = int8_linear64(x[m], w[n])
+    assert ((y[m][:, n].cpu().double() - ref).abs() <= bound).all()
+    del x, w, y
+    K, N = 65536, 40000
+    w8 = torch.randint(-127, 128, (N, K), dtype=torch.int8, device=dev)  # 2.6e9 bytes
+    ws = torch.ones(N, device=dev)
+    n = torch.tensor([0, 1, 32767, 32768, 39998, 39999])
+    for M in (1, 3, 200):
+        x = torch.randn(M, K, generator=g).to(BF)
+        y = tbf16.int8_linear(x.to(dev), w8, ws)
+        cx, sx = codes64(x)
+        ref = (cx @ w8[n].cpu().double().t()) * sx
+        assert ((y[:, n].cpu().double() - ref).abs() <= 2.0 ** -8 * ref.abs() * (1 + 2.0 ** -10) + 6 * 2.0 ** -24 * ref.abs()).all()
 
 
 # ---- streams, graphs, modules -------------------------------------------------------------

@@ -66,7 +66,7 @@ __device__ __forceinline__ float row_scale(uint32_t bits) {
 }
 
 // One block of 4 waves per row: the row's latency is what a call of few rows waits for (256 x 4096:
-// 6.2 us with a wave per row, Q_BLK us so). VEC: rows of 16-byte chunks (K % 8 == 0), up to 8192
+// 6.2 us with a wave per row, 4.2 us so; 4096 x 4096, bound by memory: 12.4 and 11.1 us, 4.5 TB/s). VEC: rows of 16-byte chunks (K % 8 == 0), up to 8192
 // values held in registers between the maximum and the codes (one read of x), longer ones read
 // twice; otherwise value by value. Codes are written up to Kp (zeros past K).
 constexpr int kQThreads = 256, kQChunks = 4;
@@ -133,10 +133,14 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
 // weights straight from memory into registers, PF turns of a wave in flight; the int32 sums of
 // the waves meet in LDS. A lane's fragment is 16 bytes of weight row l % 16, and the same k of
 // token l % 16.
-// FUSED (1: of a single token, 2): every block quantises the tokens into LDS for itself, while its first weights are on their
-// way: one launch, no workspace (16 x 2560 x 10240: DEC_F us, DEC_S with a pass of its own).
+// FUSED (1: of a single token, 2): every block quantises the tokens into LDS for itself, while its
+// first weights are on their way: one launch, no workspace (1 x 4096 x 4096: 6.4 us, 8.8 with a pass
+// of its own; 4 x 4096 x 4096: 8.1 and 9.0; 1 x 32768 x 2048: 21 and 31), up to kFusedCodes values,
+// of one or two tokens four times that; above them the blocks' repeated work costs more than the pass
+// (16 x 4096 x 4096: 15.6 and 10.0; 8 x 4096 x 4096: 10.3 and 9.6).
 // Otherwise the codes come from a pass of their own (padded with zeros to a multiple of 128, so
 // that what lies behind a weight row does not matter).
+// 1 x 2560 x 10240: 8.4 us, 3.1 TB/s of weights; 16 tokens: 7.7 us after a pass of 3.4.
 constexpr int kDecodeRows = 16, kFusedCodes = 16384;
 template <int T, int FUSED>
 __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restrict__ x, int64_t ldx,
@@ -266,7 +270,12 @@ __global__ __launch_bounds__(256) void splitk_i8_kernel(const intx4* __restrict_
 }
 
 // The tile kernels (gemm_tiles.h), and the estimate of their times: a round of at most CU-count
-// blocks takes c1 + k tiles x slope us, the slope from `light` (few blocks) to `full`.
+// blocks takes c1 + k tiles x slope us, the slope from `light` (few blocks) to `full`, a k tile being
+// 128 integers; splitting K over s blocks a tile adds the partial sums' round trip and a launch.
+// The figures are those of the fp16 kernels by 128 bytes of k: the MFMAs take as long, and so do
+// LDS and L2, which bound both. On 30 shapes (M 16 to 8192) the tile they pick is the best one's time
+// but for 1% on average, 7% at most. 4096^3: 52 us, 2640 TOPS, MFMAs busy 0.56 at 2.2 GHz (LDS traffic:
+// a 64-deep step of a wave's 128 x 64 tile reads 192 rows for 32 MFMAs).
 struct Tile {
   int bm, bn;
   bool ksplit;

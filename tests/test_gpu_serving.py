@@ -302,7 +302,7 @@ def test_write(dev, T, Hkv, D, page):
     assert torch.equal(kv.view(torch.int16), want.view(torch.int16))
 
 
-@pytest.mark.parametrize("T,distinct", [(2, 1), (64, 5), (1000, 400), (9000, 8000), (20000, 1)])
+@pytest.mark.parametrize("T,distinct", [(2, 1), (64, 5), (1000, 400), (9000, 8000), (20000, 1), (70000, 66000), (140000, 70000)])
 def test_write_repeated_slots(dev, T, distinct):
     """The last token of a slot stays, keys and values both."""
     g = gen(T)

@@ -65,25 +65,32 @@ __device__ __forceinline__ float row_scale(uint32_t bits) {
   return bits < 0x7f80u ? __uint_as_float(bits << 16) / 127.f : NAN;
 }
 
-// One block of 4 waves per row: the row's latency is what a call of few rows waits for (256 x 4096:
-// 6.2 us with a wave per row, 4.2 us so; 4096 x 4096, bound by memory: 12.4 and 11.1 us, 4.5 TB/s). VEC: rows of 16-byte chunks (K % 8 == 0), up to 8192
-// values held in registers between the maximum and the codes (one read of x), longer ones read
+// TPR threads per row: a block of 4 waves (the row's latency is what a call of few rows waits for: 256 x
+// 4096 6.2 us with a wave per row, 4.2 us so; 4096 x 4096, bound by memory: 12.4 and 11.1 us, 4.5 TB/s),
+// or a wave where there are many rows of up to 2048 values (7363 x 448 with its product: 19.0 -> 14.2 us;
+// 249 x 2040: 10.0 and, by waves, 10.7). VEC: rows of 16-byte chunks (K % 8 == 0), up to 4 chunks a
+// thread held in registers between the maximum and the codes (one read of x), longer rows read
 // twice; otherwise value by value. Codes are written up to Kp (zeros past K).
 constexpr int kQThreads = 256, kQChunks = 4;
-template <bool VEC>
-__global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int K, int64_t ldx,
-                                                                     uint8_t* __restrict__ y, int64_t ldy, int Kp,
-                                                                     float* __restrict__ scale) {
+template <bool VEC, int TPR>
+__global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int R, int K,
+                                                                     int64_t ldx, uint8_t* __restrict__ y, int64_t ldy,
+                                                                     int Kp, float* __restrict__ scale) {
   __shared__ uint32_t amax[kQThreads / kWave];
-  const int tid = threadIdx.x;
-  const uint16_t* xr = x + blockIdx.x * ldx;
-  uint8_t* yr = y + blockIdx.x * ldy;
+  constexpr int ROWS = kQThreads / TPR;
+  const int tid = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (ROWS > 1 && row >= R) return;
+  const uint16_t* xr = x + row * ldx;
+  uint8_t* yr = y + row * ldy;
   auto reduce = [&](uint32_t bits) {
     bits = wave_max_u(bits);
-    if ((tid & 63) == 0) amax[tid >> 6] = bits;
-    __syncthreads();
-    bits = max(max(amax[0], amax[1]), max(amax[2], amax[3]));
-    if (tid == 0) scale[blockIdx.x] = row_scale(bits);
+    if constexpr (ROWS == 1) {
+      if ((tid & 63) == 0) amax[tid >> 6] = bits;
+      __syncthreads();
+      bits = max(max(amax[0], amax[1]), max(amax[2], amax[3]));
+    }
+    if (tid == 0) scale[row] = row_scale(bits);
     return bits;
   };
   uint32_t bits = 0;
@@ -91,12 +98,12 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
     const uint4* src = reinterpret_cast<const uint4*>(xr);
     uint2* dst = reinterpret_cast<uint2*>(yr);
     const int K8 = K >> 3, Kp8 = Kp >> 3;
-    constexpr int STEP = kQThreads * kQChunks;
+    constexpr int STEP = TPR * kQChunks;
     uint4 v[kQChunks];
     auto load = [&](int i0) {
 #pragma unroll
       for (int c = 0; c < kQChunks; ++c) {
-        const int i = i0 + tid + c * kQThreads;
+        const int i = i0 + tid + c * TPR;
         v[c] = make_uint4(0, 0, 0, 0);
         if (i < K8) v[c] = src[i];
       }
@@ -112,15 +119,15 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
       if (Kp8 > STEP) load(i0);
 #pragma unroll
       for (int c = 0; c < kQChunks; ++c) {
-        const int i = i0 + tid + c * kQThreads;
+        const int i = i0 + tid + c * TPR;
         if (i < Kp8) dst[i] = bits < 0x7f80u ? codes8(v[c], rc) : make_uint2(0, 0);
       }
     }
   } else {
-    for (int i = tid; i < K; i += kQThreads) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
+    for (int i = tid; i < K; i += TPR) bits = max(bits, (uint32_t)xr[i] & 0x7fffu);
     bits = reduce(bits);
     const RowCode rc = row_code(row_max(bits));
-    for (int i = tid; i < Kp; i += kQThreads)
+    for (int i = tid; i < Kp; i += TPR)
       yr[i] = i < K && bits < 0x7f80u ? (uint8_t)code_of(bf16_lo(xr[i]), rc) : (uint8_t)0;
   }
 }
@@ -354,11 +361,19 @@ bool rows_vec(const void* x, int64_t K, int64_t ldx) { return K % 8 == 0 && ldx 
 
 int launch_quantize_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y8, int64_t ldy, int64_t Kp, float* scale,
                        hipStream_t st) {
-  const unsigned rows = (unsigned)R;
-  if (rows_vec(x, K, ldx))
-    quantize_rows_i8_kernel<true><<<rows, kQThreads, 0, st>>>((const uint16_t*)x, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
-  else
-    quantize_rows_i8_kernel<false><<<rows, kQThreads, 0, st>>>((const uint16_t*)x, (int)K, ldx, (uint8_t*)y8, ldy, (int)Kp, scale);
+  const bool vec = rows_vec(x, K, ldx), wave = K <= 2048 && R > num_cus();
+  const unsigned blocks = (unsigned)(wave ? cdiv(R, kQThreads / kWave) : R);
+#define QUANTIZE(VEC_, TPR_)                                                                                     \
+  quantize_rows_i8_kernel<VEC_, TPR_><<<blocks, kQThreads, 0, st>>>((const uint16_t*)x, (int)R, (int)K, ldx, (uint8_t*)y8, ldy, \
+                                                                    (int)Kp, scale)
+  if (vec) {
+    if (wave) QUANTIZE(true, kWave);
+    else QUANTIZE(true, kQThreads);
+  } else {
+    if (wave) QUANTIZE(false, kWave);
+    else QUANTIZE(false, kQThreads);
+  }
+#undef QUANTIZE
   TB_LAUNCH_CHECK("quantize_rows_i8");
   return 0;
 }

@@ -21,13 +21,15 @@ struct CacheGeom {
 
 // ---- write ------------------------------------------------------------------------
 
-// A copy, bound by memory. A block takes TB tokens: a thread one 16-byte chunk of the keys' or values'
-// heads, over the block's tokens (W threads a token, so 256 / W tokens at once).
+// A copy, bound by memory (8192 tokens of 8 heads of 128: 14.3 us, 4.7 TB/s). A block takes TB tokens: a
+// thread one 16-byte chunk of the keys' or values' heads, over the block's tokens (W threads a token,
+// so 256 / W tokens at once).
 // A slot that a later token names too is left to that token, so a repeated slot holds the last one's
-// whole rows whatever the order of the blocks: the block marks its slots in a small table of bits and
-// looks up every later token's slot there, those that hit it in full. Longer lists than kWriteTokens
-// are written by launches in turn, which keeps that search short.
-constexpr int kWriteBlock = 16, kWriteTokens = 16384;
+// whole rows whatever the order of the blocks: the block marks its slots in a table of bits (by their low
+// 16 bits; with 11 the false hits cost more than the copy) and looks up every later token's slot
+// there, those that hit it in full. That search grows with the square of the tokens, so more than
+// kWriteTokens are written by launches in turn (84140 short rows: 72 us; by 16384 at once 90, floor 26).
+constexpr int kWriteBlock = 32, kWriteTokens = 65536, kNamed = 65536;
 __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                           int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
                                                           const int32_t* __restrict__ slots, int T, int TB, int C, int D8,
@@ -35,9 +37,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
                                                           CacheGeom kg, CacheGeom vg, int n_slots, int page) {
   __shared__ int mine[kWriteBlock];  // the block's slots, -1: nowhere
   __shared__ int64_t koff[kWriteBlock], voff[kWriteBlock];
-  __shared__ uint32_t named[64];
+  __shared__ uint32_t named[kNamed / 32];
   const int tid = threadIdx.x, t0 = blockIdx.x * TB, nt = min(TB, T - t0);
-  if (tid < 64) named[tid] = 0;
+  for (int i = tid; i < kNamed / 32; i += 256) named[i] = 0;
   int slot = -1;
   if (tid < nt) {
     slot = slots[t0 + tid];
@@ -48,18 +50,34 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
     voff[tid] = p * vg.sp + r * vg.ss;
   }
   __syncthreads();
-  if (slot >= 0) atomicOr(&named[(slot >> 5) & 63], 1u << (slot & 31));
+  if (slot >= 0) atomicOr(&named[(slot % kNamed) >> 5], 1u << (slot & 31));
   __syncthreads();
   constexpr int U = 4;
-  for (int u0 = t0 + 1 + tid; u0 < T; u0 += 256 * U) {
+  auto look = [&](int s, int u) {  // (threads that find the same loss write the same)
+    if (s >= 0 && (named[(s % kNamed) >> 5] >> (s & 31) & 1))
+      for (int t = 0; t < nt; ++t)
+        if (mine[t] == s && t0 + t < u) mine[t] = -1;
+  };
+  int u0 = t0 + 1 + 4 * tid;
+  for (; u0 - 4 * tid + 256 * 4 * U <= T; u0 += 256 * 4 * U) {
+    int4 s[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) __builtin_memcpy(&s[i], slots + u0 + 1024 * i, 16);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = u0 + 1024 * i;
+      look(s[i].x, u);
+      look(s[i].y, u + 1);
+      look(s[i].z, u + 2);
+      look(s[i].w, u + 3);
+    }
+  }
+  for (int u = u0 - 3 * tid; u < T; u += 256 * U) {
     int s[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) s[i] = u0 + 256 * i < T ? slots[u0 + 256 * i] : -1;
+    for (int i = 0; i < U; ++i) s[i] = u + 256 * i < T ? slots[u + 256 * i] : -1;
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (s[i] >= 0 && (named[(s[i] >> 5) & 63] >> (s[i] & 31) & 1))
-        for (int t = 0; t < nt; ++t)
-          if (mine[t] == s[i] && t0 + t < u0 + 256 * i) mine[t] = -1;  // (every thread that writes it writes this)
+    for (int i = 0; i < U; ++i) look(s[i], u + 256 * i);
   }
   __syncthreads();
   for (int j = tid & (W - 1); j < 2 * C; j += W) {
@@ -751,8 +769,8 @@ extern "C" int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_
   while (W < 256 && W < 2 * C) W *= 2;
   for (int64_t t = 0; t < T; t += kWriteTokens) {
     const int n = (int)std::min<int64_t>(kWriteTokens, T - t);
-    // at least 4 blocks a CU as long as there are tokens
-    const int TB = (int)std::min<int64_t>(kWriteBlock, std::max<int64_t>(256 / W, n / (4 * num_cus())));
+    // 8 blocks a CU as long as there are tokens (16384 of 8 heads: 34.8 us; 4 blocks 38.5, 16 blocks 41.2)
+    const int TB = (int)std::min<int64_t>(kWriteBlock, std::max<int64_t>(256 / W, n / (8 * num_cus())));
     paged_write_kernel<<<(unsigned)cdiv(n, TB), 256, 0, as_stream(stream)>>>(
         (const uint16_t*)k + t * k_st, (const uint16_t*)v + t * v_st, k_st, k_sh, v_st, v_sh, slots + t, n, TB, C, (int)(D / 8),
         W, (uint16_t*)k_cache, (uint16_t*)v_cache, kg, vg, (int)(pages * page), (int)page);

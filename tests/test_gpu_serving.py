@@ -82,6 +82,8 @@ ATTEND = [  # H, Hkv, D, page, lengths
     (80, 2, 128, 16, [1200, 31]),
     (40, 1, 256, 16, [900, 45]),
     (3, 1, 200, 16, [100, 7]),
+    (16, 1, 128, 16, [500, 20]),
+    (32, 2, 128, 16, [1500, 20]),
     (8, 4, 200, 16, [3000, 7, 0, 900]),
 ]
 

@@ -9,7 +9,8 @@ with one rounding to bf16:
 
 Beside scaled_linear, which keeps every bit of bf16: half its weight bytes (decoding) and
 twice its matrix rate (prefill), for the rounding of x and W to 8 bits relative to each row's
-maximum. No counterpart in the reference.
+maximum. The scales are fp32: rows of x with a maximum below 2^-95 lose bits of theirs, weight
+rows above 2^110 overflow. No counterpart in the reference.
 """
 from __future__ import annotations
 

@@ -131,7 +131,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     new token's own is among them once paged_write has put it there). A sequence of length 0
     gives zeros. Entries of page_table outside [0, pages) hold no keys: their positions are
     left out. scale: 1 / sqrt(D) if None. Logits, softmax statistics and sums in fp32, one
-    rounding to bf16."""
+    rounding to bf16 (so values beyond 3.4e38 / n may overflow the sum over n keys)."""
     (pages, Hkv, page, D), k_st, v_st = _cache("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
     shape = q.shape
     if len(shape) != 3 or shape[2] != D:

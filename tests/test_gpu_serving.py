@@ -411,7 +411,8 @@ LINEAR = [(1, 1, 1), (1, 16, 8), (1, 4096, 512), (1, 1000, 1001), (2, 64, 64), (
           (17, 1040, 250), (31, 333, 96), (33, 96, 4096), (64, 4096, 640), (65, 512, 512), (100, 1000, 3001),
           (128, 1024, 128), (129, 640, 264), (200, 2048, 1024), (256, 4096, 256), (257, 130, 1030), (384, 384, 384),
           (513, 2049, 200), (1024, 512, 1024), (1500, 64, 2000), (2048, 200, 24), (4097, 136, 520), (8, 16, 40000),
-          (700, 16, 16), (1, 131072, 40), (40, 40000, 72), (300, 33000, 64)]
+          (700, 16, 16), (6, 4096, 100), (16, 4096, 33), (9, 8, 3000), (13, 4104, 70), (2, 32768, 24), (5, 24, 16),
+          (1, 131072, 40), (40, 40000, 72), (300, 33000, 64)]
 
 
 @pytest.mark.parametrize("M,K,N", LINEAR)
@@ -439,7 +440,7 @@ def test_linear_largest_sums(dev, M):
     assert torch.equal(y.cpu(), want.to(BF))
 
 
-@pytest.mark.parametrize("M", [1, 30, 500])
+@pytest.mark.parametrize("M", [1, 3, 14, 30, 500])
 def test_linear_special_rows(dev, M):
     x = torch.randn(M, 200, generator=gen(2)).to(BF).to(dev)
     w = torch.randn(90, 200, generator=gen(3)).to(BF).to(dev)
@@ -467,7 +468,7 @@ def test_linear_special_rows(dev, M):
 
 
 @pytest.mark.parametrize("scale", [1e30, 1e-25])
-@pytest.mark.parametrize("M", [1, 20, 300])
+@pytest.mark.parametrize("M", [1, 4, 12, 20, 300])
 def test_linear_extreme_scales(dev, scale, M):
     x = (torch.randn(M, 256, generator=gen(5)) * scale).to(BF).to(dev)
     w = (torch.randn(64, 256, generator=gen(6)) / 16).to(BF).to(dev)
@@ -510,7 +511,7 @@ def test_linear_rows_alone(dev):
     x = torch.randn(600, 520, generator=gen(8)).to(BF).to(dev)
     w8, ws = tbf16.prepare_weight_i8(torch.randn(136, 520, generator=gen(9)).to(BF).to(dev))
     y = tbf16.int8_linear(x, w8, ws)
-    for n in (1, 2, 3, 16, 17, 64, 100, 128, 300):
+    for n in (1, 2, 3, 4, 5, 8, 9, 16, 17, 64, 100, 128, 300):
         assert torch.equal(y[:n], tbf16.int8_linear(x[:n], w8, ws)), n
 
 

@@ -140,15 +140,16 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
 // weights straight from memory into registers, PF turns of a wave in flight; the int32 sums of
 // the waves meet in LDS. A lane's fragment is 16 bytes of weight row l % 16, and the same k of
 // token l % 16.
-// FUSED (1: of a single token, 2): every block quantises the tokens into LDS for itself, while its
-// first weights are on their way: one launch, no workspace (1 x 4096 x 4096: 6.4 us, 8.8 with a pass
-// of its own; 4 x 4096 x 4096: 8.1 and 9.0; 1 x 32768 x 2048: 21 and 31), up to kFusedCodes values,
-// of one or two tokens four times that; above them the blocks' repeated work costs more than the pass
-// (16 x 4096 x 4096: 15.6 and 10.0; 8 x 4096 x 4096: 10.3 and 9.6).
-// Otherwise the codes come from a pass of their own (padded with zeros to a multiple of 128, so
-// that what lies behind a weight row does not matter).
-// 1 x 2560 x 10240: 8.4 us, 3.1 TB/s of weights; 16 tokens: 7.7 us after a pass of 3.4.
-constexpr int kDecodeRows = 16, kFusedCodes = 16384;
+// FUSED: every block quantises the tokens into LDS for itself, while its first weights are on their
+// way: one launch, no workspace. 1: a single token (1 x 4096 x 4096: 6.4 us, 8.8 with a pass of its own;
+// 1 x 32768 x 2048: 21 and 31). 3: 5 to 16 tokens of up to kFusedK values, two a wave, held in registers
+// (8 x 4096 x 4096: 8.0 and 9.6; 16 x 2560 x 10240: 11.6 and 11.2, but 11 and 14 with the host's second
+// launch). 2: the others of up to kFusedCodes values, of two tokens four times that, read twice (4 x 4096
+// x 4096: 8.1 and 9.0); above them the blocks' repeated work costs more than the pass (8 x 8192).
+// 0: the codes come from a pass of their own (padded with zeros to a multiple of 128, so that what
+// lies behind a weight row does not matter).
+// 1 x 2560 x 10240: 8.4 us, 3.1 TB/s of weights.
+constexpr int kDecodeRows = 16, kFusedCodes = 16384, kFusedK = 4096;
 template <int T, int FUSED>
 __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restrict__ x, int64_t ldx,
                                                         const uint8_t* __restrict__ x8, const float* __restrict__ sx,
@@ -179,7 +180,39 @@ __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restri
   for (int u = 0; u < PF; ++u)
     if (wave + u * WAVES < turns) load(w[u], wave + u * WAVES);
 
-  if constexpr (FUSED != 0) {
+  if constexpr (FUSED == 3) {
+    // a wave takes tokens `wave` and `wave` + 8, all their chunks in registers
+    const int K8 = K >> 3, Kp8 = Kp >> 3;
+    constexpr int NC = kFusedK / 512;
+    uint4 v[2][NC];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int m = wave + 8 * r;
+      const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        v[r][c] = make_uint4(0, 0, 0, 0);
+        if (m < M && 64 * c + lane < K8) v[r][c] = src[64 * c + lane];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int m = wave + 8 * r;
+      if (m >= M) break;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) bits = max(bits, mag8(v[r][c]));
+      bits = wave_max_u(bits);
+      const RowCode rc = row_code(row_max(bits));
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (64 * c + lane < Kp8)
+          *reinterpret_cast<uint2*>(xl + m * (Kp + 16) + 8 * (64 * c + lane)) =
+              bits < 0x7f80u ? codes8(v[r][c], rc) : make_uint2(0, 0);
+      if (lane == 0) scale[m] = row_scale(bits);
+    }
+    __syncthreads();
+  } else if constexpr (FUSED != 0) {
     const int K8 = K >> 3, Kp8 = Kp >> 3;
     // `per` waves on a row, 8 / per rows at once
     const int lg = FUSED == 1 ? 3 : M == 2 ? 2 : M <= 4 ? 1 : 0, per = 1 << lg;
@@ -312,7 +345,7 @@ Plan plan_of(int64_t M, int64_t K, int64_t N, bool vec) {
     p.R = (int)std::min<int64_t>(64, std::max<int64_t>(8, cdiv(cdiv(N, cus), 8) * 8));
     p.T = (int)cdiv(p.R, 16);
     p.form = Plan::kDecode;
-    if (vec && M * Kp <= (M <= 2 ? 4 : 1) * kFusedCodes) {
+    if (vec && (M * Kp <= (M <= 2 ? 4 : 1) * kFusedCodes || Kp <= kFusedK)) {
       p.form = Plan::kFused;
       return p;
     }
@@ -443,8 +476,10 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
       DECODE_T(0)
     } else if (M == 1) {
       DECODE_T(1)
-    } else {
+    } else if (M <= 4 || Kp > kFusedK) {
       DECODE_T(2)
+    } else {
+      DECODE_T(3)
     }
 #undef DECODE_T
 #undef DECODE

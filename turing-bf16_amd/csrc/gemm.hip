@@ -8,8 +8,8 @@
 //
 // Kernels, all for 64-wide waves and 160 KB LDS; the dispatch (pick_f16, pick_fused) says
 // where each runs, and its configuration number pins it:
-//  - pingpong_kernel, fp16 a: large tiles, two wave groups alternating MFMAs and loads.
-//  - ksplit_kernel, fp16 a: small tiles (decode to mid-size M), the groups on alternate k
+//  - pingpong_kernel (gemm_tiles.h), fp16 a: large tiles, two wave groups alternating MFMAs and loads.
+//  - ksplit_kernel (gemm_tiles.h), fp16 a: small tiles (decode to mid-size M), the groups on alternate k
 //    tiles; also the implicit convolutions.
 //  - gemm_kernel: the form that converts bf16 a in its staging (a short K, or few columns
 //    for many rows; tbf16_linear_exps; the no-allocation entry point where x16 does not

@@ -41,9 +41,16 @@ def _device(x, *others) -> int:
     return dev
 
 
-def _rows(x):
-    """x with its columns side by side and rows apart (a single row's stride does not matter)."""
-    return x if (x.stride(1) == 1 or x.shape[1] == 1) and (x.stride(0) >= x.shape[1] or x.shape[0] == 1) else x.contiguous()
+def _rows(x, K):
+    """(x, its row stride) with columns side by side and rows apart (a single row's stride does
+    not matter): x itself or a copy."""
+    ld, step = x.stride()
+    if (step == 1 or K == 1) and ld >= K:
+        return x, ld
+    if (step == 1 or K == 1) and x.shape[0] == 1:
+        return x, K
+    x = x.contiguous()
+    return x, max(x.stride(0), K)
 
 
 def quantize_rows_i8(x: torch.Tensor):
@@ -59,11 +66,11 @@ def quantize_rows_i8(x: torch.Tensor):
     R, K = x.shape
     if K > MAX_K:
         raise ValueError(f"tbf16.quantize_rows_i8: K = {K} is above {MAX_K}, int32 sums could overflow")
-    x = _rows(x)
+    x, ld = _rows(x, K)
     y = torch.empty((R, _up(K, 16)), device=x.device, dtype=torch.int8)
     scale = torch.empty((R,), device=x.device, dtype=torch.float32)
     if R:
-        launch("tbf16_quantize_rows_i8", x, ptr(x), R, K, max(x.stride(0), K), ptr(y), y.stride(0), ptr(scale))
+        launch("tbf16_quantize_rows_i8", x, ptr(x), R, K, ld, ptr(y), y.stride(0), ptr(scale))
     return (y if y.shape[1] == K else y[:, :K]), scale
 
 
@@ -74,14 +81,16 @@ def prepare_weight_i8(w: torch.Tensor):
 
 
 def _weight_rows(w8, K):
-    """w8 with rows the kernels read in place: 16-byte aligned, apart by a multiple of 16 and
-    readable up to K rounded up to 128 or to the next row (what prepare_weight_i8 returns);
-    else a padded copy."""
-    N, ld = w8.shape[0], w8.stride(0)
-    if (w8.stride(1) == 1 or K == 1) and ld % 16 == 0 and K <= ld < 1 << 23 and w8.data_ptr() % 16 == 0:
-        if ld == K or w8.untyped_storage().nbytes() >= w8.storage_offset() + (N - 1) * ld + min(ld, _up(K, 128)):
-            return w8
-    return F.pad(w8, (0, -K % 16)) if K % 16 else w8.clone(memory_format=torch.contiguous_format)
+    """(w8, its row stride) with rows the kernels read in place: 16-byte aligned, apart by a
+    multiple of 16 and readable up to K rounded up to 128 or to the next row (what
+    prepare_weight_i8 returns); else a padded copy."""
+    ld, step = w8.stride()
+    if (step == 1 or K == 1) and not ld & 15 and K <= ld < 1 << 23 and not w8.data_ptr() & 15:
+        if ld == K or (w8.untyped_storage().nbytes()
+                       >= w8.storage_offset() + (w8.shape[0] - 1) * ld + min(ld, _up(K, 128))):
+            return w8, ld
+    w8 = F.pad(w8, (0, -K % 16)) if K % 16 else w8.clone(memory_format=torch.contiguous_format)
+    return w8, _up(K, 16)
 
 
 # tbf16_linear_i8's workspace bytes per (device, M, K, N): its choice of kernel counts the
@@ -127,13 +136,13 @@ def int8_linear(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias=N
     Np = _up(N, 8)
     y = x.new_empty((M, Np))
     if M and N:
-        x2 = _rows(x2)
-        w8 = _weight_rows(w8, K)
+        x2, ldx = _rows(x2, K)
+        w8, ldw = _weight_rows(w8, K)
         ws = w_scale if w_scale.dtype == torch.float32 and w_scale.is_contiguous() else w_scale.float().contiguous()
         wsb = _ws_bytes(dev, M, K, N)
         work = x.new_empty(wsb, dtype=torch.uint8) if wsb else None
-        launch("tbf16_linear_i8", x2, x2.data_ptr(), M, K, max(x2.stride(0), K), w8.data_ptr(), N, max(w8.stride(0), K + -K % 16),
-               ws.data_ptr(), ptr(b), y.data_ptr(), Np, ptr(work), wsb)
+        launch("tbf16_linear_i8", x2, x2.data_ptr(), M, K, ldx, w8.data_ptr(), N, ldw, ws.data_ptr(), ptr(b), y.data_ptr(),
+               Np, ptr(work), wsb)
     if Np != N:
         y = y[:, :N]
     return y if len(shape) == 2 else y.reshape(*shape[:-1], N)

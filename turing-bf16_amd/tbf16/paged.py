@@ -26,26 +26,25 @@ from ._ext import launch, lib
 MAX_HEAD_DIM = 256
 
 
-def _cache(fn, k_cache, v_cache, *others):
-    """(shape, k_cache's strides, v_cache's) of a cache the kernels take, on the device of
-    `others` too; raises for any other."""
+def _cache(fn, k_cache, v_cache):
+    """(shape, k_cache's strides and address, v_cache's) of a cache the kernels take; raises for
+    any other."""
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"tbf16.{fn}: expected k_cache and v_cache of one shape (pages, Hkv, page, D), got "
                          f"{tuple(shape)} and {tuple(v_cache.shape)}")
     _, Hkv, page, D = shape
-    if D % 8 or not 0 < D <= MAX_HEAD_DIM:
+    if D & 7 or not 0 < D <= MAX_HEAD_DIM:
         raise ValueError(f"tbf16.{fn}: head dim {D} is not a multiple of 8 up to {MAX_HEAD_DIM}")
     if Hkv == 0 or page == 0:
         raise ValueError(f"tbf16.{fn}: cache of shape {tuple(shape)} holds nothing")
-    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+    if k_cache.dtype is not torch.bfloat16 or v_cache.dtype is not torch.bfloat16:
         raise TypeError(f"tbf16.{fn}: expected a bf16 cache")
-    k_st, v_st = k_cache.stride(), v_cache.stride()
+    k_st, v_st, kc, vc = k_cache.stride(), v_cache.stride(), k_cache.data_ptr(), v_cache.data_ptr()
     if (k_st[3] != 1 or v_st[3] != 1 or (k_st[0] | k_st[1] | k_st[2] | v_st[0] | v_st[1] | v_st[2]) & 7
-            or (k_cache.data_ptr() | v_cache.data_ptr()) & 15):
+            or (kc | vc) & 15):
         raise ValueError(f"tbf16.{fn}: cache rows must be contiguous and 16-byte aligned (strides multiples of 8)")
-    _same_device(fn, k_cache, v_cache, *others)
-    return shape, k_st, v_st
+    return shape, k_st, kc, v_st, vc
 
 
 def _same_device(fn, first, *others):
@@ -58,7 +57,7 @@ def _same_device(fn, first, *others):
 
 
 def _index(fn, name, t, dim):
-    if t.dtype != torch.int32 or t.dim() != dim:
+    if t.dtype is not torch.int32 or t.dim() != dim:
         raise TypeError(f"tbf16.{fn}: expected {name} as an int32 tensor of {dim} dimension(s)")
     return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
 
@@ -78,12 +77,13 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
     token t. k, v bf16 (T, Hkv, D), any strides; slots int32 (T,). Slots outside the cache
     (negative: a padded batch) leave it as it is; where slots repeat, the last token's rows
     stay. In place; k and v must not lie in the cache's own storage."""
-    (pages, Hkv, page, D), kc_st, vc_st = _cache("paged_write", k_cache, v_cache, k, v, slots)
+    (pages, Hkv, page, D), kc_st, kc, vc_st, vc = _cache("paged_write", k_cache, v_cache)
+    _same_device("paged_write", k_cache, v_cache, k, v, slots)
     shape = k.shape
     T = shape[0] if len(shape) else 0
     if v.shape != shape or shape != (T, Hkv, D):
         raise ValueError(f"tbf16.paged_write: k {tuple(shape)} and v {tuple(v.shape)} are not (T, {Hkv}, {D})")
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
         raise TypeError("tbf16.paged_write: expected bf16 k and v")
     slots = _index("paged_write", "slots", slots, 1)
     if slots.shape[0] != T:
@@ -94,7 +94,6 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
         for c in (k_cache, v_cache):
             if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
                 raise ValueError("tbf16.paged_write: the cache is an expanded view")
-    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
     if kc == vc and pages:
         raise ValueError("tbf16.paged_write: k_cache and v_cache are the same memory")
     held = k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr()
@@ -132,13 +131,13 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     gives zeros. Entries of page_table outside [0, pages) hold no keys: their positions are
     left out. scale: 1 / sqrt(D) if None. Logits, softmax statistics and sums in fp32, one
     rounding to bf16 (so values beyond 3.4e38 / n may overflow the sum over n keys)."""
-    (pages, Hkv, page, D), k_st, v_st = _cache("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
-    shape = q.shape
-    if len(shape) != 3 or shape[2] != D:
-        raise ValueError(f"tbf16.paged_sdpa: q {tuple(shape)} is not (B, H, {D})")
-    if q.dtype != torch.bfloat16:
+    (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa", k_cache, v_cache)
+    _same_device("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"tbf16.paged_sdpa: q {tuple(q.shape)} is not (B, H, {D})")
+    if q.dtype is not torch.bfloat16:
         raise TypeError("tbf16.paged_sdpa: expected bf16 q")
-    B, H, _ = shape
+    B, H, _ = q.shape
     if H == 0 or H % Hkv:
         raise ValueError(f"tbf16.paged_sdpa: {H} query heads over {Hkv} key/value heads")
     page_table = _index("paged_sdpa", "page_table", page_table, 2)
@@ -152,7 +151,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
         return o
     wsb = _ws_bytes(q.get_device(), B, H, Hkv, D, n * page)
     ws = q.new_empty(wsb, dtype=torch.uint8) if wsb else o  # (o: nothing is written there)
-    launch("tbf16_paged_attn", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], k_cache.data_ptr(), v_cache.data_ptr(),
-           pages, page, k_st[0], k_st[1], k_st[2], v_st[0], v_st[1], v_st[2], page_table.data_ptr(), page_table.stride(0), n,
-           lengths.data_ptr(), D ** -0.5 if scale is None else float(scale), o.data_ptr(), ws.data_ptr(), wsb)
+    launch("tbf16_paged_attn", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], kc, vc, pages, page, k_st[0], k_st[1],
+           k_st[2], v_st[0], v_st[1], v_st[2], page_table.data_ptr(), page_table.stride(0), n, lengths.data_ptr(),
+           D ** -0.5 if scale is None else float(scale), o.data_ptr(), ws.data_ptr(), wsb)
     return o

@@ -431,9 +431,8 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
       const int64_t off = ok ? (int64_t)p.id * a.vg.sp + (int64_t)p.row * a.vg.ss : 0;
       const int e = PAD && CH * r16 >= a.D ? 0 : CH * r16;  // (what lies past D goes to outputs past D)
       const uint16_t* base = a.vc + p.head * a.vg.sh + e;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t* row = reinterpret_cast<const uint32_t*>(base + shfl_off(off, 16 * (j >> 2) + 4 * g + (j & 3)));
+      auto load = [&](int j, const uint16_t* at) {
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(at);
 #pragma unroll
         for (int w = 0; w < VW; w += CH >= 8 ? 4 : 2) {
           if constexpr (CH >= 8) {
@@ -444,6 +443,17 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
             vr[j][w] = v.x; vr[j][w + 1] = v.y;
           }
         }
+      };
+      if ((a.page & 3) == 0) {  // a lane's 4 keys of a half tile lie side by side in one page
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint16_t* at = base + shfl_off(off, 16 * h + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) load(4 * h + j, at + j * a.vg.ss);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load(j, base + shfl_off(off, 16 * (j >> 2) + 4 * g + (j & 3)));
       }
     };
     auto alive = [&](const Page& p) { return (uint32_t)__ballot((uint32_t)p.id < a.pages); };  // lanes l and l + 32 alike

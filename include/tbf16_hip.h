@@ -301,12 +301,13 @@ int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int6
  * k_j) v_j over positions j < lengths[b], position j in page table[b, j / page], row j % page,
  * head h / (H / Hkv). fp32 logits, running maximum, sum and output, one rounding to bf16.
  * Positions past max_pages * page and positions whose page lies outside [0, pages) are left
- * out; a sequence with none gives zeros. B * H * positions / 32 below 2e9. q bf16 (B, H, D), element strides (b, h); caches as tbf16_paged_write's
- * (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row stride
- * table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. ws:
- * tbf16_paged_attn_ws_bytes(B, H, Hkv, D, max_pages * page) bytes (asked with the stream's
- * device current; 0 for few short sequences, ws may then be NULL), 16-byte aligned, this call's alone until
- * it has run. Serves the calls the reference leaves to torch (tbf16/convert.py:29-30). */
+ * out; a sequence with none gives zeros. q bf16 (B, H, D), element strides (b, h); caches as
+ * tbf16_paged_write's (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row
+ * stride table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. B * H * max_pages * page
+ * / 32 below 2e9. ws: tbf16_paged_attn_ws_bytes(B, H, Hkv, D, max_pages * page) bytes (asked with
+ * the stream's device current; 0 for few short sequences, ws may then be NULL), 16-byte aligned,
+ * this call's alone until it has run. Serves the calls the reference leaves to torch
+ * (tbf16/convert.py:29-30). */
 size_t tbf16_paged_attn_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t positions);
 int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
                      const void* k_cache, const void* v_cache, int64_t pages, int64_t page, int64_t kc_sp, int64_t kc_sh,

@@ -272,6 +272,9 @@ def test_attend_empty(dev):
     q = torch.ones(2, 4, 64, dtype=BF, device=dev)
     assert (tbf16.paged_sdpa(q, k, k, i32(2, 0), i32(2) + 5) == 0).all()
     assert (tbf16.paged_sdpa(q, k[:0], k[:0], i32(2, 3), i32(2) + 5) == 0).all()
+    many = torch.ones(300, 4, 64, dtype=BF, device=dev)
+    for n, pages in ((0, 3), (3, 0), (900, 0), (3, 3)):
+        assert (tbf16.paged_sdpa(many, k[:pages], k[:pages], i32(300, n), i32(300) + (5 if n * pages == 0 else 0)) == 0).all()
 
 
 def test_attend_same_bits_again(dev):

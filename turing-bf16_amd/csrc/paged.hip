@@ -803,7 +803,7 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
                                 const int32_t* table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
                                 float scale, void* o, void* ws, int64_t ws_bytes, void* stream) {
   const CacheGeom kg{kc_sp, kc_sh, kc_ss}, vg{vc_sp, vc_sh, vc_ss};
-  TB_CHECK(B >= 0 && H > 0, "paged_attn: bad shape");
+  TB_CHECK(B >= 0 && H > 0 && H < (int64_t)1 << 24, "paged_attn: bad shape");
   if (int rc = check_cache("paged_attn", k_cache, v_cache, pages, Hkv, page, D, kg, vg)) return rc;
   TB_CHECK(H % Hkv == 0, "paged_attn: query heads must be a multiple of key/value heads");
   TB_CHECK(D <= 256, "paged_attn: head dim must be at most 256");

@@ -15,7 +15,7 @@ as (pages, page, Hkv, D) is passed as its transpose(1, 2).
 Both run on the current stream without waiting for the GPU and can be captured into a graph:
 what changes from step to step (slots, page_table, lengths) is read on the device. Inference
 only: no gradients. Keys and values stay bf16 and are multiplied as such (bf16 MFMA), so no
-power-of-two scales are needed and any bf16 magnitude is taken.
+power-of-two scales are needed.
 """
 from __future__ import annotations
 
@@ -130,7 +130,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     new token's own is among them once paged_write has put it there). A sequence of length 0
     gives zeros. Entries of page_table outside [0, pages) hold no keys: their positions are
     left out. scale: 1 / sqrt(D) if None. Logits, softmax statistics and sums in fp32, one
-    rounding to bf16 (so values beyond 3.4e38 / n may overflow the sum over n keys)."""
+    rounding to bf16 (values beyond 1e36 / n may overflow the sum over n keys)."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa", k_cache, v_cache)
     _same_device("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
     if q.dim() != 3 or q.shape[2] != D:

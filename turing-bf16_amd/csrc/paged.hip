@@ -137,6 +137,13 @@ constexpr int kTile = 32;
 // Running maxima start at kNone; a unit that had any key ends at kFew or above.
 constexpr float kNone = -FLT_MAX, kFew = -3.0e38f;
 
+// n / d for 0 <= n < 2^31 as (n magic) >> shift: with d <= 2^l, magic = ceil(2^(31 + l) / d) is off by
+// less than 2^-31 of itself.
+struct Div {
+  uint32_t magic, shift;
+};
+__device__ __forceinline__ uint32_t operator/(uint32_t n, Div d) { return (uint32_t)((uint64_t)n * d.magic >> d.shift); }
+
 struct AttnArgs {
   const uint16_t *q, *kc, *vc;
   int64_t q_sb, q_sh;
@@ -144,7 +151,8 @@ struct AttnArgs {
   const int32_t *table, *lengths;
   int64_t t_sb;
   int cap;  // positions a table row covers
-  uint32_t pages, page, magic, shift;  // j / page = (j magic) >> shift for j < 2^31
+  uint32_t pages, page;
+  Div by_page, by_units, by_blocks, by_waves;  // units of a sequence; blocks and waves of the list form
   float scale_log2;
   int B, H, Hkv, G, D, R, RG;  // R rows a unit, RG units a key/value head
   uint16_t* o;
@@ -180,76 +188,69 @@ struct Run {
   int n;
   Cursor at;
 };
+// Inclusive prefix sums over the wave: in rows of 16 lanes, then the rows' last lanes (DPP row_shr 1, 2,
+// 4, 8, row_bcast 15 and 31; a scan by ds_bpermute took 0.3 us longer).
+__device__ __forceinline__ uint32_t prefix_sum(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+  return v;
+}
 __device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t block, uint32_t wave, uint32_t blocks, uint32_t wpb,
-                                      int units, int lane) {
-  constexpr int PF = 4;  // groups of 64 sequences whose lengths are loaded at once
-  int len[PF];
-  uint32_t up[PF];  // tiles of the group's sequences up to the lane's own
-#pragma unroll
-  for (int k = 0; k < PF; ++k) len[k] = lane + k * kWave < a.B ? seq_len(a, lane + k * kWave) : 0;
+                                      int lane) {
+  auto length = [&](int b) { return b < a.B ? seq_len(a, b) : 0; };
   auto tiles = [&](int l) { return (uint32_t)((l + kTile - 1) / kTile); };
-  auto prefix = [&](uint32_t v) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const uint32_t u = __shfl_up((int)v, o, kWave);
-      if (lane >= o) v += u;
-    }
-    return v;
-  };
-  auto last = [&](uint32_t v) { return (uint32_t)uniform(__builtin_amdgcn_readlane((int)v, kWave - 1)); };
-  uint32_t all = 0;
-#pragma unroll
-  for (int k = 0; k < PF; ++k) {
-    up[k] = 0;
-    if (k * kWave < a.B) {
-      up[k] = prefix(tiles(len[k]));
-      all += last(up[k]);
-    }
-  }
-  if (a.B > PF * kWave) {
+  auto last = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1); };
+  // 64 sequences at a time: a lane's own length and tiles, and those up to its own
+  int len = length(lane);
+  uint32_t up = prefix_sum(tiles(len)), all = last(up);
+  if (a.B > kWave) {
+    constexpr int U = 4;
     uint32_t more = 0;
-    for (int b = lane + PF * kWave; b < a.B; b += kWave) more += tiles(seq_len(a, b));
-    all += last(prefix(more));
+    for (int b = lane + kWave; b < a.B + lane; b += U * kWave) {
+      int l[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) l[i] = length(b + i * kWave);
+#pragma unroll
+      for (int i = 0; i < U; ++i) more += tiles(l[i]);
+    }
+    all += last(prefix_sum(more));
   }
+  const uint32_t units = a.Hkv * a.RG;
   all *= units;
-  Run r{1, 1, 0, {0, 0, 0, 0, 0, 0}};
-  r.act = min(wpb, max(1u, (all + blocks - 1) / blocks));
-  r.c = max(1u, (all + blocks * r.act - 1) / (blocks * r.act));
+  // act = ceil(all / blocks) up to wpb, c = ceil(all / (blocks act))
+  Run r{1, wpb, 0, {0, 0, 0, 0, 0, 0}};
+  if (all <= blocks * wpb) r.act = max(1u, (all + blocks - 1) / a.by_blocks);
+  else r.c = (all + blocks * wpb - 1) / a.by_waves;
   const uint64_t first = ((uint64_t)block * r.act + wave) * r.c;
   if (wave >= r.act || first >= all) return r;
   r.n = min(r.c, all - (uint32_t)first);
   // the sequence: the first one that ends behind tile `first`
-  uint32_t t = (uint32_t)first / units, rest = (uint32_t)first % units;  // in tiles of one unit
-  for (int k = 0;; ++k) {
-    int l = 0;
-    uint32_t u = 0;
-#pragma unroll
-    for (int i = 0; i < PF; ++i)
-      if (k == i) {
-        l = len[i];
-        u = up[i];
-      }
-    if (k >= PF) {
-      const int b = k * kWave + lane;
-      l = b < a.B ? seq_len(a, b) : 0;
-      u = prefix(tiles(l));
-    }
-    const uint64_t past = __ballot(u > t);
-    if (past == 0) {
-      t -= last(u);
-      continue;
-    }
-    const int w = __builtin_ctzll(past);
-    r.at.b = k * kWave + w;
-    r.at.len = __builtin_amdgcn_readlane(l, w);
-    r.at.nt = (r.at.len + kTile - 1) / kTile;
-    t = (t - (__builtin_amdgcn_readlane((int)u, w) - r.at.nt)) * units + rest;  // in the sequence's own tiles
-    break;
+  uint32_t t = (uint32_t)first / a.by_units;  // in tiles of one unit
+  const uint32_t rest = (uint32_t)first - t * units;
+  int b0 = 0;
+  uint64_t past;
+  while ((past = __ballot(up > t)) == 0) {
+    t -= last(up);
+    b0 += kWave;
+    len = length(b0 + lane);
+    up = prefix_sum(tiles(len));
   }
+  const int w = __builtin_ctzll(past);
+  r.at.b = b0 + w;
+  r.at.len = __builtin_amdgcn_readlane(len, w);
+  r.at.nt = (r.at.len + kTile - 1) / kTile;
+  t = (t - (__builtin_amdgcn_readlane((int)up, w) - r.at.nt)) * units + rest;  // in the sequence's own tiles
   const uint32_t unit = t / (uint32_t)r.at.nt;
   r.at.tile = t - unit * r.at.nt;
-  r.at.head = unit / (uint32_t)a.RG;
-  r.at.grp = unit - r.at.head * a.RG;
+  r.at.head = unit;
+  if (a.RG > 1) {
+    r.at.head = unit / (uint32_t)a.RG;
+    r.at.grp = unit - r.at.head * a.RG;
+  }
   return r;
 }
 
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     cur.tile = min(wave * per, cur.nt);
     n = min(per, cur.nt - cur.tile);
   } else {
-    const Run r = run_of(a, blockIdx.x, wave, gridDim.x, WPB, a.Hkv * a.RG, lane);
+    const Run r = run_of(a, blockIdx.x, wave, gridDim.x, WPB, lane);
     c = r.c;
     act = r.act;
     n = r.n;
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     // the page and row of the lane's key (l % 32) of a tile
     auto page_of = [&](const Cursor& c) {
       const uint32_t pos = c.tile * kTile + (lane & 31);
-      const uint32_t idx = (uint32_t)((uint64_t)pos * a.magic >> a.shift);
+      const uint32_t idx = pos / a.by_page;
       Page p{-1, (int)(pos - idx * a.page), c.head};
       if (pos < (uint32_t)c.len) p.id = a.table[c.b * a.t_sb + idx];
       return p;
@@ -737,6 +738,12 @@ AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   return p;
 }
 
+Div div_by(int64_t d) {  // 1 <= d < 2^31
+  int l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return Div{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), (uint32_t)(31 + l)};
+}
+
 template <int DP, int RT, int WPB>
 void launch_attn(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
   const dim3 grid = unit ? dim3((unsigned)a.B, (unsigned)a.Hkv, (unsigned)a.RG) : dim3((unsigned)blocks);
@@ -835,11 +842,10 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   a.cap = pages == 0 ? 0 : (int)std::min<int64_t>(max_pages * page, ((int64_t)1 << 31) - 64);
   a.pages = (uint32_t)pages;
   a.page = (uint32_t)page;
-  // page <= 2^l: magic = ceil(2^(31 + l) / page) is off by less than 2^l / page of 2^-31
-  int l = 0;
-  while (((int64_t)1 << l) < page) ++l;
-  a.magic = (uint32_t)((((uint64_t)1 << (31 + l)) + page - 1) / page);
-  a.shift = 31 + l;
+  a.by_page = div_by(page);
+  a.by_units = div_by(Hkv * p.RG);
+  a.by_blocks = div_by(std::max<int64_t>(p.blocks, 1));
+  a.by_waves = div_by(std::max<int64_t>(p.blocks * p.wpb, 1));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.B = (int)B;
   a.H = (int)H;

@@ -68,11 +68,11 @@ __device__ __forceinline__ float row_scale(uint32_t bits) {
 // TPR threads per row: a block of 4 waves (the row's latency is what a call of few rows waits for: 256 x
 // 4096 6.2 us with a wave per row, 4.2 us so; 4096 x 4096, bound by memory: 12.4 and 11.1 us, 4.5 TB/s),
 // or a wave where there are many rows of up to 2048 values (7363 x 448 with its product: 19.0 -> 14.2 us;
-// 249 x 2040: 10.0 and, by waves, 10.7). VEC: rows of 16-byte chunks (K % 8 == 0), up to 4 chunks a
+// 249 x 2040: 10.0 and, by waves, 10.7). VEC: rows of 16-byte chunks (K % 8 == 0), up to NC a
 // thread held in registers between the maximum and the codes (one read of x), longer rows read
 // twice; otherwise value by value. Codes are written up to Kp (zeros past K).
-constexpr int kQThreads = 256, kQChunks = 4;
-template <bool VEC, int TPR>
+constexpr int kQThreads = 256;
+template <bool VEC, int TPR, int NC>
 __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint16_t* __restrict__ x, int R, int K,
                                                                      int64_t ldx, uint8_t* __restrict__ y, int64_t ldy,
                                                                      int Kp, float* __restrict__ scale) {
@@ -98,11 +98,11 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
     const uint4* src = reinterpret_cast<const uint4*>(xr);
     uint2* dst = reinterpret_cast<uint2*>(yr);
     const int K8 = K >> 3, Kp8 = Kp >> 3;
-    constexpr int STEP = TPR * kQChunks;
-    uint4 v[kQChunks];
+    constexpr int STEP = TPR * NC;
+    uint4 v[NC];
     auto load = [&](int i0) {
 #pragma unroll
-      for (int c = 0; c < kQChunks; ++c) {
+      for (int c = 0; c < NC; ++c) {
         const int i = i0 + tid + c * TPR;
         v[c] = make_uint4(0, 0, 0, 0);
         if (i < K8) v[c] = src[i];
@@ -111,14 +111,14 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
     for (int i = 0; i < K8; i += STEP) {
       load(i);
 #pragma unroll
-      for (int c = 0; c < kQChunks; ++c) bits = max(bits, mag8(v[c]));
+      for (int c = 0; c < NC; ++c) bits = max(bits, mag8(v[c]));
     }
     bits = reduce(bits);
     const RowCode rc = row_code(row_max(bits));
     for (int i0 = 0; i0 < Kp8; i0 += STEP) {
       if (Kp8 > STEP) load(i0);
 #pragma unroll
-      for (int c = 0; c < kQChunks; ++c) {
+      for (int c = 0; c < NC; ++c) {
         const int i = i0 + tid + c * TPR;
         if (i < Kp8) dst[i] = bits < 0x7f80u ? codes8(v[c], rc) : make_uint2(0, 0);
       }
@@ -396,15 +396,16 @@ int launch_quantize_i8(const void* x, int64_t R, int64_t K, int64_t ldx, void* y
                        hipStream_t st) {
   const bool vec = rows_vec(x, K, ldx), wave = K <= 2048 && R > num_cus();
   const unsigned blocks = (unsigned)(wave ? cdiv(R, kQThreads / kWave) : R);
-#define QUANTIZE(VEC_, TPR_)                                                                                     \
-  quantize_rows_i8_kernel<VEC_, TPR_><<<blocks, kQThreads, 0, st>>>((const uint16_t*)x, (int)R, (int)K, ldx, (uint8_t*)y8, ldy, \
+#define QUANTIZE(VEC_, TPR_, NC_)                                                                                \
+  quantize_rows_i8_kernel<VEC_, TPR_, NC_><<<blocks, kQThreads, 0, st>>>((const uint16_t*)x, (int)R, (int)K, ldx, (uint8_t*)y8, ldy, \
                                                                     (int)Kp, scale)
   if (vec) {
-    if (wave) QUANTIZE(true, kWave);
-    else QUANTIZE(true, kQThreads);
+    if (wave) QUANTIZE(true, kWave, 4);
+    else if (K <= 4096) QUANTIZE(true, kQThreads, 2);
+    else QUANTIZE(true, kQThreads, 4);
   } else {
-    if (wave) QUANTIZE(false, kWave);
-    else QUANTIZE(false, kQThreads);
+    if (wave) QUANTIZE(false, kWave, 1);
+    else QUANTIZE(false, kQThreads, 1);
   }
 #undef QUANTIZE
   TB_LAUNCH_CHECK("quantize_rows_i8");

@@ -518,6 +518,18 @@ def test_linear_rows_alone(dev):
         assert torch.equal(y[:n], tbf16.int8_linear(x[:n], w8, ws)), n
 
 
+@pytest.mark.parametrize("M,K,N", [(4096, 640, 4096), (4300, 1041, 4099), (4096, 128, 4096), (2048, 4096, 2056), (1100, 2000, 8200),
+                                   (9000, 136, 1500), (520, 4096, 16384), (2000, 260, 1000), (6000, 16, 3000), (3000, 4224, 700)])
+def test_linear_large_tiles(dev, M, K, N):
+    """Every tile's outputs are those of a few rows at a time, bit for bit."""
+    x = torch.randn(M, K, generator=gen(M)).to(BF).to(dev)
+    w8, ws = tbf16.prepare_weight_i8(torch.randn(N, K, generator=gen(N)).to(BF).to(dev))
+    b = torch.randn(N, generator=gen(K)).to(BF).to(dev)
+    y = tbf16.int8_linear(x, w8, ws, b)
+    for m in range(0, M, 60):
+        assert torch.equal(y[m:m + 60], tbf16.int8_linear(x[m:m + 60], w8, ws, b)), m
+
+
 def test_linear_far_offsets(dev):
     """Outputs and weights past 2^31 elements and bytes."""
     g = gen(10)

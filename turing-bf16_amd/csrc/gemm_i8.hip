@@ -314,8 +314,10 @@ __global__ __launch_bounds__(256) void splitk_i8_kernel(const intx4* __restrict_
 // 128 integers; splitting K over s blocks a tile adds the partial sums' round trip and a launch.
 // The figures are those of the fp16 kernels by 128 bytes of k: the MFMAs take as long, and so do
 // LDS and L2, which bound both. On 30 shapes (M 16 to 8192) the tile they pick is the best one's time
-// but for 1% on average, 7% at most. 4096^3: 52 us, 2640 TOPS, MFMAs busy 0.56 at 2.2 GHz (LDS traffic:
-// a 64-deep step of a wave's 128 x 64 tile reads 192 rows for 32 MFMAs).
+// but for 1% on average, 7% at most. 4096^3: 52 us, 2640 TOPS, MFMAs busy 0.56 at 2.2 GHz. The direct
+// loads' way into LDS beside the MFMAs costs the most of the rest: timed at 4096 x 16384 x 4096, 234 us a
+// call, 175 with the loop's loads left out, 230 with all of them from one place (so not HBM), 227 with
+// half of x's LDS reads. The weight from memory to registers, only x through LDS, is slower (336 us).
 struct Tile {
   int bm, bn;
   bool ksplit;

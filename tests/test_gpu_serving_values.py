@@ -1,0 +1,57 @@
+"""paged_sdpa where single weights and values decide the output: weights whose difference is what
+is left of them. Every form of the kernel: head dims of 64, 128 and 256 and below, one to four
+blocks of 16 query heads, a block per unit and equal runs of the list of tiles."""
+import pytest
+import torch
+
+import tbf16
+
+from _serving64 import paged_sdpa64
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+# H, Hkv, D: (DP, RT) of (64, 1), (64, 2), (64, 4), (128, 1), (128, 2), (256, 1); rows of D padded and not
+FORMS = [(8, 2, 64), (6, 1, 40), (24, 1, 64), (64, 1, 64), (50, 1, 56), (16, 4, 128), (8, 1, 80), (32, 1, 128), (40, 2, 96),
+         (16, 1, 256), (4, 2, 160)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def cache_of(dev, k, v, wide):
+    """k, v (B, n, Hkv, D) as a cache of pages of 16 in order; a table of a page more than needed, or
+    (wide) of so many that the list form runs."""
+    B, n, Hkv, D = k.shape
+    need = -(-n // 16)
+
+    def pages(t):
+        full = torch.full((B, need * 16, Hkv, D), float("nan"), dtype=BF)
+        full[:, :n] = t
+        return full.view(B * need, 16, Hkv, D).transpose(1, 2).contiguous().to(dev)
+
+    table = torch.full((B, 200 if wide else need + 1), -1, dtype=torch.int32)
+    table[:, :need] = torch.arange(B * need, dtype=torch.int32).view(B, need)
+    return pages(k), pages(v), table.to(dev), torch.full((B,), n, dtype=torch.int32, device=dev)
+
+
+@pytest.mark.parametrize("H,Hkv,D", FORMS)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_weights_that_cancel(dev, H, Hkv, D, wide):
+    """Two keys of almost the same weight and opposite values: the output is the difference of the
+    weights, 2^-10 to 2^-13 of either, so it shows what the weights lose on their way to it."""
+    B = 6
+    q = torch.randn(B, H, D, generator=gen(H)).to(BF)
+    k = torch.zeros(B, 2, Hkv, D)
+    k[:, 1] = torch.randn(B, Hkv, D, generator=gen(D)) * 2.0 ** -10
+    r = torch.randn(B, Hkv, D, generator=gen(1)).to(BF)
+    args = (q.to(dev), *cache_of(dev, k.to(BF), torch.stack((r, -r), 1), wide))
+    o = tbf16.paged_sdpa(*args).cpu().double()
+    ref, _ = paged_sdpa64(*args)
+    # before the rounding to bf16 an output is off by at most 2^-20 of r: exp2 1 ulp (2^-23) of a weight of
+    # at most 1, the logit behind it below 2^-24, and 8 fp32 roundings of sums of at most r
+    bound = 2.0 ** -8 * ref.abs() + 2.0 ** -20 * r.abs().repeat_interleave(H // Hkv, 1).double()
+    err = (o - ref).abs()
+    assert (err <= bound).all(), ((err - bound).max(), err.max())
+    assert ref.abs().median() < 2.0 ** -10  # (the difference is what is tested)

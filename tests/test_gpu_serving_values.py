@@ -55,3 +55,17 @@ def test_attend_weights_that_cancel(dev, H, Hkv, D, wide):
     err = (o - ref).abs()
     assert (err <= bound).all(), ((err - bound).max(), err.max())
     assert ref.abs().median() < 2.0 ** -10  # (the difference is what is tested)
+
+
+@pytest.mark.parametrize("D", [136, 152, 168, 184, 216, 232, 248])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_rows_of_half_a_chunk(dev, D, wide):
+    """Head dims past 128 whose last chunk of 16 is half there, up to the cache's last row."""
+    B, n, Hkv = 3, 48, 2
+    k, v = (torch.randn(B, n, Hkv, D, generator=gen(D + i)).to(BF) for i in range(2))
+    q = torch.randn(B, 6, D, generator=gen(D + 2)).to(BF)
+    args = (q.to(dev), *cache_of(dev, k, v, wide))
+    o = tbf16.paged_sdpa(*args).cpu().double()
+    ref, bound = paged_sdpa64(*args)
+    err = (o - ref).abs()
+    assert (err <= bound).all(), (err - bound).max()

@@ -10,6 +10,7 @@
 
 #include "abi_util.h"
 #include "common.h"
+#include "paged_rows.h"
 
 using namespace tbf16;
 
@@ -423,26 +424,24 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
         const uint16_t* row = base + shfl_off(off, 16 * h + r16);
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-          const int e = 8 * (g + 4 * i);
-          kr[h][i] = ldg16(row + (PAD && e >= a.D ? 0 : e));
+          kr[h][i] = ldg16(row + (PAD ? key_piece(a.D, g, i) : 8 * (g + 4 * i)));
         }
       }
     };
     auto load_v = [&](const Page& p) {
       const bool ok = (uint32_t)p.id < a.pages;
       const int64_t off = ok ? (int64_t)p.id * a.vg.sp + (int64_t)p.row * a.vg.ss : 0;
-      const int e = PAD && CH * r16 >= a.D ? 0 : CH * r16;  // (what lies past D goes to outputs past D)
-      const uint16_t* base = a.vc + p.head * a.vg.sh + e;
+      auto piece = [&](int i) { return PAD ? value_piece(a.D, DP, r16, i) : CH * r16 + 8 * i; };
+      const uint16_t* base = a.vc + p.head * a.vg.sh + piece(0);
       auto load = [&](int j, const uint16_t* at) {
-        const uint32_t* row = reinterpret_cast<const uint32_t*>(at);
+        if constexpr (CH == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(at);
+          vr[j][0] = v.x; vr[j][1] = v.y;
+        } else {
 #pragma unroll
-        for (int w = 0; w < VW; w += CH >= 8 ? 4 : 2) {
-          if constexpr (CH >= 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(row + w);
-            vr[j][w] = v.x; vr[j][w + 1] = v.y; vr[j][w + 2] = v.z; vr[j][w + 3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(row + w);
-            vr[j][w] = v.x; vr[j][w + 1] = v.y;
+          for (int i = 0; i < value_pieces(DP); ++i) {
+            const uint4 v = ldg16(at + (piece(i) - piece(0)));
+            vr[j][4 * i] = v.x; vr[j][4 * i + 1] = v.y; vr[j][4 * i + 2] = v.z; vr[j][4 * i + 3] = v.w;
           }
         }
       };

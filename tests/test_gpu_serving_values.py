@@ -69,3 +69,56 @@ def test_attend_rows_of_half_a_chunk(dev, D, wide):
     ref, bound = paged_sdpa64(*args)
     err = (o - ref).abs()
     assert (err <= bound).all(), (err - bound).max()
+
+
+@pytest.mark.parametrize("H,Hkv,D", FORMS)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("n", [1, 2, 40, 200])
+def test_attend_infinite_values(dev, H, Hkv, D, wide, n):
+    """An infinite value makes its element infinite whatever the weight's bits (a weight of 1 for the
+    largest key, or for the only one), infinities of both signs and NaN make it NaN, and every other
+    element keeps its bits."""
+    B = 4
+    q = torch.randn(B, H, D, generator=gen(H)).to(BF)
+    k, v = (torch.randn(B, n, Hkv, D, generator=gen(D + i)).to(BF) for i in range(2))
+    k[1] = 0  # every weight 1
+    clean = tbf16.paged_sdpa(q.to(dev), *cache_of(dev, k, v, wide)).cpu()
+    bad = v.clone()
+    rows = [0, n // 2, n - 1]
+    for i, j in enumerate(rows):
+        bad[:, j, :, i] = float("inf")
+        bad[:, j, :, 3 + i] = -float("inf")
+        bad[:, j, :, D - 1 - i] = float("nan")
+    bad[:, 0, :, 6], bad[:, n - 1, :, 6] = float("inf"), -float("inf")
+    args = (q.to(dev), *cache_of(dev, k, bad, wide))
+    o = tbf16.paged_sdpa(*args).cpu()
+    ref, _ = paged_sdpa64(*args)
+    for c in range(D):
+        r = ref[..., c]
+        if torch.isfinite(r).all():
+            assert torch.equal(o[..., c], clean[..., c]), c
+        else:
+            assert not torch.isfinite(r).any()
+            assert torch.equal(o[..., c].nan_to_num(7.0, 1.0, -1.0).double(), r.nan_to_num(7.0, 1.0, -1.0)), c
+    assert (ref[..., :3] == float("inf")).all() and (ref[..., 3:6] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("first", [False, True])
+def test_attend_infinite_value_of_a_small_weight(dev, wide, first):
+    """Weights down to 2^-90 of the largest, before and behind the largest key."""
+    n, D = 300, 128
+    q = torch.zeros(1, 4, D)
+    q[..., 0] = 1
+    k = torch.zeros(1, n, 1, D)
+    far = torch.arange(1, 91.0)  # key i's weight is 2^-i of the largest
+    at = torch.arange(200, 290) if first else torch.arange(5, 95)
+    k[0, :, 0, 0] = -120 * D ** 0.5
+    k[0, 2 if first else 298, 0, 0] = 0
+    k[0, at, 0, 0] = -far * D ** 0.5
+    v = torch.randn(1, n, 1, D, generator=gen(3)).to(BF)
+    v[0, at, 0, torch.arange(90)] = float("inf")
+    k = k.to(BF)
+    args = (q.to(BF).to(dev), *cache_of(dev, k, v, wide))
+    o = tbf16.paged_sdpa(*args, scale=D ** -0.5 * 0.6931).cpu()
+    assert (o[..., :90] == float("inf")).all() and torch.isfinite(o[..., 90:]).all()

@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
 // are units and the second launch is left out.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32;
 // Running maxima start at kNone; a unit that had any key ends at kFew or above.
@@ -540,6 +541,11 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
             p0 -= bf16_hi(__float_as_uint(p0));
             p1 -= bf16_hi(__float_as_uint(p1));
           }
+          // 2^-32 of p in place of a part that is zero: an infinite value times it stays infinite
+          const ushort2v least = __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, f[0][j]), ushort2v{32 << 7, 32 << 7});
+#pragma unroll
+          for (int t = 1; t < 3; ++t)
+            f[t][j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, f[t][j]), least));
         }
 #pragma unroll
         for (int t = 0; t < 3; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));

@@ -301,7 +301,7 @@ int tbf16_paged_write(const void* k, const void* v, int64_t T, int64_t Hkv, int6
  * k_j) v_j over positions j < lengths[b], position j in page table[b, j / page], row j % page,
  * head h / (H / Hkv). fp32 logits, running maximum, sum and output, one rounding to bf16.
  * Positions past max_pages * page and positions whose page lies outside [0, pages) are left
- * out; a sequence with none gives zeros. Infinite values of weights above 2^-94 of the row's
+ * out; a sequence with none gives zeros. Infinite values of weights above 2^-90 of the row's
  * largest give infinities (below, or with both signs, NaN). q bf16 (B, H, D), element strides (b, h); caches as
  * tbf16_paged_write's (strides below 2^31); D % 8 == 0, D <= 256; table int32 (B, max_pages), row
  * stride table_stride; lengths int32 (B,); o bf16 (B, H, D) contiguous. B * H * max_pages * page

@@ -122,3 +122,20 @@ def test_attend_infinite_value_of_a_small_weight(dev, wide, first):
     args = (q.to(BF).to(dev), *cache_of(dev, k, v, wide))
     o = tbf16.paged_sdpa(*args, scale=D ** -0.5 * 0.6931).cpu()
     assert (o[..., :90] == float("inf")).all() and torch.isfinite(o[..., 90:]).all()
+
+
+@pytest.mark.parametrize("H,Hkv,D", FORMS)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_values_near_the_largest(dev, H, Hkv, D, wide):
+    """Weights that grow along the keys, over values whose weighted mean bf16 holds."""
+    n = 190
+    q = torch.zeros(2, H, D)
+    q[..., 0] = 1
+    k = torch.zeros(2, n, Hkv, D)
+    k[..., 0] = (torch.arange(n) / 4).view(n, 1)  # a weight 2^(1/4) of the one before it, 2^8 a tile
+    v = (torch.rand(2, n, Hkv, D, generator=gen(D)) + 1) * 2.0 ** 125  # the weights' sum is at most 7 of the largest's
+    args = (q.to(BF).to(dev), *cache_of(dev, k.to(BF), v.to(BF), wide))
+    scale = 0.6931
+    o = tbf16.paged_sdpa(*args, scale=scale).cpu().double()
+    ref, bound = paged_sdpa64(*args, scale=scale)
+    assert torch.isfinite(ref).all() and ((o - ref).abs() <= bound).all()

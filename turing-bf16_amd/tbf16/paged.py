@@ -130,9 +130,10 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     new token's own is among them once paged_write has put it there). A sequence of length 0
     gives zeros. Entries of page_table outside [0, pages) hold no keys: their positions are
     left out. scale: 1 / sqrt(D) if None. Logits, softmax statistics and sums in fp32, one
-    rounding to bf16 (values beyond 1e36 / n may overflow the sum over n keys). An infinite value
-    makes its element infinite; where its key's weight is below 2^-94 of the row's largest the
-    weight may count as zero, and the element is NaN."""
+    rounding to bf16 (weights relative to the row's largest, the sum of weighted values may reach
+    8e40, 256 times bf16's largest value). An infinite value makes its element infinite; where its
+    key's weight is below 2^-90 of the row's largest the weight may count as zero, and the element
+    is NaN."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa", k_cache, v_cache)
     _same_device("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
     if q.dim() != 3 or q.shape[2] != D:

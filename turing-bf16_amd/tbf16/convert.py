@@ -74,7 +74,8 @@ class Linear(nn.Module):
 class Int8Linear(nn.Module):
     """Inference stand-in for a bf16 nn.Linear in 8-bit integers (tbf16.int8_linear). Buffers
     `weight8` (int8, N x K) and `weight_scale` (fp32, N) carry the weight, rounded to 8 bits
-    relative to each row's maximum; `bias` is the original parameter."""
+    relative to each row's maximum; `bias` is the original parameter. A cast of the model
+    (.to(dtype), .half(), ...) leaves both buffers as they are: rounded scales would change every output."""
 
     def __init__(self, lin: nn.Linear):
         super().__init__()
@@ -84,6 +85,15 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight8", w8)
         self.register_buffer("weight_scale", ws)
         self.bias = lin.bias
+
+    def _apply(self, fn, recurse=True):
+        held = self.weight8, self.weight_scale
+        super()._apply(fn, recurse)
+        for name, old in zip(("weight8", "weight_scale"), held):
+            new = getattr(self, name)
+            if new.dtype != old.dtype:  # its device alone
+                setattr(self, name, old.to(new.device))
+        return self
 
     @property
     def weight(self) -> torch.Tensor:

@@ -124,6 +124,8 @@ def int8_linear(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias=N
         raise ValueError(f"tbf16.int8_linear: x has K={K}, weight has K={Kw}")
     if K > MAX_K:
         raise ValueError(f"tbf16.int8_linear: K = {K} is above {MAX_K}, int32 sums could overflow")
+    if w_scale.dtype != torch.float32 and w_scale.dtype != torch.float64:
+        raise TypeError(f"tbf16.int8_linear: expected fp32 scales, got {w_scale.dtype}")
     if w_scale.numel() != N:
         raise ValueError(f"tbf16.int8_linear: {w_scale.numel()} scales for {N} channels")
     dev = _device(x, w8, w_scale)

@@ -4,6 +4,7 @@ import torch
 import torch.nn as nn
 
 import tbf16
+from tbf16 import int8
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +23,4 @@ def test_casts_and_moves_keep_the_bits(dev, M, K, N):
             change()
             m[0].bias.data = m[0].bias.data.to(BF)  # (bf16's values in every cast)
             assert torch.equal(m(x), y)
+            assert int8._weight_rows(m[0].weight8, K)[0] is m[0].weight8  # read in place

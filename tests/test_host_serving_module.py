@@ -2,6 +2,7 @@
 quantised here by the 64-bit oracle)."""
 import copy
 import importlib
+import io
 
 import pytest
 import torch
@@ -36,6 +37,9 @@ def unchanged(m, w8, ws):
     assert m.weight8.dtype == torch.int8 and torch.equal(m.weight8, w8)
     assert m.weight_scale.dtype == torch.float32 and torch.equal(m.weight_scale, ws)
     assert m.weight8.shape == (m.out_features, m.in_features)
+    # and its rows are read in place, without a copy a call
+    rows, ld = int8._weight_rows(m.weight8, m.in_features)
+    assert rows is m.weight8 and ld % 16 == 0
     assert set(m.state_dict()) == {"weight8", "weight_scale", "bias"}
 
 
@@ -64,6 +68,20 @@ def test_moves_and_copies_keep_the_weight(module):
     unchanged(back, w8, ws)
 
 
+@pytest.mark.parametrize("assign", [False, True])
+@pytest.mark.parametrize("dense", [False, True])
+def test_loading_keeps_the_rows(module, assign, dense):
+    m, w8, ws = module
+    f = io.BytesIO()
+    torch.save({k: v.contiguous() if dense else v for k, v in m.state_dict().items()}, f)
+    f.seek(0)
+    other = copy.deepcopy(m)
+    other.weight8.zero_()
+    other.weight_scale.zero_()
+    other.load_state_dict(torch.load(f, weights_only=True), assign=assign)
+    unchanged(other, w8, ws)
+
+
 def test_rounded_scales_are_refused(module, monkeypatch):
     monkeypatch.setattr(int8, "_device", lambda *a: 0)
     m, w8, ws = module
@@ -71,3 +89,13 @@ def test_rounded_scales_are_refused(module, monkeypatch):
     for t in (BF, torch.float16, torch.int32):
         with pytest.raises(TypeError, match="fp32 scales"):
             tbf16.int8_linear(x, w8, ws.to(t))
+
+
+def test_padded_rows():
+    """Rows that the kernels read in place are left alone; others are copied, values unchanged."""
+    w = torch.randint(-127, 128, (6, 200), dtype=torch.int8)
+    for bad in (w, w[:, :199], w.t().contiguous().t(), torch.zeros(6 * 208 + 1, dtype=torch.int8)[1:].view(6, 208)):
+        p = int8.padded_rows(bad)
+        assert p is not bad and torch.equal(p, bad) and int8.padded_rows(p) is p
+    for good in (w[:, :192].contiguous(), torch.zeros(5, 16, dtype=torch.int8), w[:, :0], torch.zeros(0, 16, dtype=torch.int8)):
+        assert int8.padded_rows(good) is good

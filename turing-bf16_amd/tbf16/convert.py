@@ -30,7 +30,7 @@ import torch.nn.functional as F
 from . import autograd, routing
 from .attention import sdpa as _scaled_sdpa
 from .conv import convert_conv, convertible
-from .int8 import MAX_K, int8_linear, prepare_weight_i8
+from .int8 import MAX_K, int8_linear, padded_rows, prepare_weight_i8
 from .ops import prepare_weight, scaled_linear
 
 # Training: layers with in or out features below this run in fp32 (tbf16/convert.py:26-27).
@@ -93,7 +93,12 @@ class Int8Linear(nn.Module):
             new = getattr(self, name)
             if new.dtype != old.dtype:  # its device alone
                 setattr(self, name, old.to(new.device))
+        self.weight8 = padded_rows(self.weight8)  # (a move drops the padding)
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self.weight8 = padded_rows(self.weight8)  # (assign=True: the loaded tensor's own rows)
 
     @property
     def weight(self) -> torch.Tensor:

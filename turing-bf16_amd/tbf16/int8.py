@@ -93,6 +93,14 @@ def _weight_rows(w8, K):
     return w8, _up(K, 16)
 
 
+def padded_rows(w8: torch.Tensor) -> torch.Tensor:
+    """An int8 weight (N, K) whose rows int8_linear reads in place: w8 itself, or a copy with padded
+    rows (a weight that was moved, or loaded from elsewhere, has lost what prepare_weight_i8 gave it)."""
+    K = w8.shape[1]
+    rows = w8 if K == 0 else _weight_rows(w8, K)[0]
+    return w8 if rows is w8 else rows[:, :K]
+
+
 # tbf16_linear_i8's workspace bytes per (device, M, K, N): its choice of kernel counts the
 # device's CUs, so it is asked on the tensors' device, once
 _WS_BYTES: dict = {}

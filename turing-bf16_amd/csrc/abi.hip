@@ -1,6 +1,8 @@
 // Library identity and thread-local error reporting for the C ABI.
 #include <string.h>
 
+#include <atomic>
+
 #include "abi_util.h"
 
 namespace tbf16 {
@@ -15,15 +17,15 @@ void set_error(const char* fmt, ...) {
 }
 
 int64_t num_cus() {
-  static int64_t cache[64] = {};
+  static std::atomic<int> cache[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cache[dev] == 0) {
-    int n = 0;
+  int n = cache[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev] = n;
+    cache[dev].store(n, std::memory_order_relaxed);
   }
-  return cache[dev];
+  return n;
 }
 
 }  // namespace tbf16

@@ -36,7 +36,6 @@
 #include <stdlib.h>
 
 #include <algorithm>
-#include <atomic>
 #include <float.h>
 #include <math.h>
 
@@ -816,19 +815,6 @@ WsLayout fwd_ws(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64
   w.off_vt16 = w.off_k16 + bkv;
   w.total = w.off_vt16 + bkv;
   return w;
-}
-
-// Compute units of the current device.
-int64_t num_cus() {
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  int n = cache[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 template <int DP, int NW>

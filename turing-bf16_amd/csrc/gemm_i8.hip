@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
 // way: one launch, no workspace. 1: a single token (1 x 4096 x 4096: 6.4 us, 8.8 with a pass of its own;
 // 1 x 32768 x 2048: 21 and 31). 3: 5 to 16 tokens of up to kFusedK values, two a wave, held in registers
 // (8 x 4096 x 4096: 8.0 and 9.6; 16 x 2560 x 10240: 11.6 and 11.2, but 11 and 14 with the host's second
-// launch). 2: the others of up to kFusedCodes values, of two tokens four times that, read twice (4 x 4096
+// launch). 2: 2 to 4 tokens of up to kFusedCodes values, two of four times that, read twice (4 x 4096
 // x 4096: 8.1 and 9.0); above them the blocks' repeated work costs more than the pass (8 x 8192).
 // 0: the codes come from a pass of their own (padded with zeros to a multiple of 128, so that what
 // lies behind a weight row does not matter).
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restri
   } else if constexpr (FUSED != 0) {
     const int K8 = K >> 3, Kp8 = Kp >> 3;
     // `per` waves on a row, 8 / per rows at once
-    const int lg = FUSED == 1 ? 3 : M == 2 ? 2 : M <= 4 ? 1 : 0, per = 1 << lg;
+    const int lg = FUSED == 1 ? 3 : M == 2 ? 2 : 1, per = 1 << lg;
     const int first = wave >> lg, part = wave & (per - 1), step = per * 64, i0 = part * 64 + lane;
     for (int m = first; m < (FUSED == 1 ? 1 : M); m += WAVES >> lg) {
       const uint4* src = reinterpret_cast<const uint4*>(x + m * ldx);
@@ -325,10 +325,9 @@ struct Tile {
 };
 constexpr Tile kTiles[] = {{256, 256, false, 7.6f, 0.97f, 1.40f}, {192, 256, false, 7.4f, 0.82f, 1.04f},
                            {128, 256, false, 5.8f, 0.75f, 0.87f}, {256, 128, false, 5.8f, 0.66f, 0.87f},
-                           {128, 128, false, 4.1f, 0.51f, 0.56f}, {256, 128, true, 6.6f, 0.62f, 0.83f},
-                           {192, 128, true, 5.6f, 0.46f, 0.635f}, {128, 128, true, 3.9f, 0.44f, 0.52f},
-                           {128, 64, true, 2.7f, 0.36f, 0.37f},   {64, 128, true, 2.7f, 0.36f, 0.37f},
-                           {64, 64, true, 2.0f, 0.25f, 0.26f}};
+                           {256, 128, true, 6.6f, 0.62f, 0.83f},   {192, 128, true, 5.6f, 0.46f, 0.635f},
+                           {128, 128, true, 3.9f, 0.44f, 0.52f},   {128, 64, true, 2.7f, 0.36f, 0.37f},
+                           {64, 128, true, 2.7f, 0.36f, 0.37f},    {64, 64, true, 2.0f, 0.25f, 0.26f}};
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 constexpr size_t kSplitBytes = (size_t)16 << 20;
 
@@ -479,7 +478,7 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
       DECODE_T(0)
     } else if (M == 1) {
       DECODE_T(1)
-    } else if (M <= 4 || Kp > kFusedK) {
+    } else if (M <= 4) {
       DECODE_T(2)
     } else {
       DECODE_T(3)
@@ -509,12 +508,11 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
     case 1: PINGPONG(3, 2, 2); break;
     case 2: PINGPONG(2, 2, 3); break;
     case 3: PINGPONG(4, 1, 3); break;
-    case 4: PINGPONG(2, 1, 3); break;
-    case 5: KSPLIT(8, 4, 3); break;
-    case 6: KSPLIT(6, 4, 3); break;
-    case 7: KSPLIT(4, 4, 4); break;
-    case 8: KSPLIT(4, 2, 6); break;
-    case 9: KSPLIT(2, 4, 6); break;
+    case 4: KSPLIT(8, 4, 3); break;
+    case 5: KSPLIT(6, 4, 3); break;
+    case 6: KSPLIT(4, 4, 4); break;
+    case 7: KSPLIT(4, 2, 6); break;
+    case 8: KSPLIT(2, 4, 6); break;
     default: KSPLIT(2, 2, 6); break;
   }
 #undef PINGPONG

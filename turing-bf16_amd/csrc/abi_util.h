@@ -7,6 +7,7 @@
 #include <stdio.h>
 
 #include "../../include/tbf16_hip.h"
+#include "sizes.h"
 
 namespace tbf16 {
 
@@ -18,8 +19,6 @@ int64_t num_cus();
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Attention dropout parameters: thr16 = round(p * 65536), at least 1 for p > 0 and
 // 0 for no dropout; scale = 1 / (1 - p); the seed's two halves are the mixing words.

@@ -7,9 +7,11 @@
 
 #include "abi_util.h"
 #include "common.h"
+#include "gemm_i8_plan.h"
 #include "gemm_tiles.h"
 
 using namespace tbf16;
+using namespace tbf16::i8;
 
 namespace {
 
@@ -149,7 +151,6 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_i8_kernel(const uint1
 // 0: the codes come from a pass of their own (padded with zeros to a multiple of 128, so that what
 // lies behind a weight row does not matter).
 // 1 x 2560 x 10240: 8.4 us, 3.1 TB/s of weights.
-constexpr int kDecodeRows = 16, kFusedCodes = 16384, kFusedK = 4096;
 template <int T, int FUSED>
 __global__ __launch_bounds__(512) void decode_i8_kernel(const uint16_t* __restrict__ x, int64_t ldx,
                                                         const uint8_t* __restrict__ x8, const float* __restrict__ sx,
@@ -309,73 +310,6 @@ __global__ __launch_bounds__(256) void splitk_i8_kernel(const intx4* __restrict_
                                              pack_bf16(f[6], f[7])));
 }
 
-// The tile kernels (gemm_tiles.h), and the estimate of their times: a round of at most CU-count
-// blocks takes c1 + k tiles x slope us, the slope from `light` (few blocks) to `full`, a k tile being
-// 128 integers; splitting K over s blocks a tile adds the partial sums' round trip and a launch.
-// The figures are those of the fp16 kernels by 128 bytes of k: the MFMAs take as long, and so do
-// LDS and L2, which bound both. On 30 shapes (M 16 to 8192) the tile they pick is the best one's time
-// but for 1% on average, 7% at most. 4096^3: 52 us, 2640 TOPS, MFMAs busy 0.56 at 2.2 GHz. The direct
-// loads' way into LDS beside the MFMAs costs the most of the rest: timed at 4096 x 16384 x 4096, 234 us a
-// call, 175 with the loop's loads left out, 230 with all of them from one place (so not HBM), 227 with
-// half of x's LDS reads. The weight from memory to registers, only x through LDS, is slower (336 us).
-struct Tile {
-  int bm, bn;
-  bool ksplit;
-  float c1, light, full;
-};
-constexpr Tile kTiles[] = {{256, 256, false, 7.6f, 0.97f, 1.40f}, {192, 256, false, 7.4f, 0.82f, 1.04f},
-                           {128, 256, false, 5.8f, 0.75f, 0.87f}, {256, 128, false, 5.8f, 0.66f, 0.87f},
-                           {256, 128, true, 6.6f, 0.62f, 0.83f},   {192, 128, true, 5.6f, 0.46f, 0.635f},
-                           {128, 128, true, 3.9f, 0.44f, 0.52f},   {128, 64, true, 2.7f, 0.36f, 0.37f},
-                           {64, 128, true, 2.7f, 0.36f, 0.37f},    {64, 64, true, 2.0f, 0.25f, 0.26f}};
-constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
-constexpr size_t kSplitBytes = (size_t)16 << 20;
-
-// How a call runs.
-struct Plan {
-  enum Form { kFused, kDecode, kTiled } form;
-  int T, R;           // decode kernel: R weight rows a block in T tiles of 16
-  int tile, splits;   // tile kernels
-  size_t scale, x8, part, bytes;  // workspace
-};
-
-Plan plan_of(int64_t M, int64_t K, int64_t N, bool vec) {
-  Plan p{Plan::kTiled, 1, 1, 0, 1, 0, 0, 0, 0};
-  const int64_t Kp = (int64_t)align_up((size_t)K, 128), Np = (int64_t)align_up((size_t)N, 8), cus = num_cus();
-  if (M <= kDecodeRows) {
-    p.R = (int)std::min<int64_t>(64, std::max<int64_t>(8, cdiv(cdiv(N, cus), 8) * 8));
-    p.T = (int)cdiv(p.R, 16);
-    p.form = Plan::kDecode;
-    if (vec && (M * Kp <= (M <= 2 ? 4 : 1) * kFusedCodes || Kp <= kFusedK)) {
-      p.form = Plan::kFused;
-      return p;
-    }
-  }
-  p.x8 = align_up((size_t)M * 4, 256);
-  p.bytes = p.part = align_up(p.x8 + (size_t)M * Kp, 256);
-  if (p.form == Plan::kDecode) return p;
-  const int64_t KT = std::max<int64_t>(1, Kp / 128);
-  float best = INFINITY;
-  for (int i = 0; i < kNumTiles; ++i) {
-    const Tile& t = kTiles[i];
-    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
-    if (tiles >= (int64_t)1 << 31) continue;
-    for (int s = 1; s <= 8; s *= 2) {
-      const int64_t kt = cdiv(KT, s);
-      if (s > 1 && (kt < 8 || (s - 1) * kt >= KT || (size_t)s * M * Np * 4 > kSplitBytes)) break;
-      const float load = std::min(1.f, (float)(tiles * s) / (float)cus);
-      float us = (float)cdiv(tiles * s, cus) * (t.c1 + (float)kt * (t.light + (t.full - t.light) * load));
-      if (s > 1) us += 4.5f + (float)s * (float)M * (float)Np * 8.f / 2e6f;
-      if (us < best) {
-        best = us;
-        p.tile = i;
-        p.splits = s;
-      }
-    }
-  }
-  if (p.splits > 1) p.bytes = p.part + (size_t)p.splits * M * Np * 4;
-  return p;
-}
 // The last plans of this thread by shape (the search costs as much host time as a launch).
 const Plan& plan(int64_t M, int64_t K, int64_t N, bool vec) {
   struct Entry {
@@ -387,7 +321,7 @@ const Plan& plan(int64_t M, int64_t K, int64_t N, bool vec) {
   static thread_local Entry cache[kEntries] = {};  // M = 0: empty
   Entry& e = cache[(uint64_t)(M * 31 + N * 7 + K) % kEntries];
   const int64_t cus = num_cus();
-  if (e.M != M || e.K != K || e.N != N || e.cus != cus || e.vec != vec) e = Entry{M, K, N, cus, vec, plan_of(M, K, N, vec)};
+  if (e.M != M || e.K != K || e.N != N || e.cus != cus || e.vec != vec) e = Entry{M, K, N, cus, vec, plan_of(M, K, N, vec, cus)};
   return e.plan;
 }
 
@@ -460,9 +394,9 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
   const int64_t Kp = (int64_t)align_up((size_t)K, 128);
   const uint16_t* bi = (const uint16_t*)bias;
   uint16_t* yo = (uint16_t*)y;
-  if (p.form != Plan::kFused)
+  if (!p.fused)
     if (int rc = launch_quantize_i8(x, M, K, ldx, x8, Kp, Kp, sx, st)) return rc;
-  if (p.form != Plan::kTiled) {
+  if (p.decode) {
     const unsigned blocks = (unsigned)cdiv(N, p.R);
 #define DECODE(T_, FUSED_)                                                                                   \
   decode_i8_kernel<T_, FUSED_><<<blocks, 512, FUSED_ ? (size_t)(M * (Kp + 16)) : 0, st>>>(                   \
@@ -474,14 +408,11 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
     case 3: DECODE(3, FUSED_); break;   \
     default: DECODE(4, FUSED_); break;  \
   }
-    if (p.form == Plan::kDecode) {
-      DECODE_T(0)
-    } else if (M == 1) {
-      DECODE_T(1)
-    } else if (M <= 4) {
-      DECODE_T(2)
-    } else {
-      DECODE_T(3)
+    switch (p.fused) {
+      case 0: DECODE_T(0) break;
+      case 1: DECODE_T(1) break;
+      case 2: DECODE_T(2) break;
+      default: DECODE_T(3) break;
     }
 #undef DECODE_T
 #undef DECODE
@@ -492,17 +423,14 @@ extern "C" int tbf16_linear_i8(const void* x, int64_t M, int64_t K, int64_t ldx,
   const auto a = (const uint16_t*)x8, b = (const uint16_t*)w8;
   const Tile& t = kTiles[p.tile];
   float* part = p.splits > 1 ? reinterpret_cast<float*>(wsp + p.part) : nullptr;
-  int rows = t.bn;  // weight rows per block: fewer where a single row of tiles would leave CUs idle
-  if (t.ksplit && M <= t.bm && p.splits == 1 && cdiv(N, t.bn) < num_cus())
-    rows = (int)std::min<int64_t>(t.bn, std::max<int64_t>(8, cdiv(cdiv(N, num_cus()), 8) * 8));
   const int kt_per = (int)cdiv(Kp / 128, p.splits);
-  const dim3 grid((unsigned)(cdiv(M, t.bm) * cdiv(Np, rows)), (unsigned)p.splits);
+  const dim3 grid((unsigned)(cdiv(M, t.bm) * cdiv(Np, p.rows)), (unsigned)p.splits);
 #define PINGPONG(HA_, FB_, S_)                                                                                   \
   pingpong_kernel<I8Op, HA_, FB_, S_, true><<<grid, 512, 0, st>>>(a, Kp / 2, sx, b, ldw / 2, ws, bi, yo, ldy, (int)M, (int)Np, \
                                                                   (int)(Kp / 2), part, kt_per, (int)N)
 #define KSPLIT(RM_, RN_, S_)                                                                                             \
   ksplit_kernel<I8Op, RM_, RN_, S_, true><<<grid, 512, 0, st>>>(a, Kp / 2, sx, b, ldw / 2, ws, bi, yo, ldy, (int)M, (int)Np, \
-                                                                (int)(Kp / 2), part, kt_per, rows, (int)N, ConvGeom{})
+                                                                (int)(Kp / 2), part, kt_per, p.rows, (int)N, ConvGeom{})
   switch (p.tile) {
     case 0: PINGPONG(4, 2, 2); break;
     case 1: PINGPONG(3, 2, 2); break;

@@ -183,8 +183,10 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Cursor& c) {
   c.grp = 0;
   if (++c.head < a.Hkv) return;
   c.head = 0;
-  do c.len = uniform(seq_len(a, ++c.b));  // (the caller knows that there is a tile ahead)
-  while (c.len == 0);
+  do {  // (the caller knows that there is a tile ahead)
+    if (c.b + 1 >= a.B) c.len = 0;  // unless the lengths change meanwhile: tiles without keys, then
+    else c.len = uniform(seq_len(a, ++c.b));
+  } while (c.len == 0 && c.b + 1 < a.B);
   c.nt = (c.len + kTile - 1) / kTile;
 }
 // The list's split: `act` waves of each block (fewer than WPB where the list is so short that the
@@ -234,7 +236,6 @@ __device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t block, uint32_
   else r.c = (all + blocks * wpb - 1) / a.by_waves;
   const uint64_t first = ((uint64_t)block * r.act + wave) * r.c;
   if (wave >= r.act || first >= all) return r;
-  r.n = min(r.c, all - (uint32_t)first);
   // the sequence: the first one that ends behind tile `first`
   uint32_t t = (uint32_t)first / a.by_units;  // in tiles of one unit
   const uint32_t rest = (uint32_t)first - t * units;
@@ -243,9 +244,11 @@ __device__ __forceinline__ Run run_of(const AttnArgs& a, uint32_t block, uint32_
   while ((past = __ballot(up > t)) == 0) {
     t -= last(up);
     b0 += kWave;
+    if (b0 >= a.B) return r;  // (lengths that changed since they were summed)
     len = length(b0 + lane);
     up = prefix_sum(tiles(len));
   }
+  r.n = min(r.c, all - (uint32_t)first);
   const int w = __builtin_ctzll(past);
   r.at.b = b0 + w;
   r.at.len = __builtin_amdgcn_readlane(len, w);
@@ -678,7 +681,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a)
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int4 u = a.desc[blockIdx.x];
   if (u.w == 0) return;
-  const int first = blockIdx.x, last = u.z, rows = unit_rows(a, u.w - 1), dg = a.D / 4;
+  const int first = blockIdx.x, last = min(u.z, (int)gridDim.x - 1), rows = unit_rows(a, u.w - 1), dg = a.D / 4;
   const int e = blockIdx.y * 64 + lane;  // (row, group of 4)
   const int row = min(e / dg, rows - 1), d = e % dg * 4;
   float m = kNone, l = 0.f;

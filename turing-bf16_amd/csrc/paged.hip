@@ -22,7 +22,8 @@ struct CacheGeom {
 
 // ---- write ------------------------------------------------------------------------
 
-// A copy, bound by memory (8192 tokens of 8 heads of 128: 14.3 us, 4.7 TB/s). A block takes TB tokens: a
+// A copy, bound by memory (8192 tokens of 8 heads of 128: 18.5 us, 3.6 TB/s, from HBM; 13.5 us where the rows
+// are still in the on-chip cache). A block takes TB tokens: a
 // thread one 16-byte chunk of the keys' or values' heads, over the block's tokens (W threads a token,
 // so 256 / W tokens at once).
 // A slot that a later token names too is left to that token, so a repeated slot holds the last one's
@@ -122,10 +123,10 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
 // Memory bounds it: 16 KB a tile of D = 128 against ~ 550 instructions, 32 of them MFMAs.
 // K and V of the next tile are loaded as soon as this tile's registers are free, its page
 // entries one tile earlier, across the ends of units too. 128 sequences of 0 to 8192 keys, 8
-// heads of 128: 370 us, 5.8 TB/s; a kernel that only reads as many bytes, each wave a run of its
-// own: 352 us. 131072 keys of one sequence: 100 us, 5.3 TB/s (alone 90): ~ 10 us go into the lengths'
-// scan, the first loads, the joins and the second launch. Two tiles a wave in registers, blocks of 4
-// waves or more blocks than run at once were no faster (373, 375 and 371 to 394 us).
+// heads of 128: 366 us and 5 of the second launch, 5.9 TB/s; a kernel that only reads as many bytes, each
+// wave a run of its own: 350 us. 131072 keys of one sequence: 96 and 5 us, 5.6 TB/s (the same reading alone
+// 90): ~ 10 us go into the lengths' scan, the first loads, the joins and the second launch. Two tiles a wave
+// in registers, blocks of 4 waves or more blocks than run at once were no faster (by 1 to 7%).
 //
 // Tiles of all units form one list (by sequence, then head). Each wave takes an equal run of
 // it, so a batch of ragged lengths keeps every wave busy to the end. What a wave computes of a
@@ -737,9 +738,9 @@ AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
   p.R = (int)std::min<int64_t>(G, 16 * p.RT);
   p.RG = (int)cdiv(G, p.R);
   p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
-  // Few short units: a launch less on the host and on the device (1 x 32 heads, 100 keys: 5.2 us, the
-  // list and its join 8.7); with more tiles a wave the list's finer split wins (700 keys of 16 heads, 3
-  // tiles a wave: 10.9 and 9.6 us on the device, 14 and 17 with the host; 1000 keys, 4 tiles: 15.4 and 13.1)
+  // Few short units: a launch less on the host and on the device (1 x 32 heads, 100 keys: 5.5 us, the
+  // list and its join 8.4); with more tiles a wave the list's finer split wins (700 keys of 16 heads, 3
+  // tiles a wave: 12.6 and 9.9 us on the device, 12.6 and 16.1 with the host; at 1000 keys, 4 tiles, by 2.3)
   p.unit = cdiv(cap, kTile) <= 3 * p.wpb && B * Hkv * p.RG <= num_cus();
   p.stat = p.desc = p.bytes = 0;
   p.blocks = 0;

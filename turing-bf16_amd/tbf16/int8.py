@@ -118,8 +118,8 @@ def _ws_bytes(dev: int, *sizes: int) -> int:
 
 
 def int8_linear(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias=None):
-    """y = x @ W^T + b for bf16 x (..., K), with W given by prepare_weight_i8. Returns bf16
-    (..., N). Rows of x with an infinity or a NaN give NaN. Inference only."""
+    """y = x @ W^T + b for bf16 x (..., K), with W given by prepare_weight_i8 (its scales in fp32:
+    rounded ones are refused). Returns bf16 (..., N). Rows of x with an infinity or a NaN give NaN. Inference only."""
     if x.dtype != torch.bfloat16:
         raise TypeError("tbf16.int8_linear: expected bf16 x")
     if w8.dtype != torch.int8 or w8.dim() != 2:

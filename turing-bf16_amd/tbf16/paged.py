@@ -72,11 +72,17 @@ def _rows(t):
     return t, t.stride()
 
 
+def _span(t):
+    """The addresses from a bf16 tensor's first element to behind its last one."""
+    at = t.data_ptr()
+    return at, at + 2 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+
+
 def paged_write(k_cache, v_cache, k, v, slots) -> None:
     """k_cache[s // page, :, s % page] = k[t], v_cache likewise, for s = slots[t] of every
     token t. k, v bf16 (T, Hkv, D), any strides; slots int32 (T,). Slots outside the cache
     (negative: a padded batch) leave it as it is; where slots repeat, the last token's rows
-    stay. In place; k and v must not lie in the cache's own storage."""
+    stay. In place; k and v must not lie between the cache's first and last element."""
     (pages, Hkv, page, D), kc_st, kc, vc_st, vc = _cache("paged_write", k_cache, v_cache)
     _same_device("paged_write", k_cache, v_cache, k, v, slots)
     shape = k.shape
@@ -97,8 +103,13 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
     if kc == vc and pages:
         raise ValueError("tbf16.paged_write: k_cache and v_cache are the same memory")
     held = k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr()
-    if T and (k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held):
-        raise ValueError("tbf16.paged_write: k and v lie in the cache's storage")
+    if T and pages and (k.untyped_storage().data_ptr() in held or v.untyped_storage().data_ptr() in held):
+        # one allocation for all of them: fine where they lie apart in it
+        for t in (k, v):
+            for c in (k_cache, v_cache):
+                (t0, t1), (c0, c1) = _span(t), _span(c)
+                if t0 < c1 and c0 < t1:
+                    raise ValueError("tbf16.paged_write: k and v lie in the cache's storage, within its rows")
     torch.autograd.graph.increment_version((k_cache, v_cache))
     if T == 0 or pages == 0:
         return

@@ -316,6 +316,25 @@ int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D
                      int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale, void* o, void* ws,
                      int64_t ws_bytes, void* stream);
 
+/* A paged cache's bookkeeping: sequences get counts[b] tokens longer, or -counts[b] shorter. table
+ * int32 (B, max_pages), row stride table_stride; lengths, counts int32 (B,); free_pages int32
+ * (pages,), a stack of *n_free pages of the cache's `pages`, taken from its end; all on the device,
+ * and all but counts and prefix changed in place. First, entries of pages past the shortened lengths
+ * become -1 and go on the stack (the last sequence's last one first; those outside [0, pages) are
+ * left out). Then, with needs in pages, sequence b gets its counts[b] > 0 tokens if they fit its row,
+ * the sum of positive counts up to b is at most tokens, and it needs no page or the sum of the needs
+ * of sequences up to b that fit their rows is at most *n_free. starts int32 (B + 1,): where b's
+ * tokens begin, at most tokens. slots, positions int32 (tokens,): page id * page + row, old length +
+ * i + *prefix (0 if NULL), or -1 both for tokens that were not granted or are not there; a slot is -1
+ * too where the table names no page. B * max_pages and pages * page below 2^31. No two arrays
+ * overlap. ws: tbf16_paged_advance_ws_bytes(B) bytes, this call's alone until it has run. No
+ * counterpart in the reference. */
+size_t tbf16_paged_advance_ws_bytes(int64_t B);
+int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t B, int64_t max_pages, int32_t* lengths,
+                        const int32_t* counts, int32_t* free_pages, int64_t pages, int32_t* n_free, int64_t page,
+                        int64_t tokens, const int32_t* prefix, int32_t* slots, int32_t* positions, int32_t* starts,
+                        void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from ._ext import launch, lib
+from ._ext import launch, lib, ptr
 
 MAX_HEAD_DIM = 256
 
@@ -73,9 +73,86 @@ def _rows(t):
 
 
 def _span(t):
-    """The addresses from a bf16 tensor's first element to behind its last one."""
+    """The addresses from a tensor's first element to behind its last one."""
     at = t.data_ptr()
-    return at, at + 2 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+    return at, at + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+
+
+def _state(fn, tensors):
+    """Refuses tensors that the operator changes in place but cannot: not int32, not side by side,
+    or two of them in the same memory."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype is not torch.int32:
+            raise TypeError(f"tbf16.{fn}: expected {name} as int32, got {t.dtype}")
+        if name != "page_table" and t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1:
+            raise ValueError(f"tbf16.{fn}: {name} must be contiguous")
+    there = [t for t in tensors.values() if t is not None and t.numel()]
+    if len({t.untyped_storage().data_ptr() for t in there}) < len(there):
+        spans = sorted(_span(t) for t in there)
+        if any(b0 < a1 for (_, a1), (b0, _) in zip(spans, spans[1:])):
+            raise ValueError(f"tbf16.{fn}: {', '.join(tensors)} lie in the same memory")
+
+
+def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens, prefix_length=None):
+    """Makes sequences of a paged cache longer by counts[b] tokens, or shorter by -counts[b], and
+    says where the new tokens belong: (slots, positions, starts), int32 (tokens,), (tokens,) and
+    (B + 1,). All on the device, in place, without waiting for it:
+
+      page_table  int32 (B, n): sequence b's pages; lengths int32 (B,): its tokens so far
+      counts      int32 (B,): new tokens (0: none); negative: the last -counts[b] tokens are taken
+                  back, all of them where there are fewer (a request that ends: -lengths[b])
+      free_pages  int32 (pages,): a stack of the pages that nobody has, n_free int32 (1,) of them, the
+                  next one taken last; pages is also the number of the cache's pages
+      page        positions a page has; tokens: new tokens there is room for in this call
+
+    First, pages that no position below the shortened lengths uses go back on the stack and
+    their table entries become -1 (entries that name no page are not given back). Then sequences
+    get their new tokens in order of b. One whose tokens do not fit its table row or `tokens`, or
+    that needs pages that are no longer there after what the sequences before it asked for, gets
+    none: its length stays. The new tokens of all sequences lie one after the other, those of b
+    from starts[b] on (at most `tokens`): slots for paged_write, positions from the sequence's old
+    length on, plus prefix_length int32 (1,) where one is given (the tokens of a prefix that all
+    sequences share, which the tables do not hold). Tokens that were not granted, and those past
+    the last one, have slot and position -1, which paged_write leaves out and qk_norm_rope gives
+    zeros. Taking all granted tokens back leaves lengths, table and stack as they were.
+
+    Lengths outside [0, n * page] count as the nearest there is, n_free likewise."""
+    if page_table.dim() != 2:
+        raise ValueError(f"tbf16.paged_advance: page_table {tuple(page_table.shape)} is not (B, n)")
+    B, n = page_table.shape
+    for name, t in (("lengths", lengths), ("counts", counts)):
+        if t.shape != (B,):
+            raise ValueError(f"tbf16.paged_advance: {name} {tuple(t.shape)} for {B} sequences")
+    if free_pages.dim() != 1:
+        raise ValueError(f"tbf16.paged_advance: free_pages {tuple(free_pages.shape)} is not (pages,)")
+    for name, t in (("n_free", n_free), ("prefix_length", prefix_length)):
+        if t is not None and t.numel() != 1:
+            raise ValueError(f"tbf16.paged_advance: {name} is one number, got {tuple(t.shape)}")
+    state = {"page_table": page_table, "lengths": lengths, "counts": counts, "free_pages": free_pages, "n_free": n_free}
+    others = [lengths, counts, free_pages, n_free]
+    if prefix_length is not None:
+        state["prefix_length"] = prefix_length
+        others.append(prefix_length)
+    _same_device("paged_advance", page_table, *others)
+    _state("paged_advance", state)
+    pages, page, tokens = free_pages.shape[0], int(page), int(tokens)
+    row = page_table.stride(0) if B > 1 else max(n, 1)
+    if (n > 1 and page_table.stride(1) != 1) or row < n:
+        raise ValueError("tbf16.paged_advance: page_table's rows must be contiguous and apart")
+    if page < 1 or pages * page >= 2 ** 31 - 1:
+        raise ValueError(f"tbf16.paged_advance: {pages} pages of {page} positions")
+    if not 0 <= tokens < 2 ** 31 - 1024 or B * n >= 2 ** 31:
+        raise ValueError(f"tbf16.paged_advance: room for {tokens} tokens, page_table {tuple(page_table.shape)}")
+    torch.autograd.graph.increment_version((page_table, lengths, free_pages, n_free))
+    # one allocation: slots, positions, starts and the workspace
+    out = page_table.new_empty(2 * tokens + B + 1 + 3 * B + 4)
+    slots, positions, starts, ws = out.split((tokens, tokens, B + 1, 3 * B + 4))
+    launch("tbf16_paged_advance", page_table, page_table.data_ptr(), row, B, n, lengths.data_ptr(), counts.data_ptr(),
+           free_pages.data_ptr(), pages, n_free.data_ptr(), page, tokens, ptr(prefix_length), slots.data_ptr(),
+           positions.data_ptr(), starts.data_ptr(), ws.data_ptr(), 4 * ws.numel())
+    return slots, positions, starts
 
 
 def paged_write(k_cache, v_cache, k, v, slots) -> None:

@@ -316,6 +316,29 @@ int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D
                      int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale, void* o, void* ws,
                      int64_t ws_bytes, void* stream);
 
+/* RMS norm of each query and key head and rotation by position: with u = x / sqrt(mean x^2 + eps) and
+ * z = u w, the first R elements of z are rotated in pairs (i, i + R / 2), or (2 i, 2 i + 1) with
+ * interleaved != 0, by cos[pos][i], sin[pos][i]; the others stay. One rounding to bf16. q, k bf16 (B, S,
+ * H or Hkv, D), element strides (b, s, h) in q_st, k_st, D contiguous and a multiple of 16 up to
+ * 256, everything 16-byte aligned; wq, wk (D,) bf16, or fp32 with w_f32 != 0; cos, sin fp32 (rows, R / 2)
+ * contiguous, R a multiple of 16; pos int32 (B, S), element strides p_sb, p_ss. Tokens of negative
+ * position give zeros, of positions from `rows` on NaN. yq, yk bf16 contiguous.
+ * The gradient: dq, dk, bf16 contiguous, dwq, dwk (D,) in the weights' type, each may be NULL, from dyq,
+ * dyk with strides of their own; sums over tokens in a fixed order. ws:
+ * tbf16_qk_norm_rope_bwd_ws_bytes(B, S, D) bytes (asked with the stream's device current), this call's
+ * alone until it has run; not used without dwq and dwk. No counterpart in the reference. */
+int tbf16_qk_norm_rope(const void* q, const void* k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D,
+                       const int64_t* q_st, const int64_t* k_st, const void* wq, const void* wk, int w_f32,
+                       const float* cos, const float* sin, int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb,
+                       int64_t p_ss, float eps, int interleaved, void* yq, void* yk, void* stream);
+size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t D);
+int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, int64_t B, int64_t S, int64_t H,
+                           int64_t Hkv, int64_t D, const int64_t* q_st, const int64_t* k_st, const int64_t* dyq_st,
+                           const int64_t* dyk_st, const void* wq, const void* wk, int w_f32, const float* cos,
+                           const float* sin, int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb, int64_t p_ss,
+                           float eps, int interleaved, void* dq, void* dk, void* dwq, void* dwk, void* ws,
+                           int64_t ws_bytes, void* stream);
+
 /* A paged cache's bookkeeping: sequences get counts[b] tokens longer, or -counts[b] shorter. table
  * int32 (B, max_pages), row stride table_stride; lengths, counts int32 (B,); free_pages int32
  * (pages,), a stack of *n_free pages of the cache's `pages`, taken from its end; all on the device,

@@ -46,3 +46,55 @@ def advance_by_hand(table, lengths, counts, stack, n_free, page, tokens, prefix=
             starts.append(starts[-1])
     pad = [-1] * (tokens - len(slots))
     return n_free, slots + pad, positions + pad, starts
+
+
+def rotate64(z, cos, sin, near, back=False):
+    """The first 2 * cos.shape[-1] elements of z in pairs turned by the angles (or back)."""
+    R = 2 * cos.shape[-1]
+    a, b = (z[..., 0:R:2], z[..., 1:R:2]) if near else (z[..., :R // 2], z[..., R // 2:R])
+    s = -sin if back else sin
+    y = z.clone()
+    ya, yb = a * cos - b * s, b * cos + a * s
+    if near:
+        y[..., 0:R:2], y[..., 1:R:2] = ya, yb
+    else:
+        y[..., :R // 2], y[..., R // 2:R] = ya, yb
+    return y
+
+
+def norm_rope64(x, w, cos, sin, pos, eps=1e-6, near=False, dy=None):
+    """On the CPU in 64 bits, x (..., H, D), pos of its leading dimensions: (y, bound), and with dy
+    (y, bound, dx, bound, dw, bound before the rounding of dw). u = half a step of fp32 for each rounding:
+      r            the squares' sum (16 in turn, 4 steps across lanes, a product each) half of it, the mean, eps,
+                   the root: under 16 u of r
+      y            r, x r, w, and the rotation's two products and sum: 24 u of |z_i c| + |z_j s|
+      dx           dy turned back (3 u of A = |dy_i c| + |dy_j s|), w, x r (18 u), the mean of D products (20 sums), their
+                   difference, r, scale: under 80 u of r (A |w| + |x r| mean(A |w x r|))
+      dw           products (22 u) and as many sums as a lane makes and the blocks' shares pass through
+    and half a step of bf16 of what comes out as such."""
+    D = x.shape[-1]
+    x, w, pos = x.detach().cpu().double(), w.detach().cpu().double(), pos.cpu().long()
+    at = pos.clamp(0, cos.shape[0] - 1)
+    c, s = (t.cpu().double()[at].unsqueeze(-2) for t in (cos, sin))
+    real = (pos >= 0)[..., None, None]
+    r = 1.0 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+    u = x * r
+    z = u * w
+    y = torch.where(real, rotate64(z, c, s, near), 0.0)
+    size = rotate64(z.abs(), c.abs(), -s.abs(), near)  # |z_i c| + |z_j s| in the first of a pair
+    size = torch.maximum(size, rotate64(z.abs(), c.abs(), s.abs(), near))
+    out = [y, torch.where(real, 2.0 ** -8 * y.abs() + 24 * U24 * size, 0.0)]
+    if dy is None:
+        return tuple(out)
+    g = dy.detach().cpu().double()
+    A = torch.maximum(rotate64(g.abs(), c.abs(), -s.abs(), near), rotate64(g.abs(), c.abs(), s.abs(), near))
+    dz = torch.where(real, rotate64(g, c, s, near, back=True), 0.0)
+    A = torch.where(real, A, 0.0)
+    du = dz * w
+    dx = r * (du - u * (du * u).mean(-1, keepdim=True))
+    spread = r * (A * w.abs() + u.abs() * (A * (w * u).abs()).mean(-1, keepdim=True))
+    tokens, H = pos.numel(), x.shape[-2]
+    sums = -(-H // (64 // (4 if D <= 64 else 8 if D <= 128 else 16))) * -(-tokens // 4096) + 90
+    flat = lambda t: t.flatten(0, -2)  # noqa: E731
+    dw, dw_bound = flat(dz * u).sum(0), (22 + sums) * U24 * flat(A * u.abs()).sum(0)
+    return (*out, dx, 2.0 ** -8 * dx.abs() + 80 * U24 * spread, dw, dw_bound)

@@ -6,7 +6,7 @@ import torch
 import tbf16
 from tbf16 import _ext, paged
 
-from _operators64 import advance_by_hand
+from _operators64 import advance_by_hand, norm_rope64
 
 I32 = torch.int32
 
@@ -93,3 +93,104 @@ def test_advance_by_hand():
     table, lengths, stack = [[0, 2], [1, -1]], [5, 4], [3, 3, 3, 3]
     assert advance_by_hand(table, lengths, [-1, 1], stack, 0, 4, 2) == (0, [8, -1], [4, -1], [0, 0, 1])
     assert table == [[0, -1], [1, 2]] and lengths == [4, 5] and stack == [2, 3, 3, 3]
+
+
+BF = torch.bfloat16
+
+
+def norm(S=5, H=4, Hkv=2, D=64, R=32, rows=10):
+    return {"q": torch.zeros(S, H, D, dtype=BF), "k": torch.zeros(S, Hkv, D, dtype=BF), "q_weight": torch.ones(D, dtype=BF),
+            "k_weight": torch.ones(D, dtype=BF), "cos": torch.ones(rows, R // 2), "sin": torch.zeros(rows, R // 2),
+            "positions": torch.zeros(S, dtype=I32)}
+
+
+@pytest.mark.parametrize("wrong,error,text", [
+    (dict(q=torch.zeros(5, 64, dtype=BF)), ValueError, "are not"),
+    (dict(q=torch.zeros(1, 1, 5, 4, 64, dtype=BF)), ValueError, "are not"),
+    (dict(k=torch.zeros(6, 2, 64, dtype=BF)), ValueError, "are not"),
+    (dict(k=torch.zeros(5, 2, 48, dtype=BF)), ValueError, "are not"),
+    (dict(k=torch.zeros(5, 0, 64, dtype=BF)), ValueError, "are not"),
+    (dict(q=torch.zeros(5, 4, 72, dtype=BF), k=torch.zeros(5, 2, 72, dtype=BF)), ValueError, "head dim 72"),
+    (dict(q=torch.zeros(5, 4, 272, dtype=BF), k=torch.zeros(5, 2, 272, dtype=BF)), ValueError, "head dim 272"),
+    (dict(q=torch.zeros(5, 4, 64)), TypeError, "bf16 q"),
+    (dict(q_weight=torch.ones(32, dtype=BF)), ValueError, "weights"),
+    (dict(q_weight=torch.ones(64)), TypeError, "weights both"),
+    (dict(q_weight=torch.ones(64).half(), k_weight=torch.ones(64).half()), TypeError, "weights both"),
+    (dict(cos=torch.ones(10, 8)), ValueError, "one shape"),
+    (dict(cos=torch.ones(0, 16), sin=torch.ones(0, 16)), ValueError, "one shape"),
+    (dict(cos=torch.ones(10, 16).double(), sin=torch.ones(10, 16).double()), TypeError, "fp32 cos"),
+    (dict(cos=torch.ones(10, 12), sin=torch.ones(10, 12)), ValueError, "24 rotated"),
+    (dict(cos=torch.ones(10, 40), sin=torch.ones(10, 40)), ValueError, "80 rotated"),
+    (dict(cos=torch.ones(10, 0), sin=torch.ones(10, 0)), ValueError, "0 rotated"),
+    (dict(positions=torch.zeros(5, dtype=torch.int64)), TypeError, "int32 positions"),
+    (dict(positions=torch.zeros(4, dtype=I32)), ValueError, "positions"),
+    (dict(eps=-1.0), ValueError, "eps"),
+    (dict(eps=float("nan")), ValueError, "eps"),
+    (dict(eps=float("inf")), ValueError, "eps"),
+    (dict(), ValueError, "ROCm"),
+])
+@pytest.mark.parametrize("fn", [tbf16.qk_norm_rope, tbf16.autograd.qk_norm_rope])
+def test_norm_rope_refusals(fn, wrong, error, text):
+    with pytest.raises(error, match=text):
+        fn(**{**norm(), **wrong})
+
+
+def test_norm_rope_tables_have_no_gradient():
+    a = norm()
+    a["cos"] = a["cos"].requires_grad_()
+    with pytest.raises(ValueError, match="no gradients of cos"):
+        tbf16.autograd.qk_norm_rope(**a)
+
+
+def test_norm_rope_abi_refusals():
+    import ctypes
+    L = _ext.lib()
+    err = lambda: L.tbf16_last_error().decode()  # noqa: E731
+    st = lambda *v: (ctypes.c_int64 * 3)(*v)  # noqa: E731
+
+    def tail(rows=9, R=32, eps=1e-6, cos=16):
+        return 16, 16, 0, cos, 16, rows, R, 16, 0, 1, eps, 0
+
+    def fwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st(0, 64, 64), **kw):
+        return L.tbf16_qk_norm_rope(q, 16, B, S, H, Hkv, D, q_st, st(0, 64, 64), *tail(**kw), 16, 16, None)
+
+    def bwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st(0, 64, 64), ws=16, wsb=0, dwq=16, **kw):
+        return L.tbf16_qk_norm_rope_bwd(q, 16, 16, 16, B, S, H, Hkv, D, q_st, st(0, 64, 64), st(0, 64, 64), st(0, 64, 64),
+                                        *tail(**kw), None, None, dwq, None, ws, wsb, None)
+
+    for bad, text in [(dict(B=-1), "tokens"), (dict(S=2 ** 31), "tokens"), (dict(H=0), "heads"), (dict(D=24), "head dim"),
+                      (dict(D=272), "head dim"), (dict(R=8), "rotated"), (dict(R=0), "rotated"), (dict(R=80), "rotated"),
+                      (dict(rows=0), "tables"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+                      (dict(q=24), "aligned"), (dict(q_st=st(0, 64, 4)), "aligned"), (dict(cos=8), "misaligned")]:
+        assert fwd(**bad) == -1 and text in err(), (bad, err())
+        assert bwd(**bad) == -1 and text in err(), (bad, err())
+    assert bwd() == -3 and "workspace" in err()
+    assert bwd(ws=None, wsb=1 << 30) == -3
+    assert fwd(B=0) == 0 and fwd(S=0) == 0 and bwd(S=0, dwq=None) == 0
+    assert L.tbf16_qk_norm_rope_bwd_ws_bytes(2, 100, 64) > 0 == L.tbf16_qk_norm_rope_bwd_ws_bytes(0, 100, 64)
+
+
+@pytest.mark.parametrize("near", [False, True])
+def test_norm_rope64_against_differences(near):
+    """The oracle's gradients by central differences, its rotation as a complex product."""
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(3, 2, 32, generator=g).double(), torch.randn(32, generator=g).double()
+    ang = torch.rand(4, 8, generator=g).double() * 6
+    pos = torch.tensor([2, -1, 0], dtype=I32)
+    dy = torch.randn(3, 2, 32, generator=g).double()
+    f = lambda x, w: norm_rope64(x, w, ang.cos(), ang.sin(), pos, 1e-3, near)[0]  # noqa: E731
+    _, _, dx, _, dw, _ = norm_rope64(x, w, ang.cos(), ang.sin(), pos, 1e-3, near, dy)
+    for t, grad in ((x, dx), (w, dw)):
+        for _ in range(40):
+            i = tuple(int(torch.randint(0, n, (), generator=g)) for n in t.shape)
+            lo, hi = t.clone(), t.clone()
+            lo[i] -= 1e-5
+            hi[i] += 1e-5
+            d = ((f(hi, w) - f(lo, w)) * dy).sum() / 2e-5 if t is x else ((f(x, hi) - f(x, lo)) * dy).sum() / 2e-5
+            assert abs(d - grad[i]) <= 1e-7 * (1 + abs(grad[i]))
+    y, z = f(x, w)[0, 0], x[0, 0] / torch.sqrt(x[0, 0].square().mean() + 1e-3) * w
+    a, b = (z[0:16:2], z[1:16:2]) if near else (z[:8], z[8:16])
+    turned = torch.complex(a, b) * torch.exp(1j * ang[2])
+    got = torch.complex(y[0:16:2], y[1:16:2]) if near else torch.complex(y[:8], y[8:16])
+    # (a quotient and a product with the reciprocal: a few roundings of 2^-53 of values below 8)
+    assert (got - turned).abs().max() < 1e-14 and (y[16:] - z[16:]).abs().max() < 1e-14 and not f(x, w)[1].any()

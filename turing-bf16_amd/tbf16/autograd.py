@@ -23,7 +23,7 @@ import os
 import torch
 import torch.nn.functional as F
 
-from . import attention, ops, routing
+from . import attention, norm_rope, ops, routing
 from ._ext import launch, lib, ptr, strides3
 
 # How the attention backward applies the overflow retry (TBF16_ATTN_CHECK):
@@ -427,3 +427,29 @@ def sdpa(q, k, v, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None, en
     qp, kp, vp, sc, D = attention.pad_head_dim(q, k, v, scale)
     out = ScaledSDPAFn.apply(qp, kp, vp, attn_mask, dropout_p, is_causal, sc, enable_gqa, D)
     return out if out.shape[-1] == D else out[..., :D]
+
+
+class QKNormRopeFn(torch.autograd.Function):
+    """tbf16.qk_norm_rope with its gradients: the norms are computed again in the backward pass from the
+    saved inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.how = eps, interleaved
+        return norm_rope.Call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved).forward()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        call = norm_rope.Call(*ctx.saved_tensors, *ctx.how)
+        return (*call.backward(dyq, dyk, *ctx.needs_input_grad[:4]), None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):
+    """Differentiable tbf16.qk_norm_rope: gradients of q, k (bf16) and both weights (their own type), sums
+    over tokens and heads in fp32 in a fixed order. Tokens of a negative position have no share in
+    any. cos, sin and positions are constants."""
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("tbf16.autograd.qk_norm_rope: no gradients of cos and sin")
+    return QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)

@@ -316,6 +316,21 @@ int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D
                      int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale, void* o, void* ws,
                      int64_t ws_bytes, void* stream);
 
+/* tbf16_paged_attn where all sequences begin with the same tokens: keys are positions j <
+ * *prefix_length of prefix_table int32 (prefix_pages,) and then positions j < lengths[b] of the
+ * sequence's own table, in one softmax. The prefix is read once for the batch. B * H below 1e9. Other
+ * arguments and limits as tbf16_paged_attn's; the size query takes prefix_pages * page and max_pages
+ * * page. Weights of prefix keys below 2^-80 of the row's largest may count as zero. No counterpart in
+ * the reference. */
+size_t tbf16_paged_attn_prefix_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_positions,
+                                        int64_t positions);
+int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
+                            const void* k_cache, const void* v_cache, int64_t pages, int64_t page, int64_t kc_sp,
+                            int64_t kc_sh, int64_t kc_ss, int64_t vc_sp, int64_t vc_sh, int64_t vc_ss,
+                            const int32_t* prefix_table, int64_t prefix_pages, const int32_t* prefix_length,
+                            const int32_t* table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                            float scale, void* o, void* ws, int64_t ws_bytes, void* stream);
+
 /* RMS norm of each query and key head and rotation by position: with u = x / sqrt(mean x^2 + eps) and
  * z = u w, the first R elements of z are rotated in pairs (i, i + R / 2), or (2 i, 2 i + 1) with
  * interleaved != 0, by cos[pos][i], sin[pos][i]; the others stay. One rounding to bf16. q, k bf16 (B, S,

@@ -98,3 +98,41 @@ def norm_rope64(x, w, cos, sin, pos, eps=1e-6, near=False, dy=None):
     flat = lambda t: t.flatten(0, -2)  # noqa: E731
     dw, dw_bound = flat(dz * u).sum(0), (22 + sums) * U24 * flat(A * u.abs()).sum(0)
     return (*out, dx, 2.0 ** -8 * dx.abs() + 80 * U24 * spread, dw, dw_bound)
+
+
+def prefix_sdpa64(q, k_cache, v_cache, prefix_table, prefix_length, table, lengths, scale=None):
+    """(o, bound) on the CPU: attention of each sequence over the prefix's positions and its own, from the
+    definition in 64 bits. bound: half a bf16 step of o, and of the error before it at most e sum_j p_j
+    |v_j| / sum_j p_j, where e sums
+      2 (D + 4) 2^-23 max_j scale sum |q k_j|   a logit's products, D sums and factors, in a weight and in their sum
+      2^-16 + 2^-17                             a weight as two bf16 (8 bits cut off, the rest, below 2^-7 of it, to 8
+                                                bits: half of 2^-15); exp2 and the joins' factors
+      (n / 32 + 64) 2^-23                       n weighted values added 32 at a time, the parts of the joins"""
+    q, k_cache, v_cache, prefix_table, table = (t.cpu() for t in (q, k_cache, v_cache, prefix_table, table))
+    B, H, D = q.shape
+    pages, Hkv, page, _ = k_cache.shape
+    G = H // Hkv
+    sc = D ** -0.5 if scale is None else scale
+
+    def places(ids, n):
+        j = torch.arange(max(0, min(int(n), ids.shape[0] * page)))
+        at = ids.long()[j // page] if len(j) else j
+        ok = (at >= 0) & (at < pages)
+        return at[ok], (j % page)[ok]
+    far = places(prefix_table, prefix_length)
+    shared = [(k_cache[far[0], h, far[1]].double(), v_cache[far[0], h, far[1]].double()) for h in range(Hkv)]
+    o, bound = torch.zeros(B, H, D, dtype=torch.float64), torch.zeros(B, H, D, dtype=torch.float64)
+    for b, n in enumerate(lengths.tolist()):
+        at, off = places(table[b], n)
+        if len(at) + len(far[0]) == 0:
+            continue
+        for h in range(Hkv):
+            k = torch.cat((shared[h][0], k_cache[at, h, off].double()))
+            v = torch.cat((shared[h][1], v_cache[at, h, off].double()))
+            qg = q[b, h * G:(h + 1) * G].double()
+            p = torch.softmax(qg @ k.t() * sc, -1)
+            o[b, h * G:(h + 1) * G] = p @ v
+            size = (qg.abs() @ k.abs().t() * abs(sc)).amax(-1, keepdim=True)
+            e = 2 * (D + 4) * 2 * U24 * size + 1.5 * 2.0 ** -16 + (len(k) / 32 + 64) * 2 * U24
+            bound[b, h * G:(h + 1) * G] = 2.0 ** -8 * o[b, h * G:(h + 1) * G].abs() + 1.01 * e * (p @ v.abs())
+    return o, bound

@@ -194,3 +194,56 @@ def test_norm_rope64_against_differences(near):
     got = torch.complex(y[0:16:2], y[1:16:2]) if near else torch.complex(y[:8], y[8:16])
     # (a quotient and a product with the reciprocal: a few roundings of 2^-53 of values below 8)
     assert (got - turned).abs().max() < 1e-14 and (y[16:] - z[16:]).abs().max() < 1e-14 and not f(x, w)[1].any()
+
+
+def prefix(pages=4, Hkv=2, page=16, D=64, B=3, H=4, m=2, n=2):
+    z = lambda *s, t=I32: torch.zeros(*s, dtype=t)  # noqa: E731
+    return {"q": z(B, H, D, t=BF), "k_cache": z(pages, Hkv, page, D, t=BF), "v_cache": z(pages, Hkv, page, D, t=BF),
+            "prefix_table": z(m), "prefix_length": z(1), "page_table": z(B, n), "lengths": z(B)}
+
+
+@pytest.mark.parametrize("wrong,error,text", [
+    (dict(k_cache=torch.zeros(4, 2, 16, 64)), TypeError, "bf16 cache"),
+    (dict(v_cache=torch.zeros(4, 2, 16, 72, dtype=BF)), ValueError, "one shape"),
+    (dict(k_cache=torch.zeros(4, 2, 16, 264, dtype=BF), v_cache=torch.zeros(4, 2, 16, 264, dtype=BF)), ValueError, "head dim"),
+    (dict(q=torch.zeros(3, 4, 72, dtype=BF)), ValueError, "is not"),
+    (dict(q=torch.zeros(3, 4, 64)), TypeError, "bf16 q"),
+    (dict(q=torch.zeros(3, 5, 64, dtype=BF)), ValueError, "query heads"),
+    (dict(page_table=torch.zeros(3, 2, dtype=torch.int64)), TypeError, "page_table as an int32"),
+    (dict(page_table=torch.zeros(2, 2, dtype=I32)), ValueError, "sequences"),
+    (dict(lengths=torch.zeros(4, dtype=I32)), ValueError, "sequences"),
+    (dict(prefix_table=torch.zeros(1, 2, dtype=I32)), TypeError, "prefix_table as an int32"),
+    (dict(prefix_table=torch.zeros(2)), TypeError, "prefix_table as an int32"),
+    (dict(prefix_length=torch.zeros(3, dtype=I32)), TypeError, "one int32"),
+    (dict(prefix_length=torch.zeros(1, dtype=torch.int64)), TypeError, "one int32"),
+])
+def test_prefix_refusals(host, wrong, error, text):
+    with pytest.raises(error, match=text):
+        tbf16.paged_sdpa_prefix(**{**prefix(), **wrong})
+
+
+def test_prefix_host_tensors_are_refused():
+    with pytest.raises(ValueError, match="ROCm"):
+        tbf16.paged_sdpa_prefix(**prefix())
+
+
+def test_prefix_abi_refusals():
+    L = _ext.lib()
+    err = lambda: L.tbf16_last_error().decode()  # noqa: E731
+    s2, s3 = (128, 64), (2048, 1024, 64)
+
+    def call(B=1, H=2, Hkv=2, D=64, qs=s2, kc=16, pages=4, page=16, ks=s3, vs=s3, pt=16, pn=100, n=400, ws=16, wsb=1 << 40, q=16):
+        return L.tbf16_paged_attn_prefix(q, B, H, Hkv, D, *qs, kc, 16, pages, page, *ks, *vs, pt, pn, 16, 16, 400, n, 16, 1.0, 16,
+                                         ws, wsb, None)
+
+    for bad, text in [(dict(H=3), "multiple of key/value heads"), (dict(D=60), "multiple of 8"), (dict(D=264), "256"),
+                      (dict(kc=18), "aligned"), (dict(ks=(2048, 1020, 64)), "strides"), (dict(vs=(2 ** 31, 1024, 64)), "stride"),
+                      (dict(qs=(128, 60)), "q must"), (dict(q=24), "q must"), (dict(page=0), "bad cache"),
+                      (dict(Hkv=0), "bad cache"), (dict(B=-1), "bad shape"), (dict(ws=24), "workspace"), (dict(ws=None), "workspace"),
+                      (dict(pn=-1), "too wide"), (dict(n=2 ** 31), "too wide"), (dict(pt=6), "4-byte"), (dict(B=10 ** 9), "large")]:
+        assert call(**bad) == -1, bad
+        assert text in err(), (bad, err())
+    assert call(B=64, wsb=0) == -3 and "workspace" in err()
+    assert call(B=0) == 0
+    small, large = (L.tbf16_paged_attn_prefix_ws_bytes(B, 32, 8, 128, 4096, 512) for B in (1, 64))
+    assert 0 < small < large and L.tbf16_paged_attn_prefix_ws_bytes(0, 32, 8, 128, 4096, 512) == 0

@@ -12,10 +12,10 @@ from .convert import Int8Linear, Linear, TrainLinear, convert, install_sdpa, is_
 from .int8 import int8_linear, prepare_weight_i8, quantize_rows_i8
 from .norm_rope import qk_norm_rope
 from .ops import prepare_weight, quantize_rows, scaled_linear
-from .paged import paged_advance, paged_sdpa, paged_write
+from .paged import paged_advance, paged_sdpa, paged_sdpa_prefix, paged_write
 from .patch import TuringBF16Mode, patch
 
 __all__ = ["quantize_rows", "scaled_linear", "prepare_weight", "sdpa", "patch", "TuringBF16Mode", "convert",
            "Linear", "TrainLinear", "autograd", "install_sdpa", "uninstall_sdpa",
-           "is_supported_gpu", "qk_norm_rope", "paged_advance", "paged_sdpa", "paged_write", "int8_linear", "prepare_weight_i8", "quantize_rows_i8",
+           "is_supported_gpu", "qk_norm_rope", "paged_advance", "paged_sdpa", "paged_sdpa_prefix", "paged_write", "int8_linear", "prepare_weight_i8", "quantize_rows_i8",
            "Int8Linear"]

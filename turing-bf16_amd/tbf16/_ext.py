@@ -73,6 +73,8 @@ _SIGS = {
     "tbf16_paged_write": (I, [P, P] + [I64] * 7 + [P, P, P] + [I64] * 8 + [P]),
     "tbf16_paged_advance_ws_bytes": (SZ, [I64]),
     "tbf16_paged_advance": (I, [P, I64, I64, I64, P, P, P, I64, P, I64, I64, P, P, P, P, P, I64, P]),
+    "tbf16_paged_attn_prefix_ws_bytes": (SZ, [I64] * 6),
+    "tbf16_paged_attn_prefix": (I, [P] + [I64] * 6 + [P, P] + [I64] * 8 + [P, I64, P, P, I64, I64, P, F, P, P, I64, P]),
     "tbf16_paged_attn_ws_bytes": (SZ, [I64] * 5),
     "tbf16_paged_attn": (I, [P] + [I64] * 6 + [P, P] + [I64] * 8 + [P, I64, I64, P, F, P, P, I64, P]),
 }

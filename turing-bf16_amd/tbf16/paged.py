@@ -195,20 +195,39 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
            slots.data_ptr(), kc, vc, pages, page, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
 
 
-# tbf16_paged_attn's workspace bytes per (device, B, H, Hkv, D, positions a table row covers): its
-# blocks are counted by the device's CUs, so it is asked on the tensors' device, once
+# workspace bytes per (device, entry point, its sizes): blocks are counted by the device's CUs, so it
+# is asked on the tensors' device, once
 _WS_BYTES: dict = {}
 
 
-def _ws_bytes(dev: int, *sizes: int) -> int:
-    key = (dev, sizes)
+def _ws_bytes(dev: int, name: str, *sizes: int) -> int:
+    key = (dev, name, sizes)
     n = _WS_BYTES.get(key)
     if n is None:
         if len(_WS_BYTES) > 4096:
             _WS_BYTES.clear()
         with torch.cuda.device(dev):
-            n = _WS_BYTES[key] = int(lib().tbf16_paged_attn_ws_bytes(*sizes))
+            n = _WS_BYTES[key] = int(getattr(lib(), name)(*sizes))
     return n
+
+
+def _queries(fn, q, shape, page_table, lengths):
+    """The checked q, page_table and lengths of an attention over a cache of `shape`."""
+    _, Hkv, _, D = shape
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"tbf16.{fn}: q {tuple(q.shape)} is not (B, H, {D})")
+    if q.dtype is not torch.bfloat16:
+        raise TypeError(f"tbf16.{fn}: expected bf16 q")
+    B, H, _ = q.shape
+    if H == 0 or H % Hkv:
+        raise ValueError(f"tbf16.{fn}: {H} query heads over {Hkv} key/value heads")
+    page_table = _index(fn, "page_table", page_table, 2)
+    lengths = _index(fn, "lengths", lengths, 1)
+    rows = page_table.shape[0]
+    if rows != B or lengths.shape[0] != B:
+        raise ValueError(f"tbf16.{fn}: page_table for {rows} and lengths for {lengths.shape[0]} sequences, q has {B}")
+    q, q_st = _rows(q)
+    return q, q_st, page_table, lengths
 
 
 def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
@@ -224,25 +243,43 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     is NaN."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa", k_cache, v_cache)
     _same_device("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"tbf16.paged_sdpa: q {tuple(q.shape)} is not (B, H, {D})")
-    if q.dtype is not torch.bfloat16:
-        raise TypeError("tbf16.paged_sdpa: expected bf16 q")
-    B, H, _ = q.shape
-    if H == 0 or H % Hkv:
-        raise ValueError(f"tbf16.paged_sdpa: {H} query heads over {Hkv} key/value heads")
-    page_table = _index("paged_sdpa", "page_table", page_table, 2)
-    lengths = _index("paged_sdpa", "lengths", lengths, 1)
-    rows, n = page_table.shape
-    if rows != B or lengths.shape[0] != B:
-        raise ValueError(f"tbf16.paged_sdpa: page_table for {rows} and lengths for {lengths.shape[0]} sequences, q has {B}")
-    q, q_st = _rows(q)
+    q, q_st, page_table, lengths = _queries("paged_sdpa", q, k_cache.shape, page_table, lengths)
+    (B, H, _), n = q.shape, page_table.shape[1]
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return o
-    wsb = _ws_bytes(q.get_device(), B, H, Hkv, D, n * page)
+    wsb = _ws_bytes(q.get_device(), "tbf16_paged_attn_ws_bytes", B, H, Hkv, D, n * page)
     ws = q.new_empty(wsb, dtype=torch.uint8) if wsb else o  # (o: nothing is written there)
     launch("tbf16_paged_attn", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], kc, vc, pages, page, k_st[0], k_st[1],
            k_st[2], v_st[0], v_st[1], v_st[2], page_table.data_ptr(), page_table.stride(0), n, lengths.data_ptr(),
            D ** -0.5 if scale is None else float(scale), o.data_ptr(), ws.data_ptr(), wsb)
+    return o
+
+
+def paged_sdpa_prefix(q, k_cache, v_cache, prefix_table, prefix_length, page_table, lengths, scale=None):
+    """paged_sdpa where all sequences begin with the same tokens (a system prompt, a document that
+    all of them ask about): positions j < prefix_length[0] of prefix_table int32 (m,), int32 (1,), come
+    before each sequence's own positions j < lengths[b] of page_table. The prefix's keys and values
+    are read once for the whole batch and multiplied with all its queries. One softmax over both:
+    the result is paged_sdpa's on tables that begin with prefix_table's pages.
+
+    Arguments, results and limits as paged_sdpa's; a sequence without any key gives zeros. Weights of
+    prefix keys enter the second product with 16 bits, and below 2^-80 of the row's largest may count
+    as zero (an infinite value then gives NaN)."""
+    (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa_prefix", k_cache, v_cache)
+    _same_device("paged_sdpa_prefix", k_cache, v_cache, q, prefix_table, prefix_length, page_table, lengths)
+    q, q_st, page_table, lengths = _queries("paged_sdpa_prefix", q, k_cache.shape, page_table, lengths)
+    prefix_table = _index("paged_sdpa_prefix", "prefix_table", prefix_table, 1)
+    if prefix_length.dtype is not torch.int32 or prefix_length.numel() != 1:
+        raise TypeError(f"tbf16.paged_sdpa_prefix: expected prefix_length as one int32, got {tuple(prefix_length.shape)}")
+    (B, H, _), m, n = q.shape, prefix_table.shape[0], page_table.shape[1]
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if B == 0:
+        return o
+    wsb = _ws_bytes(q.get_device(), "tbf16_paged_attn_prefix_ws_bytes", B, H, Hkv, D, m * page, n * page)
+    ws = q.new_empty(wsb, dtype=torch.uint8)
+    launch("tbf16_paged_attn_prefix", q, q.data_ptr(), B, H, Hkv, D, q_st[0], q_st[1], kc, vc, pages, page, k_st[0],
+           k_st[1], k_st[2], v_st[0], v_st[1], v_st[2], prefix_table.data_ptr(), m, prefix_length.data_ptr(),
+           page_table.data_ptr(), page_table.stride(0), n, lengths.data_ptr(), D ** -0.5 if scale is None else float(scale),
+           o.data_ptr(), ws.data_ptr(), wsb)
     return o

@@ -196,7 +196,7 @@ extern "C" int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv
   const AttnArgs a = attn_args(p, q, B, H, Hkv, D, q_sb, q_sh, k_cache, v_cache, pages, page, kg, vg, table, table_stride,
                                max_pages, lengths, scale, o, ws);
   const hipStream_t st = as_stream(stream);
-  launch_attn<false>(a, p, st);
+  launch_attn(a, p, st);
   TB_LAUNCH_CHECK("paged_attn");
   if (!p.unit) {
     paged_join_kernel<<<dim3((unsigned)p.blocks, (unsigned)cdiv(p.R * D, 256)), kJoinWaves * 64, 0, st>>>(a);

@@ -233,10 +233,10 @@ struct Acc {
       if (lane < 16) *reinterpret_cast<float2*>(stat + 2 * row) = make_float2(m[r], l[r]);
     }
   }
-  // adds what n others put, part w at rows + w step and stat + w stat_step: the common maximum
+  // adds what n others put, part w at rows_of(w) and stat + w stat_step: the common maximum
   // first, so that the parts' loads do not wait for each other
-  __device__ __forceinline__ void take(const float* rows, int step, int ld, const float* stat, int stat_step, int n, int R,
-                                       int D, int lane) {
+  template <class Rows>
+  __device__ __forceinline__ void take(Rows rows_of, int ld, const float* stat, int stat_step, int n, int R, int D, int lane) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = 16 * r + (lane & 15);
@@ -255,7 +255,7 @@ struct Acc {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int d = 0; d < CH; d += 4)
-            v[i][d / 4] = *reinterpret_cast<const float4*>(rows + w * step + row * ld + CH * (4 * (lane >> 4) + i) + d);
+            v[i][d / 4] = *reinterpret_cast<const float4*>(rows_of(w) + row * ld + CH * (4 * (lane >> 4) + i) + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -313,35 +313,35 @@ __device__ __forceinline__ void unit_done(const AttnArgs& a, const A& acc, int b
 
 // DP: D rounded up to 64, 128 or 256 (D == DP unless PAD). WPB waves a block. UNIT: one block
 // per unit instead of equal runs of the list. PART: sums for a later launch instead of outputs.
-template <int DP, int RT, int WPB, bool PAD, bool UNIT, bool PART>
-__global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 : 2) void paged_attn_kernel(AttnArgs a) {
+// Block `block` of `blocks` (the list), or unit (block, head, grp). In LDS: rows_of(wave) [R][DP + 4], stat0
+// [wave][R][2], flags[WPB] (1: the wave left a part of a unit begun before it, 2: its last).
+template <int DP, int RT, int WPB, bool PAD, bool UNIT, bool PART, class Rows>
+__device__ __forceinline__ void attn_block(const AttnArgs& a, Rows rows_of, float* stat0, int* flags, int block, int blocks,
+                                           int head, int grp) {
   constexpr int CH = DP / 16, KI = DP / 32, VW = CH / 2;  // V dwords a lane holds of a key
-  extern __shared__ __align__(16) float lds[];  // [wave][R][DP + 4], [wave][R][2]
-  __shared__ int flags[WPB];  // 1: the wave left a part of a unit begun before it, 2: its last
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
   constexpr int ld = DP + 4;
-  float* const stat0 = lds + WPB * a.R * ld;
 
   Cursor cur;
   int n;  // this wave's tiles
   int per = 0;  // UNIT: tiles of a wave
   uint32_t c = 0, act = WPB;
   if constexpr (UNIT) {
-    cur.b = blockIdx.x;
-    cur.head = blockIdx.y;
-    cur.grp = blockIdx.z;
+    cur.b = block;
+    cur.head = head;
+    cur.grp = grp;
     cur.len = uniform(seq_len(a, cur.b));
     cur.nt = (cur.len + kTile - 1) / kTile;
     per = (cur.nt + WPB - 1) / WPB;
     cur.tile = min(wave * per, cur.nt);
     n = min(per, cur.nt - cur.tile);
   } else {
-    const Run r = run_of(a, blockIdx.x, wave, gridDim.x, WPB, lane);
+    const Run r = run_of(a, block, wave, blocks, WPB, lane);
     c = r.c;
     act = r.act;
     n = r.n;
     cur = r.at;
-    if (!PART && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (!PART && threadIdx.x == 0) a.desc[block] = make_int4(0, 0, 0, 0);
   }
   if (!UNIT && lane == 0) flags[wave] = 0;
 
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
       }
       acc.total();
       if constexpr (UNIT) {
-        acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, unit_rows(a, cur.grp), a.D, lane);
+        acc.put(rows_of(wave), ld, stat0 + wave * a.R * 2, unit_rows(a, cur.grp), a.D, lane);
         break;
       }
       const Cursor done = cur;
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
       if (begun && end) {
         unit_done<PART>(a, acc, done.b, done.head, done.grp, lane);
       } else if (!begun) {
-        acc.put(lds + wave * a.R * ld, ld, stat0 + wave * a.R * 2, unit_rows(a, done.grp), a.D, lane);
+        acc.put(rows_of(wave), ld, stat0 + wave * a.R * 2, unit_rows(a, done.grp), a.D, lane);
         if (lane == 0) flags[wave] = end ? 3 : 1;
       } else {
         tail = true;
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
         if (w < parts) {
           const float f = ex2(st[w].x - m);
           l = fmaf(f, st[w].y, l);
-          o += f * *reinterpret_cast<const floatx4*>(lds + (w * a.R + row) * ld + d);
+          o += f * *reinterpret_cast<const floatx4*>(rows_of(w) + row * ld + d);
         }
       if constexpr (PART) {
         const int64_t at = unit_row(a, cur.b, cur.head, cur.grp) + row;
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
   }
   // joins inside the block: a wave that began a unit takes what the waves after it left, the
   // first wave what they left of a unit begun in an earlier block
-  const int64_t slot = (int64_t)blockIdx.x * 2;
+  const int64_t slot = (int64_t)block * 2;
   int last;  // the last wave before the end of the unit that wave `from` - 1 goes on with, or of the block
   auto span = [&](int from) {
     for (last = from; last < (int)act - 1 && uniform(flags[last]) == 1; ++last) {
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     return uniform(flags[last]) == 3;
   };
   auto take = [&](int from) {
-    acc.take(lds + from * a.R * ld, a.R * ld, ld, stat0 + from * a.R * 2, a.R * 2, last + 1 - from, a.R, a.D, lane);
+    acc.take([&](int w) { return rows_of(from + w); }, ld, stat0 + from * a.R * 2, a.R * 2, last + 1 - from, a.R, a.D, lane);
   };
   if (tail) {
     const bool ended = wave + 1 < (int)act && span(wave + 1);
@@ -604,9 +604,9 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     } else {
       acc.put(a.part + (slot + 1) * a.R * a.D, a.D, a.stat + (slot + 1) * a.R * 2, a.R, a.D, lane);
       // the unit's last tile: this wave's last one is its tile cur.tile
-      const uint32_t end = (blockIdx.x * act + wave) * c + n - 1 - cur.tile + cur.nt - 1;
-      if constexpr (PART) unit_where(a, cur.b, cur.head, cur.grp, blockIdx.x, end / (c * act), lane);
-      else if (lane == 0) a.desc[blockIdx.x] = make_int4(cur.b, cur.head, end / (c * act), cur.grp + 1);
+      const uint32_t end = (block * act + wave) * c + n - 1 - cur.tile + cur.nt - 1;
+      if constexpr (PART) unit_where(a, cur.b, cur.head, cur.grp, block, end / (c * act), lane);
+      else if (lane == 0) a.desc[block] = make_int4(cur.b, cur.head, end / (c * act), cur.grp + 1);
     }
   }
   if (wave == 0 && uniform(flags[0]) != 0) {
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
     take(0);
     acc.put(a.part + slot * a.R * a.D, a.D, a.stat + slot * a.R * 2, a.R, a.D, lane);
   }
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x)  // sequences without keys
+  for (int b = block; b < a.B; b += blocks)  // sequences without keys
     if (uniform(seq_len(a, b)) == 0) {
       if constexpr (PART) {
         for (int i = threadIdx.x; i < a.Hkv * a.RG; i += WPB * 64)
@@ -625,6 +625,15 @@ __global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 :
           stg16(a.o + (int64_t)b * a.H * a.D + 8 * i, make_uint4(0, 0, 0, 0));
       }
     }
+}
+
+template <int DP, int RT, int WPB, bool PAD, bool UNIT>
+__global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 : 2) void paged_attn_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) float lds[];
+  __shared__ int flags[WPB];
+  attn_block<DP, RT, WPB, PAD, UNIT, false>(
+      a, [&](int w) { return lds + w * a.R * (DP + 4); }, lds + WPB * a.R * (DP + 4), flags, blockIdx.x, gridDim.x, blockIdx.y,
+      blockIdx.z);
 }
 
 // How a call is split: head dim DP, RT blocks of 16 rows a unit, wpb waves a block, blocks of
@@ -664,13 +673,13 @@ Div div_by(int64_t d) {  // 1 <= d < 2^31
   return Div{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), (uint32_t)(31 + l)};
 }
 
-template <int DP, int RT, int WPB, bool PART>
+template <int DP, int RT, int WPB>
 void launch_rows(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
   const dim3 grid = unit ? dim3((unsigned)a.B, (unsigned)a.Hkv, (unsigned)a.RG) : dim3((unsigned)blocks);
   const size_t lds = (size_t)WPB * a.R * (DP + 4 + 2) * 4;
   const bool pad = a.D != DP;
 #define ATTN(PAD_, UNIT_) \
-  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_, PART><<<grid, WPB * 64, lds, st>>>(a)
+  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_><<<grid, WPB * 64, lds, st>>>(a)
   if (unit) {
     if (pad) ATTN(true, true);
     else ATTN(false, true);
@@ -681,9 +690,8 @@ void launch_rows(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
 #undef ATTN
 }
 
-template <bool PART>
 void launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-#define ATTN(DP_, RT_, WPB_) launch_rows<DP_, RT_, WPB_, PART>(a, p.unit, p.blocks, st)
+#define ATTN(DP_, RT_, WPB_) launch_rows<DP_, RT_, WPB_>(a, p.unit, p.blocks, st)
   if (p.DP == 64) {
     if (p.RT == 1) ATTN(64, 1, 8);
     else if (p.RT == 2) ATTN(64, 2, 4);

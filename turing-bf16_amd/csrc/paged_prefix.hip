@@ -4,8 +4,11 @@
 // o = softmax of the logits of prefix keys and own keys together, times their values. Any split of the keys into
 // parts gives (m, l, o) with o = sum_j 2^(x_j - m) v_j and l = sum_j 2^(x_j - m), and parts join as
 //   m = max m_i,   l = sum l_i 2^(m_i - m),   o = sum o_i 2^(m_i - m).
-// Three launches: the prefix (prefix_kernel), the sequences' own keys (paged_attn_kernel of paged_attn.h, which
-// leaves sums instead of outputs), the join of all parts of a row (prefix_join_kernel).
+// Two launches: the prefix beside the sequences' own keys (prefix_kernel: blocks of either kind, the latter
+// attn_block of paged_attn.h, which leaves sums instead of outputs), and the join of all parts of a row.
+#include <cmath>
+#include <type_traits>
+
 #include "paged_attn.h"
 
 using namespace tbf16;
@@ -59,7 +62,9 @@ __device__ __forceinline__ int swz(int row) {
   else return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
 }
 
-constexpr int kIds = 4096;  // page ids a block holds at a time
+constexpr int kIds = 2048;  // page ids a block holds at a time
+// rows of a unit of own keys
+constexpr int own_rows(int DP) { return DP == 256 ? 8 : 16; }
 constexpr float kLag = 8.f;
 
 typedef __attribute__((address_space(1))) void global_void;
@@ -67,44 +72,67 @@ __device__ __forceinline__ void load16_lds(const void* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((global_void*)from, (lds_void*)to, 16, 0, 0);
 }
 
+// Which block of a launch does what: `own` blocks and `pre` blocks, eight of each in turn (one on every XCD)
+// as long as there are both, so that both kinds begin together.
+struct Mix {
+  int own, pre;
+};
+__device__ __forceinline__ bool mine(Mix m, int x, int& block) {  // whether x is an own block
+  const int both = min(m.own, m.pre) & ~7;
+  if (x < 2 * both) {
+    block = (x >> 4) * 8 + (x & 7);
+    return !(x & 8);
+  }
+  block = both + x - 2 * both;
+  if (block < m.own) return true;
+  block -= m.own - both;
+  return false;
+}
+
+struct LaunchArgs {
+  PrefixArgs pre;
+  AttnArgs own;
+  Mix mix;
+  bool unit;  // own blocks are units
+};
+
 template <int DP, int RB, int WR, int WK, int KB, int ST, bool PAD>
-__global__ __launch_bounds__(WR * WK * 64, 1) void prefix_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchArgs args) {
+  const PrefixArgs& a = args.pre;
   constexpr int NW = WR * WK, KS = 32 * KB * WK, CPR = DP / 8, RPI = 64 / CPR;  // chunks of a row, rows of a load
   constexpr int KPW = KS / RPI / NW;                                             // loads of K a wave does for a stage
   constexpr int KBYTES = KS * DP * 2, STAGE = 2 * KBYTES, KI = DP / 32, DB = DP / 16;
-  static_assert(KS % (RPI * NW) == 0 && ST >= 2 && ST <= 4 && (ST - 2) * 2 * KPW < 63, "stage shape");
+  static_assert(NW == 4 && KS % (RPI * NW) == 0 && ST >= 2 && ST <= 4 && (ST - 2) * 2 * KPW < 63, "stage shape");
   __shared__ __align__(1024) uint8_t st0[STAGE], st1[STAGE], st2[ST > 2 ? STAGE : 16], st3[ST > 3 ? STAGE : 16];
   __shared__ int s_ids[kIds];
   __shared__ float2 s_stat[NW][16 * RB];
+  __shared__ int s_flags[NW];
   uint8_t* const stages[4] = {st0, st1, st2, st3};
+  int block;
+  if (mine(args.mix, blockIdx.x, block)) {  // own keys
+    const AttnArgs& o = args.own;
+    static_assert(3 * own_rows(DP) * (DP + 4) * 4 <= STAGE, "three waves' rows fit a stage");
+    auto rows_of = [&](int w) {
+      return w < 3 ? reinterpret_cast<float*>(st0) + w * o.R * (DP + 4) : reinterpret_cast<float*>(st1);
+    };
+    if (args.unit) {
+      const int grp = block % o.RG, bh = block / o.RG, b = bh / o.Hkv;
+      attn_block<DP, 1, NW, PAD, true, true>(o, rows_of, &s_stat[0][0].x, s_flags, b, 0, bh - b * o.Hkv, grp);
+    } else {
+      attn_block<DP, 1, NW, PAD, false, true>(o, rows_of, &s_stat[0][0].x, s_flags, block, args.mix.own, 0, 0);
+    }
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
   const int wr = wave % WR, kg = wave / WR;
-  const int head = blockIdx.x % a.Hkv, split = blockIdx.x / a.Hkv % a.S, rt = blockIdx.x / a.Hkv / a.S;
+  const int head = block % a.Hkv, split = block / a.Hkv % a.S, rt = block / a.Hkv / a.S;
   const int length = prefix_len(a.length, a.cap);
   const Splits sp = splits_of(length, KS, a.S);
   const int t0 = split * sp.each, tn = min(sp.each, sp.tiles - t0);
   if (tn <= 0) return;
 
-  // the wave's rows
-  const int rows = a.B * a.G, row0 = (rt * WR + wr) * 16 * RB;
   const float c = fabsf(a.scale_log2);
-  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   bf16x8 qf[RB][KI];
-  int64_t out[RB];  // the lane's rows' place in the parts, -1: none
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int row = row0 + 16 * r + r16, b = min(row, rows - 1) / a.by_group, h = head * a.G + min(row, rows - 1) - b * a.G;
-    out[r] = row < rows ? ((int64_t)split * a.B + b) * a.H + h : -1;
-    const uint16_t* src = a.q + b * a.q_sb + h * a.q_sh;
-#pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      const int e = 8 * (g + 4 * i);
-      uint4 v = ldg16(src + (!PAD || e < a.D ? e : 0));
-      if (PAD && e >= a.D) v = make_uint4(0, 0, 0, 0);
-      qf[r][i] = __builtin_bit_cast(bf16x8, make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
-    }
-  }
-
   floatx4 o[RB][DB];
   float m[RB], l[RB];  // m: what the weights refer to
   bool fresh = true;
@@ -117,26 +145,29 @@ __global__ __launch_bounds__(WR * WK * 64, 1) void prefix_kernel(PrefixArgs a) {
   }
 
   const uint16_t *kc = a.kc + head * a.kg.sh, *vc = a.vc + head * a.vg.sh;
-  int id0 = 0;  // the first page whose id s_ids holds
-  // id of the page of position pos, -1 past the prefix's end
-  auto page_of = [&](int pos, int& row) {
-    const uint32_t at = min(pos, length - 1), idx = at / a.by_page;
-    row = (int)(at - idx * a.page);
-    const int id = s_ids[(int)idx - id0];
-    return pos < length && (uint32_t)id < a.pages ? id : -1;
+  int id0 = 0, last = 0;  // the first page whose id s_ids holds, the last position it covers
+  bool named = true;      // all of these ids name pages
+  // page id and row of position pos, or of the last one
+  auto page_of = [&](int pos, uint32_t& row) {
+    const uint32_t at = min(pos, last), idx = at / a.by_page;
+    row = at - idx * a.page;
+    return (uint32_t)s_ids[(int)idx - id0];
   };
+  // (a wave's loads are rows 16 apart and more, or their chunk is another: see swz)
   const int lrow = lane / CPR, lchunk = lane % CPR;
+  const uint32_t k_sp = 2 * (uint32_t)a.kg.sp, k_ss = 2 * (uint32_t)a.kg.ss, v_sp = 2 * (uint32_t)a.vg.sp, v_ss = 2 * (uint32_t)a.vg.ss;
+  // Rows of keys that are not there are some row that is: `masked` leaves them out.
   auto issue = [&](uint8_t* stage, int tile) {
 #pragma unroll
     for (int j = 0; j < KPW; ++j) {
-      const int n = wave * KPW + j, krow = n * RPI + lrow, chunk = lchunk ^ swz<DP>(krow);
-      int row;
-      const int id = page_of(tile * KS + krow, row);
-      const bool there = id >= 0 && (!PAD || chunk * 8 < a.D);
-      const uint16_t* k = kc + (int64_t)id * a.kg.sp + (int64_t)row * a.kg.ss + chunk * 8;
-      const uint16_t* v = vc + (int64_t)id * a.vg.sp + (int64_t)row * a.vg.ss + chunk * 8;
-      load16_lds(there ? (const void*)k : &kZeros, stage + n * 1024);
-      load16_lds(there ? (const void*)v : &kZeros, stage + KBYTES + n * 1024);
+      const int n = wave + NW * j, krow = n * RPI + lrow, chunk = lchunk ^ swz<DP>(krow);
+      uint32_t row, id = page_of(tile * KS + krow, row);
+      if (!named) id = id < a.pages ? id : 0;
+      uint64_t k = (uint64_t)row * k_ss + ((uint64_t)id * k_sp + (uint64_t)(kc + chunk * 8));
+      uint64_t v = (uint64_t)row * v_ss + ((uint64_t)id * v_sp + (uint64_t)(vc + chunk * 8));
+      if (PAD && chunk * 8 >= a.D) k = v = (uint64_t)&kZeros;
+      load16_lds(reinterpret_cast<const void*>(k), stage + n * 1024);
+      load16_lds(reinterpret_cast<const void*>(v), stage + KBYTES + n * 1024);
     }
   };
 
@@ -147,46 +178,31 @@ __global__ __launch_bounds__(WR * WK * 64, 1) void prefix_kernel(PrefixArgs a) {
   typedef short v4s __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-  auto compute = [&](const uint8_t* stage, int tile) {
-    int unused;
-    const int key = lane & (32 * KB - 1);
-    uint64_t live = __ballot(page_of(tile * KS + kg * 32 * KB + key, unused) >= 0);
-    if constexpr (KB == 1) live &= 0xffffffffu;
-    if (live == 0) return;
-    const bool whole = live == (KB == 1 ? 0xffffffffull : ~0ull);
-    floatx4 s[2 * KB][RB];
+  typedef floatx4 Logits[2][RB];
+  typedef bf16x8 Weights[RB][2];
+  // 32 keys at a time: logits, ...
+  auto logits = [&](const uint8_t* stage, int kl, int h, Logits& s) {
 #pragma unroll
-    for (int k = 0; k < 2 * KB; ++k)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int r = 0; r < RB; ++r) s[k][r] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < KI; ++t)
 #pragma unroll
-      for (int k = 0; k < 2 * KB; ++k) {
-        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(stage + (klane ^ (t << 6)) + k * 16 * DP * 2);
+      for (int k = 0; k < 2; ++k) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(stage + (kl ^ (t << 6)) + (2 * h + k) * 16 * DP * 2);
 #pragma unroll
         for (int r = 0; r < RB; ++r) s[k][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[r][t], s[k][r], 0, 0, 0);
       }
-    float cc = c;
-    if (!whole) {
-      cc = 1.f;
-#pragma unroll
-      for (int k = 0; k < 2 * KB; ++k)
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[k][r][i] = live >> (16 * k + 4 * g + i) & 1 ? s[k][r][i] * c : -INFINITY;
-    }
+  };
+  // ... what the weights refer to, ...
+  auto follow = [&](const Logits& s, float cc) {
     float mx[RB];
     bool grown = fresh;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      mx[r] = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < 2 * KB; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[r] = fmaxf(mx[r], s[k][r][i]);
-      mx[r] *= cc;
+      mx[r] = fmaxf(fmaxf(fmaxf(fmaxf(s[0][r][0], s[0][r][1]), fmaxf(s[0][r][2], s[0][r][3])), fmaxf(s[1][r][0], s[1][r][1])),
+                    fmaxf(s[1][r][2], s[1][r][3])) * cc;
       grown |= mx[r] > m[r] + kLag;
     }
     if (__any(grown)) {
@@ -204,69 +220,160 @@ __global__ __launch_bounds__(WR * WK * 64, 1) void prefix_kernel(PrefixArgs a) {
         for (int d = 0; d < DB; ++d) o[r][d] *= f;
       }
     }
+  };
+  // ... weights, ...
+  auto weights = [&](const Logits& s, float cc, Weights& pf) {
 #pragma unroll
-    for (int h = 0; h < KB; ++h) {  // 32 keys
-      bf16x8 pf[RB][2];
+    for (int r = 0; r < RB; ++r) {
+      const float mo = m[r] + 2 * kLag;
+      uint32_t f[2][4];
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const float mo = m[r] + 2 * kLag;
-        uint32_t f[2][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const floatx4& sv = s[2 * h + (j >> 1)][r];
-          const float p0 = ex2(fmaf(sv[2 * (j & 1)], cc, -mo)), p1 = ex2(fmaf(sv[2 * (j & 1) + 1], cc, -mo));
-          l[r] += p0 + p1;
-          f[0][j] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
-          f[1][j] = pack_bf16(p0 - bf16_hi(__float_as_uint(p0)), p1 - bf16_hi(__float_as_uint(p1)));
-          // 2^-28 of p in place of a part that is zero: an infinite value times it stays infinite
-          const ushort2v least = __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, f[0][j]), ushort2v{28 << 7, 28 << 7});
-          f[1][j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, f[1][j]), least));
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));
+      for (int j = 0; j < 4; ++j) {
+        const floatx4& sv = s[j >> 1][r];
+        const float p0 = ex2(fmaf(sv[2 * (j & 1)], cc, -mo)), p1 = ex2(fmaf(sv[2 * (j & 1) + 1], cc, -mo));
+        l[r] += p0 + p1;
+        f[0][j] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
+        // the rest, and 2^-22 of p so that it is never zero: an infinite value times it stays infinite
+        f[1][j] = pack_bf16(fmaf(p0, 0x1.000004p0f, -bf16_hi(__float_as_uint(p0))),
+                            fmaf(p1, 0x1.000004p0f, -bf16_hi(__float_as_uint(p1))));
       }
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const uint8_t* at = stage + (vlane ^ (d << 5)) + h * 32 * DP * 2;
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 16 * DP * 2));
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int t = 0; t < 2; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));
+    }
+  };
+  // ... and outputs; live: the keys that there are
+  auto values = [&](const uint8_t* stage, int vl, int h, const Weights& pf, auto all, uint32_t live) {
+    uint4 keep;  // the lane's 8 keys of the 32
+    if constexpr (!decltype(all)::value) {
+      auto two = [&](int k) { return (live >> k & 1 ? 0xffffu : 0u) | (live >> (k + 1) & 1 ? 0xffff0000u : 0u); };
+      keep = make_uint4(two(4 * g), two(4 * g + 2), two(16 + 4 * g), two(18 + 4 * g));
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint8_t* at = stage + (vl ^ (d << 5)) + h * 32 * DP * 2;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 16 * DP * 2));
+      uint4 v = __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      // (a weight of zero times whatever lies there has to be zero)
+      if constexpr (!decltype(all)::value) v = make_uint4(v.x & keep.x, v.y & keep.y, v.z & keep.z, v.w & keep.w);
+      const bf16x8 vf = __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][t], o[r][d], 0, 0, 0);
+    }
+  };
+  // A whole tile, from a stage that the next loads must not go into yet. (They go out behind the first reads: where
+  // the compiler cannot tell the stages apart it waits for all loads before a read, which by then are those of
+  // earlier steps.)
+  auto whole = [&](const uint8_t* stage, uint8_t* next, int next_tile) {
+    // (opaque, or every stage's addresses are kept in registers of their own)
+    int kl = klane, vl = vlane;
+    asm volatile("" : "+v"(kl), "+v"(vl));
+    Logits s[2];
+    Weights pf;
+    logits(stage, kl, 0, s[0]);
+    issue(next, next_tile);
+    follow(s[0], c);
+#pragma unroll
+    for (int h = 0; h < KB; ++h) {
+      if (h + 1 < KB) logits(stage, kl, h + 1, s[(h + 1) & 1]);
+      weights(s[h & 1], c, pf);
+      values(stage, vl, h, pf, std::true_type(), 0u);
+      if (h + 1 < KB) follow(s[(h + 1) & 1], c);
+    }
+  };
+  auto masked = [&](const uint8_t* stage, int tile) {
+    for (int h = 0; h < KB; ++h) {
+      const int pos = tile * KS + (kg * KB + h) * 32 + (lane & 31);
+      uint32_t row;
+      const bool there = page_of(pos, row) < a.pages && pos <= last;
+      const uint32_t live = (uint32_t)__ballot(there);
+      if (live == 0) continue;
+      Logits s;
+      Weights pf;
+      logits(stage, klane, h, s);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][t], o[r][d], 0, 0, 0);
-      }
+          for (int i = 0; i < 4; ++i) s[k][r][i] = live >> (16 * k + 4 * g + i) & 1 ? s[k][r][i] * c : -INFINITY;
+      follow(s, 1.f);
+      weights(s, 1.f, pf);
+      values(stage, vlane, h, pf, std::false_type(), live);
     }
   };
 
-  // as many tiles at a time as s_ids covers
+  // as many tiles at a time as s_ids covers: the ids, the first loads
   const int most = (int)min((int64_t)tn, max((int64_t)1, (int64_t)(kIds - 2) * a.page / KS));
-  for (int done = 0; done < tn; done += most) {
-    const int first = t0 + done, n = min(most, tn - done);
-    const int from = first * KS, last = min(from + n * KS, length) - 1;
-    __syncthreads();  // nobody reads the ids or stages of the tiles before
+  auto begin = [&](int done) {
+    const int from = (t0 + done) * KS;
+    last = min(from + min(most, tn - done) * KS, length) - 1;
     id0 = (int)((uint32_t)from / a.by_page);
     const int ids = (int)((uint32_t)last / a.by_page) - id0 + 1;
-    for (int i = threadIdx.x; i < ids; i += NW * 64) s_ids[i] = a.table[id0 + i];
-    __syncthreads();
+    int bad = 0;
+    for (int i = threadIdx.x; i < ids; i += NW * 64) {
+      const int id = a.table[id0 + i];
+      s_ids[i] = id;
+      bad |= (uint32_t)id >= a.pages;
+    }
+    named = __syncthreads_or(bad) == 0;
+    // (tiles past the last one load its last row: as many loads in every step, so that it is known without a
+    // branch which have come)
 #pragma unroll
-    for (int u = 0; u < ST - 1; ++u)
-      if (u < n) issue(stages[u], first + u);
-    for (int i0 = 0; i0 < n; i0 += ST) {
+    for (int u = 0; u < ST - 1; ++u) issue(stages[u], t0 + done + u);
+  };
+  begin(0);
+  // the wave's rows
+  const int rows = a.B * a.G, row0 = (rt * WR + wr) * 16 * RB;
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a maximum is looked for: the sign goes to q)
+  int64_t out[RB];  // the lane's rows' place in the parts, -1: none
 #pragma unroll
-      for (int u = 0; u < ST; ++u) {
-        const int i = i0 + u;
-        if (i >= n) break;
-        // stage u is there once only the later stages' loads are on their way
-        if (i + ST - 2 < n) wait_vmem_n<(ST - 2) * 2 * KPW>();
-        else wait_vmem_n<0>();
-        wait_lds();
-        barrier_no_fence();
-        if (i + ST - 1 < n) issue(stages[(u + ST - 1) % ST], first + i + ST - 1);
-        compute(stages[u], first + i);
-      }
+  for (int r = 0; r < RB; ++r) {
+    const int row = row0 + 16 * r + r16, b = min(row, rows - 1) / a.by_group, h = head * a.G + min(row, rows - 1) - b * a.G;
+    out[r] = row < rows ? ((int64_t)split * a.B + b) * a.H + h : -1;
+    const uint16_t* src = a.q + b * a.q_sb + h * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int e = 8 * (g + 4 * i);
+      uint4 v = ldg16(src + (!PAD || e < a.D ? e : 0));
+      if (PAD && e >= a.D) v = make_uint4(0, 0, 0, 0);
+      qf[r][i] = __builtin_bit_cast(bf16x8, make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
     }
   }
+
+  for (int done = 0; done < tn; done += most) {
+    const int first = t0 + done, n = min(most, tn - done);
+    const int full = named ? (last + 1 - first * KS) / KS : 0;  // whole tiles, in the ring; a last one, or all, on their own
+    for (int i0 = 0; i0 < full; i0 += ST) {
+#pragma unroll
+      for (int u = 0; u < ST; ++u) {
+        if (i0 + u >= full) break;
+        wait_vmem_n<(ST - 2) * 2 * KPW>();  // stage u is there once only the later stages' loads are on their way
+        wait_lds();
+        barrier_no_fence();
+        whole(stages[u], stages[(u + ST - 1) % ST], first + i0 + u + ST - 1);
+      }
+    }
+    for (int i = full; i < n; ++i) {
+      const int u = named ? i % ST : 0;
+      if (!named) {
+        wait_vmem_n<0>();
+        __syncthreads();
+        issue(st0, first + i);
+      }
+      wait_vmem_n<0>();
+      __syncthreads();
+      masked(u == 0 ? st0 : u == 1 ? st1 : u == 2 ? st2 : st3, first + i);
+    }
+    if (done + most < tn) {
+      wait_vmem_n<0>();
+      __syncthreads();  // nobody reads the ids or stages any more, or loads into them
+      begin(done + most);
+    }
+  }
+  wait_vmem_n<0>();
 
 #pragma unroll
   for (int r = 0; r < RB; ++r) l[r] = sum_xor32(sum_xor16(l[r]));
@@ -407,59 +514,62 @@ __global__ __launch_bounds__(kMeet * 64) void prefix_join_kernel(JoinArgs j) {
 
 // ---- host -------------------------------------------------------------------------------
 
-// How a call is split: rows of a block and keys of a tile by the form, splits of the prefix.
+// How a call is split: rows of a block and keys of a tile by the form, splits of the prefix, own keys.
 struct PrefixPlan {
-  int DP, form, rows, keys;
+  int DP, few, rows, keys;
   int64_t tiles, S;  // row tiles of a key/value head, splits
   AttnPlan own;
   size_t part, stat, own_part, own_stat, where, bytes;
 };
 PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_cap, int64_t cap) {
   PrefixPlan p;
-  const int64_t n = B * (H / Hkv);
+  const int64_t G = H / Hkv, n = B * G;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  if (p.DP == 256) {
-    p.form = n <= 32 ? 2 : n <= 64 ? 1 : 0;
-    p.rows = p.form == 2 ? 32 : p.form == 1 ? 64 : 128;
-    p.keys = 64;
-  } else {
-    p.form = n <= 32 ? 3 : n <= 64 ? 2 : n <= 128 ? 1 : 0;
-    p.rows = 256 >> p.form;
-    p.keys = p.form >= 2 ? 128 : 64;
-  }
+  p.few = p.DP < 256 && n <= 64;
+  p.rows = p.DP == 256 || p.few ? 64 : 128;
+  p.keys = p.DP == 256 ? 32 : 64;
   p.tiles = cdiv(n, p.rows);
-  p.S = std::min(cdiv(prefix_cap, p.keys), std::max<int64_t>(1, num_cus() / (Hkv * p.tiles)));
-  p.own = attn_plan(B, H, Hkv, D, cap);
-  p.part = align_up(p.own.bytes, 256);
+  // Splits: two blocks a CU, but no more than pays for the parts they leave: a tile takes ~ 2.5 us, a split's
+  // part of all rows 8 bytes an element, written and read at 4 TB/s.
+  const int64_t all = cdiv(prefix_cap, p.keys);
+  const double part_us = (double)(B * H * D) * 8 / 4e6;
+  const int64_t most = std::max<int64_t>(1, (int64_t)std::sqrt(2.5 * (double)all / part_us));
+  p.S = std::min({all, most, std::max<int64_t>(1, 2 * num_cus() / (Hkv * p.tiles))});
+
+  AttnPlan& o = p.own;
+  o.DP = p.DP;
+  o.RT = 1;
+  o.wpb = 4;
+  o.R = (int)std::min<int64_t>(G, own_rows(p.DP));
+  o.RG = (int)cdiv(G, o.R);
+  o.unit = cdiv(cap, kTile) <= 4 * o.wpb && B * Hkv * o.RG <= num_cus();
+  o.blocks = o.unit ? B * Hkv * o.RG : num_cus();
+  o.stat = align_up((size_t)o.blocks * 2 * o.R * (size_t)D * 4, 256);
+  o.desc = o.bytes = o.unit ? 0 : o.stat + align_up((size_t)o.blocks * 2 * o.R * 2 * 4, 256);
+  p.part = o.bytes;
   p.stat = p.part + align_up((size_t)(p.S * B * H * D) * 4, 256);
   p.own_part = p.stat + align_up((size_t)(p.S * B * H) * 8, 256);
   p.own_stat = p.own_part + align_up((size_t)(B * H * D) * 4, 256);
   p.where = p.own_stat + align_up((size_t)(B * H) * 8, 256);
-  p.bytes = p.where + align_up((size_t)(B * Hkv * p.own.RG) * 8, 256);
+  p.bytes = p.where + align_up((size_t)(B * Hkv * o.RG) * 8, 256);
   return p;
 }
 
 template <int DP, int RB, int WR, int WK, int KB, int ST>
-void launch_form(const PrefixArgs& a, const PrefixPlan& p, hipStream_t st) {
-  const unsigned grid = (unsigned)(a.Hkv * p.S * p.tiles);
-  if (a.D == DP) prefix_kernel<DP, RB, WR, WK, KB, ST, false><<<grid, WR * WK * 64, 0, st>>>(a);
-  else prefix_kernel<DP, RB, WR, WK, KB, ST, true><<<grid, WR * WK * 64, 0, st>>>(a);
+void launch_form(const LaunchArgs& a, hipStream_t st) {
+  const unsigned grid = (unsigned)(a.mix.own + a.mix.pre);
+  if (a.pre.D == DP) prefix_kernel<DP, RB, WR, WK, KB, ST, false><<<grid, 256, 0, st>>>(a);
+  else prefix_kernel<DP, RB, WR, WK, KB, ST, true><<<grid, 256, 0, st>>>(a);
 }
-void launch_prefix(const PrefixArgs& a, const PrefixPlan& p, hipStream_t st) {
+void launch_prefix(const LaunchArgs& a, const PrefixPlan& p, hipStream_t st) {
   if (p.DP == 64) {
-    if (p.form == 0) launch_form<64, 2, 8, 1, 2, 4>(a, p, st);
-    else if (p.form == 1) launch_form<64, 2, 4, 2, 1, 4>(a, p, st);
-    else if (p.form == 2) launch_form<64, 2, 2, 4, 1, 4>(a, p, st);
-    else launch_form<64, 2, 1, 4, 1, 4>(a, p, st);
+    if (p.few) launch_form<64, 2, 2, 2, 1, 4>(a, st);
+    else launch_form<64, 2, 4, 1, 2, 4>(a, st);
   } else if (p.DP == 128) {
-    if (p.form == 0) launch_form<128, 2, 8, 1, 2, 4>(a, p, st);
-    else if (p.form == 1) launch_form<128, 2, 4, 2, 1, 4>(a, p, st);
-    else if (p.form == 2) launch_form<128, 2, 2, 4, 1, 2>(a, p, st);
-    else launch_form<128, 2, 1, 4, 1, 2>(a, p, st);
+    if (p.few) launch_form<128, 2, 2, 2, 1, 2>(a, st);
+    else launch_form<128, 2, 4, 1, 2, 2>(a, st);
   } else {
-    if (p.form == 0) launch_form<256, 1, 8, 1, 2, 2>(a, p, st);
-    else if (p.form == 1) launch_form<256, 1, 4, 2, 1, 2>(a, p, st);
-    else launch_form<256, 1, 2, 2, 1, 2>(a, p, st);
+    launch_form<256, 1, 4, 1, 1, 2>(a, st);
   }
 }
 
@@ -500,7 +610,7 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
   const int64_t pcap = pages == 0 ? 0 : std::min<int64_t>(prefix_pages * page, top);
   // (the plan goes by what the workspace query was asked for, whatever the cache holds)
   const PrefixPlan p = prefix_plan(B, H, Hkv, D, prefix_pages * page, max_pages * page);
-  TB_CHECK(B * Hkv * p.own.RG < (int64_t)1 << 31 && Hkv * p.S * p.tiles < (int64_t)1 << 31 &&
+  TB_CHECK(B * Hkv * p.own.RG < (int64_t)1 << 31 && Hkv * p.S * p.tiles + p.own.blocks < (int64_t)1 << 31 &&
                (double)(B * Hkv * p.own.RG) * (double)cdiv(std::min<int64_t>(max_pages * page, (int64_t)1 << 31), kTile) < 2e9,
            "paged_attn_prefix: shape too large");
   TB_CHECK(aligned16(ws) && ws != nullptr, "paged_attn_prefix: workspace missing or misaligned");
@@ -509,13 +619,14 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
     return TBF16_EWS;
   }
   uint8_t* const w = (uint8_t*)ws;
-  JoinArgs j;
-  j.own = attn_args(p.own, q, B, H, Hkv, D, q_sb, q_sh, k_cache, v_cache, pages, page, kg, vg, table, table_stride, max_pages,
-                    lengths, scale, o, ws);
-  j.own.own = (float*)(w + p.own_part);
-  j.own.own_stat = (float*)(w + p.own_stat);
-  j.own.where = (int2*)(w + p.where);
-  PrefixArgs& a = j.pre;
+  LaunchArgs la;
+  la.own = attn_args(p.own, q, B, H, Hkv, D, q_sb, q_sh, k_cache, v_cache, pages, page, kg, vg, table, table_stride, max_pages,
+                     lengths, scale, o, ws);
+  la.own.own = (float*)(w + p.own_part);
+  la.own.own_stat = (float*)(w + p.own_stat);
+  la.own.where = (int2*)(w + p.where);
+  la.unit = p.own.unit;
+  PrefixArgs& a = la.pre;
   a.q = (const uint16_t*)q;
   a.kc = (const uint16_t*)k_cache;
   a.vc = (const uint16_t*)v_cache;
@@ -531,7 +642,7 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
   a.page = (uint32_t)page;
   a.by_page = div_by(page);
   a.by_group = div_by(H / Hkv);
-  a.scale_log2 = j.own.scale_log2;
+  a.scale_log2 = la.own.scale_log2;
   a.B = (int)B;
   a.H = (int)H;
   a.Hkv = (int)Hkv;
@@ -539,17 +650,11 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
   a.D = (int)D;
   a.part = (float*)(w + p.part);
   a.stat = (float*)(w + p.stat);
-  j.keys = p.keys;
-  j.unit = p.own.unit;
-  j.blocks = (int)p.own.blocks;
-  j.o = (uint16_t*)o;
+  la.mix = {(int)p.own.blocks, (int)(Hkv * a.S * p.tiles)};
+  JoinArgs j{la.own, la.pre, p.keys, p.own.unit, (int)p.own.blocks, (uint16_t*)o};
   const hipStream_t st = as_stream(stream);
-  if (a.S > 0) {
-    launch_prefix(a, p, st);
-    TB_LAUNCH_CHECK("paged_attn_prefix");
-  }
-  launch_attn<true>(j.own, p.own, st);
-  TB_LAUNCH_CHECK("paged_attn_prefix own keys");
+  launch_prefix(la, p, st);
+  TB_LAUNCH_CHECK("paged_attn_prefix");
   prefix_join_kernel<<<(unsigned)cdiv(B * H * (D / 4), 64), kMeet * 64, 0, st>>>(j);
   TB_LAUNCH_CHECK("paged_attn_prefix join");
   return 0;

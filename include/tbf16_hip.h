@@ -334,7 +334,7 @@ int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int64_t Hkv, in
 /* RMS norm of each query and key head and rotation by position: with u = x / sqrt(mean x^2 + eps) and
  * z = u w, the first R elements of z are rotated in pairs (i, i + R / 2), or (2 i, 2 i + 1) with
  * interleaved != 0, by cos[pos][i], sin[pos][i]; the others stay. One rounding to bf16. q, k bf16 (B, S,
- * H or Hkv, D), element strides (b, s, h) in q_st, k_st, D contiguous and a multiple of 16 up to
+ * H or Hkv, D), element strides (b, s, h), D contiguous and a multiple of 16 up to
  * 256, everything 16-byte aligned; wq, wk (D,) bf16, or fp32 with w_f32 != 0; cos, sin fp32 (rows, R / 2)
  * contiguous, R a multiple of 16; pos int32 (B, S), element strides p_sb, p_ss. Tokens of negative
  * position give zeros, of positions from `rows` on NaN. yq, yk bf16 contiguous.
@@ -343,16 +343,18 @@ int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int64_t Hkv, in
  * tbf16_qk_norm_rope_bwd_ws_bytes(B, S, D) bytes (asked with the stream's device current), this call's
  * alone until it has run; not used without dwq and dwk. No counterpart in the reference. */
 int tbf16_qk_norm_rope(const void* q, const void* k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D,
-                       const int64_t* q_st, const int64_t* k_st, const void* wq, const void* wk, int w_f32,
-                       const float* cos, const float* sin, int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb,
-                       int64_t p_ss, float eps, int interleaved, void* yq, void* yk, void* stream);
+                       int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* wq,
+                       const void* wk, int w_f32, const float* cos, const float* sin, int64_t rows, int64_t R,
+                       const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps, int interleaved, void* yq, void* yk,
+                       void* stream);
 size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t D);
 int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, int64_t B, int64_t S, int64_t H,
-                           int64_t Hkv, int64_t D, const int64_t* q_st, const int64_t* k_st, const int64_t* dyq_st,
-                           const int64_t* dyk_st, const void* wq, const void* wk, int w_f32, const float* cos,
-                           const float* sin, int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb, int64_t p_ss,
-                           float eps, int interleaved, void* dq, void* dk, void* dwq, void* dwk, void* ws,
-                           int64_t ws_bytes, void* stream);
+                           int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t k_sb, int64_t k_ss,
+                           int64_t k_sh, int64_t dyq_sb, int64_t dyq_ss, int64_t dyq_sh, int64_t dyk_sb, int64_t dyk_ss,
+                           int64_t dyk_sh, const void* wq, const void* wk, int w_f32, const float* cos, const float* sin,
+                           int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps,
+                           int interleaved, void* dq, void* dk, void* dwq, void* dwk, void* ws, int64_t ws_bytes,
+                           void* stream);
 
 /* A paged cache's bookkeeping: sequences get counts[b] tokens longer, or -counts[b] shorter. table
  * int32 (B, max_pages), row stride table_stride; lengths, counts int32 (B,); free_pages int32
@@ -365,9 +367,10 @@ int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const 
  * tokens begin, at most tokens. slots, positions int32 (tokens,): page id * page + row, old length +
  * i + *prefix (0 if NULL), or -1 both for tokens that were not granted or are not there; a slot is -1
  * too where the table names no page. B * max_pages and pages * page below 2^31. No two arrays
- * overlap. ws: tbf16_paged_advance_ws_bytes(B) bytes, this call's alone until it has run. No
+ * overlap. ws: tbf16_paged_advance_ws_bytes(B, tokens) bytes, this call's alone until it has run (0 for
+ * small batches, ws may then be NULL). No
  * counterpart in the reference. */
-size_t tbf16_paged_advance_ws_bytes(int64_t B);
+size_t tbf16_paged_advance_ws_bytes(int64_t B, int64_t tokens);
 int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t B, int64_t max_pages, int32_t* lengths,
                         const int32_t* counts, int32_t* free_pages, int64_t pages, int32_t* n_free, int64_t page,
                         int64_t tokens, const int32_t* prefix, int32_t* slots, int32_t* positions, int32_t* starts,

@@ -31,14 +31,14 @@ packed = torch.zeros(100, dtype=I32)
     (dict(page_table=torch.zeros(4, 3, dtype=I32).t()), ValueError, "rows must be"),
     (dict(page_table=torch.zeros(1, 4, dtype=I32).expand(3, 4)), ValueError, "rows must be"),
     (dict(lengths=torch.zeros(2, dtype=I32)), ValueError, "for 3 sequences"),
-    (dict(lengths=torch.zeros(3, dtype=torch.int64)), TypeError, "lengths as int32"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int64)), TypeError, "expected int32"),
     (dict(lengths=torch.zeros(6, dtype=I32)[::2]), ValueError, "contiguous"),
-    (dict(counts=torch.zeros(3, 1, dtype=I32)), ValueError, "for 3 sequences"),
+    (dict(counts=torch.zeros(3, 1, dtype=I32)), ValueError, "one dimension"),
     (dict(counts=torch.zeros(1, dtype=I32).expand(3)), ValueError, "contiguous"),
-    (dict(free_pages=torch.zeros(4, 5, dtype=I32)), ValueError, "free_pages"),
+    (dict(free_pages=torch.zeros(4, 5, dtype=I32)), ValueError, "one dimension"),
     (dict(n_free=torch.zeros(2, dtype=I32)), ValueError, "one number"),
     (dict(prefix_length=torch.zeros(0, dtype=I32)), ValueError, "one number"),
-    (dict(prefix_length=torch.zeros(1)), TypeError, "prefix_length as int32"),
+    (dict(prefix_length=torch.zeros(1)), TypeError, "expected int32"),
     (dict(lengths=packed[:3], counts=packed[:3]), ValueError, "same memory"),
     (dict(free_pages=packed[:20], n_free=packed[19:20]), ValueError, "same memory"),
     (dict(page=0), ValueError, "positions"),
@@ -76,11 +76,13 @@ def test_advance_abi_refusals():
     for bad, text in [(dict(B=-1), "table shape"), (dict(n=2 ** 31), "table shape"), (dict(n=2 ** 30), "table shape"),
                       (dict(st=3), "overlap"), (dict(page=0), "slots"), (dict(pages=2 ** 28), "slots"),
                       (dict(tokens=-1), "tokens"), (dict(tokens=2 ** 31), "tokens"), (dict(nf=None), "missing"),
-                      (dict(starts=None), "missing"), (dict(ws=None), "missing"), (dict(table=18), "misaligned")]:
+                      (dict(starts=None), "missing"), (dict(table=18), "misaligned"), (dict(ws=18), "misaligned")]:
         assert call(**bad) == -1, bad
         assert text in err(), (bad, err())
-    assert call(wsb=0) == -3 and "workspace" in err()
-    assert L.tbf16_paged_advance_ws_bytes(100) >= 1200
+    for bad in (dict(tokens=10 ** 5, wsb=0), dict(tokens=10 ** 5, ws=None), dict(B=5000, wsb=10 ** 4)):
+        assert call(**bad) == -3 and "workspace" in err(), bad
+    size = L.tbf16_paged_advance_ws_bytes
+    assert size(100, 100) == 0 < size(100, 10 ** 5) < size(10 ** 4, 0) and size(0, 10 ** 5) > 0
 
 
 def test_advance_by_hand():
@@ -143,25 +145,24 @@ def test_norm_rope_tables_have_no_gradient():
 
 
 def test_norm_rope_abi_refusals():
-    import ctypes
     L = _ext.lib()
     err = lambda: L.tbf16_last_error().decode()  # noqa: E731
-    st = lambda *v: (ctypes.c_int64 * 3)(*v)  # noqa: E731
+    st = 0, 64, 64
 
     def tail(rows=9, R=32, eps=1e-6, cos=16):
         return 16, 16, 0, cos, 16, rows, R, 16, 0, 1, eps, 0
 
-    def fwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st(0, 64, 64), **kw):
-        return L.tbf16_qk_norm_rope(q, 16, B, S, H, Hkv, D, q_st, st(0, 64, 64), *tail(**kw), 16, 16, None)
+    def fwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st, **kw):
+        return L.tbf16_qk_norm_rope(q, 16, B, S, H, Hkv, D, *q_st, *st, *tail(**kw), 16, 16, None)
 
-    def bwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st(0, 64, 64), ws=16, wsb=0, dwq=16, **kw):
-        return L.tbf16_qk_norm_rope_bwd(q, 16, 16, 16, B, S, H, Hkv, D, q_st, st(0, 64, 64), st(0, 64, 64), st(0, 64, 64),
-                                        *tail(**kw), None, None, dwq, None, ws, wsb, None)
+    def bwd(B=1, S=2, H=4, Hkv=2, D=64, q=16, q_st=st, ws=16, wsb=0, dwq=16, **kw):
+        return L.tbf16_qk_norm_rope_bwd(q, 16, 16, 16, B, S, H, Hkv, D, *q_st, *st, *st, *st, *tail(**kw), None, None, dwq, None,
+                                        ws, wsb, None)
 
     for bad, text in [(dict(B=-1), "tokens"), (dict(S=2 ** 31), "tokens"), (dict(H=0), "heads"), (dict(D=24), "head dim"),
                       (dict(D=272), "head dim"), (dict(R=8), "rotated"), (dict(R=0), "rotated"), (dict(R=80), "rotated"),
                       (dict(rows=0), "tables"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
-                      (dict(q=24), "aligned"), (dict(q_st=st(0, 64, 4)), "aligned"), (dict(cos=8), "misaligned")]:
+                      (dict(q=24), "aligned"), (dict(q_st=(0, 64, 4)), "aligned"), (dict(cos=8), "misaligned")]:
         assert fwd(**bad) == -1 and text in err(), (bad, err())
         assert bwd(**bad) == -1 and text in err(), (bad, err())
     assert bwd() == -3 and "workspace" in err()

@@ -319,12 +319,12 @@ int check_norm(const char* fn, const NormArgs& a, int64_t B, int64_t S, int64_t 
   return 0;
 }
 
-NormArgs norm_args(const void* q, const void* k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D,
-                   const int64_t* q_st, const int64_t* k_st, const void* wq, const void* wk, const float* cos,
-                   const float* sin, int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps) {
+NormArgs norm_args(const Heads& q, const Heads& k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, const void* wq,
+                   const void* wk, const float* cos, const float* sin, int64_t rows, int64_t R, const int32_t* pos,
+                   int64_t p_sb, int64_t p_ss, float eps) {
   NormArgs a = {};
-  a.q = {(const uint16_t*)q, q_st[0], q_st[1], q_st[2]};
-  a.k = {(const uint16_t*)k, k_st[0], k_st[1], k_st[2]};
+  a.q = q;
+  a.k = k;
   a.wq = wq;
   a.wk = wk;
   a.cos = cos;
@@ -347,11 +347,12 @@ NormArgs norm_args(const void* q, const void* k, int64_t B, int64_t S, int64_t H
 }  // namespace
 
 extern "C" int tbf16_qk_norm_rope(const void* q, const void* k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D,
-                                  const int64_t* q_st, const int64_t* k_st, const void* wq, const void* wk, int w_f32,
-                                  const float* cos, const float* sin, int64_t rows, int64_t R, const int32_t* pos,
-                                  int64_t p_sb, int64_t p_ss, float eps, int interleaved, void* yq, void* yk,
-                                  void* stream) {
-  NormArgs a = norm_args(q, k, B, S, H, Hkv, D, q_st, k_st, wq, wk, cos, sin, rows, R, pos, p_sb, p_ss, eps);
+                                  int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                                  const void* wq, const void* wk, int w_f32, const float* cos, const float* sin,
+                                  int64_t rows, int64_t R, const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps,
+                                  int interleaved, void* yq, void* yk, void* stream) {
+  NormArgs a = norm_args({(const uint16_t*)q, q_sb, q_ss, q_sh}, {(const uint16_t*)k, k_sb, k_ss, k_sh}, B, S, H, Hkv, D, wq,
+                         wk, cos, sin, rows, R, pos, p_sb, p_ss, eps);
   a.yq = (uint16_t*)yq;
   a.yk = (uint16_t*)yk;
   if (int rc = check_norm("qk_norm_rope", a, B, S, H, Hkv, D, R)) return rc;
@@ -366,14 +367,16 @@ extern "C" size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t 
 }
 
 extern "C" int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, int64_t B, int64_t S,
-                                      int64_t H, int64_t Hkv, int64_t D, const int64_t* q_st, const int64_t* k_st,
-                                      const int64_t* dyq_st, const int64_t* dyk_st, const void* wq, const void* wk,
-                                      int w_f32, const float* cos, const float* sin, int64_t rows, int64_t R,
+                                      int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                                      int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t dyq_sb, int64_t dyq_ss,
+                                      int64_t dyq_sh, int64_t dyk_sb, int64_t dyk_ss, int64_t dyk_sh, const void* wq,
+                                      const void* wk, int w_f32, const float* cos, const float* sin, int64_t rows, int64_t R,
                                       const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps, int interleaved, void* dq,
                                       void* dk, void* dwq, void* dwk, void* ws, int64_t ws_bytes, void* stream) {
-  NormArgs a = norm_args(q, k, B, S, H, Hkv, D, q_st, k_st, wq, wk, cos, sin, rows, R, pos, p_sb, p_ss, eps);
-  a.dyq = {(const uint16_t*)dyq, dyq_st[0], dyq_st[1], dyq_st[2]};
-  a.dyk = {(const uint16_t*)dyk, dyk_st[0], dyk_st[1], dyk_st[2]};
+  NormArgs a = norm_args({(const uint16_t*)q, q_sb, q_ss, q_sh}, {(const uint16_t*)k, k_sb, k_ss, k_sh}, B, S, H, Hkv, D, wq,
+                         wk, cos, sin, rows, R, pos, p_sb, p_ss, eps);
+  a.dyq = {(const uint16_t*)dyq, dyq_sb, dyq_ss, dyq_sh};
+  a.dyk = {(const uint16_t*)dyk, dyk_sb, dyk_ss, dyk_sh};
   a.yq = (uint16_t*)dq;
   a.yk = (uint16_t*)dk;
   const bool weights = dwq != nullptr || dwk != nullptr;

@@ -108,7 +108,7 @@ __device__ __forceinline__ void token(const AdvanceArgs& a, int t, const int32_t
 __device__ __forceinline__ int prefix_of(const AdvanceArgs& a) { return a.prefix ? max(*a.prefix, 0) : 0; }
 
 // One block does everything but, with TOKENS false, the tokens. HERE: the batch's sums are kept in LDS.
-constexpr int kHere = 2048;
+constexpr int kHere = 2048, kInside = 4096;
 template <bool HERE, bool TOKENS>
 __global__ __launch_bounds__(1024) void paged_advance_kernel(AdvanceArgs a) {
   __shared__ int32_t s_mem[HERE ? 4 * kHere + 4 : 1];
@@ -219,7 +219,9 @@ __global__ __launch_bounds__(256) void paged_tokens_kernel(AdvanceArgs a) {
 
 }  // namespace
 
-extern "C" size_t tbf16_paged_advance_ws_bytes(int64_t B) { return B > 0 ? (size_t)(3 * B + 4) * 4 : 16; }
+extern "C" size_t tbf16_paged_advance_ws_bytes(int64_t B, int64_t tokens) {
+  return B < 0 ? 0 : B <= kHere && tokens <= kInside ? 0 : (size_t)(3 * B + 4) * 4;
+}
 
 extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t B, int64_t max_pages, int32_t* lengths,
                                    const int32_t* counts, int32_t* free_pages, int64_t pages, int32_t* n_free, int64_t page,
@@ -236,12 +238,13 @@ extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t
                         (const void*)n_free, (const void*)prefix, (const void*)slots, (const void*)positions,
                         (const void*)starts, (const void*)ws})
     TB_CHECK(aligned4(p), "paged_advance: misaligned pointer");
-  TB_CHECK(n_free != nullptr && starts != nullptr && ws != nullptr, "paged_advance: missing pointer");
-  if (ws_bytes < (int64_t)tbf16_paged_advance_ws_bytes(B)) {
-    set_error("paged_advance: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, tbf16_paged_advance_ws_bytes(B));
+  TB_CHECK(n_free != nullptr && starts != nullptr, "paged_advance: missing pointer");
+  const size_t need = tbf16_paged_advance_ws_bytes(B, tokens);
+  if (ws_bytes < (int64_t)need || (need && ws == nullptr)) {
+    set_error("paged_advance: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, need);
     return TBF16_EWS;
   }
-  AdvanceArgs a;
+  AdvanceArgs a = {};
   a.table = table;
   a.t_sb = table_stride;
   a.B = (int)B;
@@ -257,12 +260,14 @@ extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t
   a.slots = slots;
   a.positions = positions;
   a.starts = starts;
-  a.top = (int32_t*)ws;
-  a.base = a.top + 4;
-  a.first = a.base + B;
-  a.rel = a.first + B;
+  if (need) {
+    a.top = (int32_t*)ws;
+    a.base = a.top + 4;
+    a.first = a.base + B;
+    a.rel = a.first + B;
+  }
   const hipStream_t st = as_stream(stream);
-  const bool here = B <= kHere, inside = tokens <= 4096;
+  const bool here = B <= kHere, inside = tokens <= kInside;
   const int nt = 1024;
   if (here && inside) paged_advance_kernel<true, true><<<1, nt, 0, st>>>(a);
   else if (here) paged_advance_kernel<true, false><<<1, nt, 0, st>>>(a);

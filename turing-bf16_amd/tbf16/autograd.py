@@ -437,13 +437,12 @@ class QKNormRopeFn(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.how = eps, interleaved
-        return norm_rope.Call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved).forward()
+        return norm_rope.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
-        call = norm_rope.Call(*ctx.saved_tensors, *ctx.how)
-        return (*call.backward(dyq, dyk, *ctx.needs_input_grad[:4]), None, None, None, None, None)
+        return (*norm_rope.backward(*ctx.saved_tensors, *ctx.how, dyq, dyk, ctx.needs_input_grad[:4]), None, None, None, None, None)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):

@@ -9,14 +9,12 @@ tbf16.autograd.qk_norm_rope is the same with gradients.
 """
 from __future__ import annotations
 
-import ctypes
-import math
-
 import torch
 
 from ._ext import launch, lib, ptr
 
 MAX_HEAD_DIM = 256
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _device(x, *others) -> int:
@@ -31,93 +29,65 @@ def _device(x, *others) -> int:
 
 
 def _heads(x):
-    """(x, its (b, s, h) strides) with heads the kernels read in place: x itself or a copy."""
-    st = x.stride()
-    if st[-1] != 1 or any(v & 7 for v in st[:-1]) or x.data_ptr() & 15:
-        x = x.clone(memory_format=torch.contiguous_format)
-        st = x.stride()
-    return x, (ctypes.c_int64 * 3)(*((0, *st[:2]) if len(st) == 3 else st[:3]))
+    """(x, its address, its (b, s, h) strides) with heads the kernels read in place: x itself or a copy."""
+    st, at = x.stride(), x.data_ptr()
+    if len(st) == 3:
+        sb, (ss, sh, step) = 0, st
+    else:
+        sb, ss, sh, step = st
+    if step != 1 or (sb | ss | sh) & 7 or at & 15:
+        return _heads(x.clone(memory_format=_CONTIGUOUS))
+    return x, at, (sb, ss, sh)
 
 
 def _table(t):
-    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=_CONTIGUOUS)
 
 
-class Call:
-    """The checked arguments of one call: what forward and backward have in common."""
-
-    def __init__(self, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        shape, kshape = q.shape, k.shape
-        if len(shape) not in (3, 4) or shape[:-2] != kshape[:-2] or shape[-1] != kshape[-1] or not shape[-2] or not kshape[-2]:
-            raise ValueError(f"tbf16.qk_norm_rope: q {tuple(shape)} and k {tuple(kshape)} are not ((B,) S, H, D) and "
-                             "((B,) S, Hkv, D)")
-        D = shape[-1]
-        if D % 16 or not 0 < D <= MAX_HEAD_DIM:
-            raise ValueError(f"tbf16.qk_norm_rope: head dim {D} is not a multiple of 16 up to {MAX_HEAD_DIM}")
-        if q.dtype is not torch.bfloat16 or k.dtype is not torch.bfloat16:
-            raise TypeError("tbf16.qk_norm_rope: expected bf16 q and k")
-        if q_weight.shape != (D,) or k_weight.shape != (D,):
-            raise ValueError(f"tbf16.qk_norm_rope: weights {tuple(q_weight.shape)} and {tuple(k_weight.shape)} are not ({D},)")
-        if q_weight.dtype is not k_weight.dtype or q_weight.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError("tbf16.qk_norm_rope: expected weights both bf16 or both fp32")
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] == 0:
-            raise ValueError(f"tbf16.qk_norm_rope: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} are not tables of one "
-                             "shape (positions, rotated dims / 2)")
-        if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
-            raise TypeError("tbf16.qk_norm_rope: expected fp32 cos and sin")
-        R = 2 * cos.shape[1]
-        if R % 16 or not 0 < R <= D:
-            raise ValueError(f"tbf16.qk_norm_rope: {R} rotated dims are not a multiple of 16 up to the head dim {D}")
-        lead = shape[:-2]
-        if positions.dtype is not torch.int32:
-            raise TypeError("tbf16.qk_norm_rope: expected int32 positions")
-        if positions.shape != lead and positions.shape != lead[1:]:
-            raise ValueError(f"tbf16.qk_norm_rope: positions {tuple(positions.shape)} for tokens {tuple(lead)}")
-        if not 0.0 <= eps < math.inf:
-            raise ValueError(f"tbf16.qk_norm_rope: eps {eps}")
-        _device(q, k, q_weight, k_weight, cos, sin, positions)
-        self.B, self.S = (1, shape[0]) if len(lead) == 1 else lead
-        self.tokens = self.B * self.S
-        if self.tokens >= 2 ** 31:
-            raise ValueError(f"tbf16.qk_norm_rope: {self.tokens} tokens")
-        p_st = positions.stride()
-        self.p_st = p_st if len(p_st) == 2 else (0, *p_st) if len(p_st) else (0, 0)
-        (self.q, self.q_st), (self.k, self.k_st) = _heads(q), _heads(k)
-        self.wq, self.wk, self.cos, self.sin = q_weight.contiguous(), k_weight.contiguous(), _table(cos), _table(sin)
-        self.pos, self.eps, self.near, self.D, self.R = positions, float(eps), int(bool(interleaved)), D, R
-
-    def sizes(self):
-        return self.B, self.S, self.q.shape[-2], self.k.shape[-2], self.D
-
-    def tail(self):
-        return (self.wq.data_ptr(), self.wk.data_ptr(), int(self.wq.dtype is torch.float32), self.cos.data_ptr(),
-                self.sin.data_ptr(), self.cos.shape[0], self.R, self.pos.data_ptr(), *self.p_st, self.eps, self.near)
-
-    def forward(self):
-        q, k = self.q, self.k
-        yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
-        if self.tokens:
-            launch("tbf16_qk_norm_rope", q, q.data_ptr(), k.data_ptr(), *self.sizes(), self.q_st, self.k_st, *self.tail(),
-                   yq.data_ptr(), yk.data_ptr())
-        return yq, yk
-
-    def backward(self, dyq, dyk, want_q, want_k, want_wq, want_wk):
-        q, k = self.q, self.k
-        _device(q, dyq, dyk)
-        (dyq, dyq_st), (dyk, dyk_st) = _heads(dyq.to(torch.bfloat16)), _heads(dyk.to(torch.bfloat16))
-        dq = q.new_empty(q.shape) if want_q else None
-        dk = k.new_empty(k.shape) if want_k else None
-        dwq = torch.empty_like(self.wq) if want_wq else None
-        dwk = torch.empty_like(self.wk) if want_wk else None
-        ws = None
-        if want_wq or want_wk:
-            with torch.cuda.device(q.device):
-                wsb = lib().tbf16_qk_norm_rope_bwd_ws_bytes(self.B, self.S, self.D)
-            ws = q.new_empty(wsb, dtype=torch.uint8)
-        launch("tbf16_qk_norm_rope_bwd", q, q.data_ptr(), k.data_ptr(), dyq.data_ptr(), dyk.data_ptr(), *self.sizes(),
-               self.q_st, self.k_st, dyq_st, dyk_st, *self.tail(), ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(ws),
-               0 if ws is None else ws.numel())
-        return dq, dk, dwq, dwk
+def _checked(q, k, wq, wk, cos, sin, positions, eps, interleaved):
+    """(sizes, tail, kept): the arguments of the entry points that are alike for both directions, around the
+    heads, and the tensors that their addresses belong to. Raises for what the kernels do not take."""
+    shape, kshape = q.shape, k.shape
+    D, n = shape[-1] if len(shape) else 0, len(shape)
+    if ((n != 3 and n != 4) or len(kshape) != n or shape[0] != kshape[0] or shape[n - 3] != kshape[n - 3] or kshape[-1] != D
+            or not shape[-2] or not kshape[-2]):
+        raise ValueError(f"tbf16.qk_norm_rope: q {tuple(shape)} and k {tuple(kshape)} are not ((B,) S, H, D) and "
+                         "((B,) S, Hkv, D)")
+    if D & 15 or not 0 < D <= MAX_HEAD_DIM:
+        raise ValueError(f"tbf16.qk_norm_rope: head dim {D} is not a multiple of 16 up to {MAX_HEAD_DIM}")
+    if q.dtype is not torch.bfloat16 or k.dtype is not torch.bfloat16:
+        raise TypeError("tbf16.qk_norm_rope: expected bf16 q and k")
+    if wq.shape != (D,) or wk.shape != (D,):
+        raise ValueError(f"tbf16.qk_norm_rope: weights {tuple(wq.shape)} and {tuple(wk.shape)} are not ({D},)")
+    wide = wq.dtype is torch.float32
+    if wq.dtype is not wk.dtype or not (wide or wq.dtype is torch.bfloat16):
+        raise TypeError("tbf16.qk_norm_rope: expected weights both bf16 or both fp32")
+    table = cos.shape
+    if len(table) != 2 or table != sin.shape or table[0] == 0:
+        raise ValueError(f"tbf16.qk_norm_rope: cos {tuple(table)} and sin {tuple(sin.shape)} are not tables of one "
+                         "shape (positions, rotated dims / 2)")
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
+        raise TypeError("tbf16.qk_norm_rope: expected fp32 cos and sin")
+    R = 2 * table[1]
+    if R & 15 or not 0 < R <= D:
+        raise ValueError(f"tbf16.qk_norm_rope: {R} rotated dims are not a multiple of 16 up to the head dim {D}")
+    if positions.dtype is not torch.int32:
+        raise TypeError("tbf16.qk_norm_rope: expected int32 positions")
+    B, S = (1, shape[0]) if n == 3 else shape[:2]
+    p, p_st = positions.shape, positions.stride()
+    if p == (S,):
+        p_st = 0, p_st[0]
+    elif n == 3 or p != (B, S):
+        raise ValueError(f"tbf16.qk_norm_rope: positions {tuple(p)} for tokens {tuple(shape[:-2])}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"tbf16.qk_norm_rope: eps {eps}")
+    if B * S >= 2 ** 31:
+        raise ValueError(f"tbf16.qk_norm_rope: {B * S} tokens")
+    _device(q, k, wq, wk, cos, sin, positions)
+    wq, wk, cos, sin = wq.contiguous(), wk.contiguous(), _table(cos), _table(sin)
+    return ((B, S, shape[-2], kshape[-2], D),
+            (wq.data_ptr(), wk.data_ptr(), wide, cos.data_ptr(), sin.data_ptr(), table[0], R, positions.data_ptr(), *p_st, eps,
+             bool(interleaved)), (wq, wk, cos, sin))
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):
@@ -131,4 +101,32 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interl
     fp32. Tokens of a negative position are padding and give zeros; a position past the tables has no
     angle and gives NaN, as does a head of zeros without an eps. Inference only; gradients:
     tbf16.autograd.qk_norm_rope."""
-    return Call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved).forward()
+    sizes, tail, kept = _checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    yq = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    yk = torch.empty_like(k, memory_format=_CONTIGUOUS)
+    q, at_q, q_st = _heads(q)
+    k, at_k, k_st = _heads(k)
+    launch("tbf16_qk_norm_rope", q, at_q, at_k, *sizes, *q_st, *k_st, *tail, yq.data_ptr(), yk.data_ptr())
+    return yq, yk
+
+
+def backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dyq, dyk, wanted):
+    """Gradients of q, k and both weights (None where wanted says so) from those of the outputs."""
+    sizes, tail, kept = _checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    _device(q, dyq, dyk)
+    if dyq.shape != q.shape or dyk.shape != k.shape:
+        raise ValueError(f"tbf16.qk_norm_rope: gradients {tuple(dyq.shape)} and {tuple(dyk.shape)}")
+    grads = [torch.empty_like(t, memory_format=_CONTIGUOUS) if want else None
+             for t, want in zip((q, k, kept[0], kept[1]), wanted)]
+    q, at_q, q_st = _heads(q)
+    k, at_k, k_st = _heads(k)
+    dyq, at_dyq, dyq_st = _heads(dyq.to(torch.bfloat16))
+    dyk, at_dyk, dyk_st = _heads(dyk.to(torch.bfloat16))
+    ws, wsb = None, 0
+    if wanted[2] or wanted[3]:
+        with torch.cuda.device(q.device):
+            wsb = lib().tbf16_qk_norm_rope_bwd_ws_bytes(sizes[0], sizes[1], sizes[4])
+        ws = q.new_empty(wsb, dtype=torch.uint8)
+    launch("tbf16_qk_norm_rope_bwd", q, at_q, at_k, at_dyq, at_dyk, *sizes, *q_st, *k_st, *dyq_st, *dyk_st, *tail,
+           *map(ptr, grads), ptr(ws), wsb)
+    return grads

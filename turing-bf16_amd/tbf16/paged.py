@@ -57,9 +57,10 @@ def _same_device(fn, first, *others):
 
 
 def _index(fn, name, t, dim):
-    if t.dtype is not torch.int32 or t.dim() != dim:
+    st = t.stride()
+    if t.dtype is not torch.int32 or len(st) != dim:
         raise TypeError(f"tbf16.{fn}: expected {name} as an int32 tensor of {dim} dimension(s)")
-    return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
+    return t if st[-1] == 1 or t.shape[-1] < 2 else t.contiguous()
 
 
 def _rows(t):
@@ -76,23 +77,6 @@ def _span(t):
     """The addresses from a tensor's first element to behind its last one."""
     at = t.data_ptr()
     return at, at + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
-
-
-def _state(fn, tensors):
-    """Refuses tensors that the operator changes in place but cannot: not int32, not side by side,
-    or two of them in the same memory."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.dtype is not torch.int32:
-            raise TypeError(f"tbf16.{fn}: expected {name} as int32, got {t.dtype}")
-        if name != "page_table" and t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1:
-            raise ValueError(f"tbf16.{fn}: {name} must be contiguous")
-    there = [t for t in tensors.values() if t is not None and t.numel()]
-    if len({t.untyped_storage().data_ptr() for t in there}) < len(there):
-        spans = sorted(_span(t) for t in there)
-        if any(b0 < a1 for (_, a1), (b0, _) in zip(spans, spans[1:])):
-            raise ValueError(f"tbf16.{fn}: {', '.join(tensors)} lie in the same memory")
 
 
 def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens, prefix_length=None):
@@ -119,39 +103,48 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     zeros. Taking all granted tokens back leaves lengths, table and stack as they were.
 
     Lengths outside [0, n * page] count as the nearest there is, n_free likewise."""
-    if page_table.dim() != 2:
-        raise ValueError(f"tbf16.paged_advance: page_table {tuple(page_table.shape)} is not (B, n)")
-    B, n = page_table.shape
-    for name, t in (("lengths", lengths), ("counts", counts)):
-        if t.shape != (B,):
-            raise ValueError(f"tbf16.paged_advance: {name} {tuple(t.shape)} for {B} sequences")
-    if free_pages.dim() != 1:
-        raise ValueError(f"tbf16.paged_advance: free_pages {tuple(free_pages.shape)} is not (pages,)")
-    for name, t in (("n_free", n_free), ("prefix_length", prefix_length)):
-        if t is not None and t.numel() != 1:
-            raise ValueError(f"tbf16.paged_advance: {name} is one number, got {tuple(t.shape)}")
-    state = {"page_table": page_table, "lengths": lengths, "counts": counts, "free_pages": free_pages, "n_free": n_free}
-    others = [lengths, counts, free_pages, n_free]
-    if prefix_length is not None:
-        state["prefix_length"] = prefix_length
-        others.append(prefix_length)
-    _same_device("paged_advance", page_table, *others)
-    _state("paged_advance", state)
-    pages, page, tokens = free_pages.shape[0], int(page), int(tokens)
-    row = page_table.stride(0) if B > 1 else max(n, 1)
-    if (n > 1 and page_table.stride(1) != 1) or row < n:
+    shape, row = page_table.shape, page_table.stride()
+    others = (lengths, counts, free_pages, n_free) if prefix_length is None else (lengths, counts, free_pages, n_free, prefix_length)
+    if len(shape) != 2:
+        raise ValueError(f"tbf16.paged_advance: page_table {tuple(shape)} is not (B, n)")
+    B, n = shape
+    sizes = [t.numel() for t in others]
+    if sizes[:2] != [B, B] or sizes[3] != 1 or sizes[-1] != 1:
+        raise ValueError(f"tbf16.paged_advance: {sizes[0]} lengths and {sizes[1]} counts for {B} sequences; n_free and "
+                         f"prefix_length are one number each, got {sizes[3:]}")
+    at = page_table.data_ptr()
+    spans = [(at, at + 4 * ((B - 1) * row[0] + n))] if B and n else []
+    for t, size in zip(others, sizes):
+        if t.dtype is not torch.int32:
+            raise TypeError(f"tbf16.paged_advance: expected int32, got {t.dtype} {tuple(t.shape)}")
+        if t.dim() > 1 or not t.is_contiguous():
+            raise ValueError(f"tbf16.paged_advance: lengths, counts and free_pages must be contiguous, of one dimension, got {tuple(t.shape)}")
+        if size:
+            at = t.data_ptr()
+            spans.append((at, at + 4 * size))
+    if page_table.dtype is not torch.int32:
+        raise TypeError(f"tbf16.paged_advance: expected page_table as int32, got {page_table.dtype}")
+    if (n > 1 and row[1] != 1) or (B > 1 and row[0] < n):
         raise ValueError("tbf16.paged_advance: page_table's rows must be contiguous and apart")
+    _same_device("paged_advance", page_table, *others)
+    spans.sort()
+    end = 0
+    for span in spans:
+        if span[0] < end:
+            raise ValueError("tbf16.paged_advance: two of its arguments lie in the same memory")
+        end = span[1]
+    pages, page, tokens = sizes[2], int(page), int(tokens)
     if page < 1 or pages * page >= 2 ** 31 - 1:
         raise ValueError(f"tbf16.paged_advance: {pages} pages of {page} positions")
     if not 0 <= tokens < 2 ** 31 - 1024 or B * n >= 2 ** 31:
-        raise ValueError(f"tbf16.paged_advance: room for {tokens} tokens, page_table {tuple(page_table.shape)}")
+        raise ValueError(f"tbf16.paged_advance: room for {tokens} tokens, page_table {tuple(shape)}")
     torch.autograd.graph.increment_version((page_table, lengths, free_pages, n_free))
-    # one allocation: slots, positions, starts and the workspace
-    out = page_table.new_empty(2 * tokens + B + 1 + 3 * B + 4)
-    slots, positions, starts, ws = out.split((tokens, tokens, B + 1, 3 * B + 4))
-    launch("tbf16_paged_advance", page_table, page_table.data_ptr(), row, B, n, lengths.data_ptr(), counts.data_ptr(),
-           free_pages.data_ptr(), pages, n_free.data_ptr(), page, tokens, ptr(prefix_length), slots.data_ptr(),
-           positions.data_ptr(), starts.data_ptr(), ws.data_ptr(), 4 * ws.numel())
+    slots, positions, starts = page_table.new_empty(tokens), page_table.new_empty(tokens), page_table.new_empty(B + 1)
+    wsb = lib().tbf16_paged_advance_ws_bytes(B, tokens)
+    ws = page_table.new_empty(wsb, dtype=torch.uint8) if wsb else None
+    launch("tbf16_paged_advance", page_table, page_table.data_ptr(), max(row[0], n), B, n, lengths.data_ptr(),
+           counts.data_ptr(), free_pages.data_ptr(), pages, n_free.data_ptr(), page, tokens, ptr(prefix_length),
+           slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), ptr(ws), wsb)
     return slots, positions, starts
 
 

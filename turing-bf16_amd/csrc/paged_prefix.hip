@@ -20,7 +20,7 @@ struct PrefixArgs {
   int64_t q_sb, q_sh;
   CacheGeom kg, vg;
   const int32_t *table, *length;
-  int cap, S;  // positions the table covers; splits of the keys
+  int cap, S, tiles;  // positions the table covers; splits of the keys; tiles of a key/value head's rows
   uint32_t pages, page;
   Div by_page, by_group;
   float scale_log2;
@@ -72,28 +72,11 @@ __device__ __forceinline__ void load16_lds(const void* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((global_void*)from, (lds_void*)to, 16, 0, 0);
 }
 
-// Which block of a launch does what: `own` blocks and `pre` blocks, eight of each in turn (one on every XCD)
-// as long as there are both, so that both kinds begin together.
-struct Mix {
-  int own, pre;
-};
-__device__ __forceinline__ bool mine(Mix m, int x, int& block) {  // whether x is an own block
-  const int both = min(m.own, m.pre) & ~7;
-  if (x < 2 * both) {
-    block = (x >> 4) * 8 + (x & 7);
-    return !(x & 8);
-  }
-  block = both + x - 2 * both;
-  if (block < m.own) return true;
-  block -= m.own - both;
-  return false;
-}
-
 struct LaunchArgs {
   PrefixArgs pre;
   AttnArgs own;
-  Mix mix;
-  bool unit;  // own blocks are units
+  int pre_blocks, own_blocks;  // the prefix's blocks first, then those of the own keys
+  bool unit;                   // own blocks are units
 };
 
 template <int DP, int RB, int WR, int WK, int KB, int ST, bool PAD>
@@ -108,8 +91,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
   __shared__ float2 s_stat[NW][16 * RB];
   __shared__ int s_flags[NW];
   uint8_t* const stages[4] = {st0, st1, st2, st3};
-  int block;
-  if (mine(args.mix, blockIdx.x, block)) {  // own keys
+  int block = blockIdx.x;
+  if (block >= args.pre_blocks) {  // own keys
+    block -= args.pre_blocks;
     const AttnArgs& o = args.own;
     static_assert(3 * own_rows(DP) * (DP + 4) * 4 <= STAGE, "three waves' rows fit a stage");
     auto rows_of = [&](int w) {
@@ -119,13 +103,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
       const int grp = block % o.RG, bh = block / o.RG, b = bh / o.Hkv;
       attn_block<DP, 1, NW, PAD, true, true>(o, rows_of, &s_stat[0][0].x, s_flags, b, 0, bh - b * o.Hkv, grp);
     } else {
-      attn_block<DP, 1, NW, PAD, false, true>(o, rows_of, &s_stat[0][0].x, s_flags, block, args.mix.own, 0, 0);
+      attn_block<DP, 1, NW, PAD, false, true>(o, rows_of, &s_stat[0][0].x, s_flags, block, args.own_blocks, 0, 0);
     }
     return;
   }
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
   const int wr = wave % WR, kg = wave / WR;
-  const int head = block % a.Hkv, split = block / a.Hkv % a.S, rt = block / a.Hkv / a.S;
+  // (blocks that read the same keys one behind the other, on one XCD where there are 8 heads)
+  const int head = block % a.Hkv, rt = block / a.Hkv % a.tiles, split = block / a.Hkv / a.tiles;
   const int length = prefix_len(a.length, a.cap);
   const Splits sp = splits_of(length, KS, a.S);
   const int t0 = split * sp.each, tn = min(sp.each, sp.tiles - t0);
@@ -445,7 +430,7 @@ struct JoinArgs {
 };
 
 // 64 groups of 4 outputs a block; its waves take a row's parts in turns and meet in LDS.
-constexpr int kMeet = 8;
+constexpr int kMeet = 4;
 __global__ __launch_bounds__(kMeet * 64) void prefix_join_kernel(JoinArgs j) {
   __shared__ float4 so[kMeet][64];
   __shared__ float2 ss[kMeet][64];
@@ -525,7 +510,9 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
   PrefixPlan p;
   const int64_t G = H / Hkv, n = B * G;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  p.few = p.DP < 256 && n <= 64;
+  // Blocks of 64 rows, two groups of waves on different keys, or of 128: the former where the rows are few, or leave
+  // a fifth and more of 128 empty (192 rows on 16384 keys 38.9 and 42.8 us; 128 rows on 4096: 28.1 and 24.5).
+  p.few = p.DP < 256 && 5 * cdiv(n, 128) * 128 >= 6 * cdiv(n, 64) * 64;
   p.rows = p.DP == 256 || p.few ? 64 : 128;
   p.keys = p.DP == 256 ? 32 : 64;
   p.tiles = cdiv(n, p.rows);
@@ -557,7 +544,7 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
 
 template <int DP, int RB, int WR, int WK, int KB, int ST>
 void launch_form(const LaunchArgs& a, hipStream_t st) {
-  const unsigned grid = (unsigned)(a.mix.own + a.mix.pre);
+  const unsigned grid = (unsigned)(a.pre_blocks + a.own_blocks);
   if (a.pre.D == DP) prefix_kernel<DP, RB, WR, WK, KB, ST, false><<<grid, 256, 0, st>>>(a);
   else prefix_kernel<DP, RB, WR, WK, KB, ST, true><<<grid, 256, 0, st>>>(a);
 }
@@ -638,6 +625,7 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
   a.length = prefix_length;
   a.cap = (int)pcap;
   a.S = pcap > 0 ? (int)p.S : 0;
+  a.tiles = (int)p.tiles;
   a.pages = (uint32_t)pages;
   a.page = (uint32_t)page;
   a.by_page = div_by(page);
@@ -650,7 +638,8 @@ extern "C" int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int6
   a.D = (int)D;
   a.part = (float*)(w + p.part);
   a.stat = (float*)(w + p.stat);
-  la.mix = {(int)p.own.blocks, (int)(Hkv * a.S * p.tiles)};
+  la.pre_blocks = (int)(Hkv * a.S * p.tiles);
+  la.own_blocks = (int)p.own.blocks;
   JoinArgs j{la.own, la.pre, p.keys, p.own.unit, (int)p.own.blocks, (uint16_t*)o};
   const hipStream_t st = as_stream(stream);
   launch_prefix(la, p, st);

@@ -516,12 +516,14 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
   p.rows = p.DP == 256 || p.few ? 64 : 128;
   p.keys = p.DP == 256 ? 32 : 64;
   p.tiles = cdiv(n, p.rows);
-  // Splits: two blocks a CU, but no more than pays for the parts they leave: a tile takes ~ 2.5 us, a split's
-  // part of all rows 8 bytes an element, written and read at 4 TB/s.
+  // Splits: a block a CU, which leaves half of its room to the own keys' blocks (256 rows of 8 heads on 8192 keys:
+  // 16 splits 35.2 us, two blocks a CU 47.5), but no more than pays for the parts they leave: a tile takes a block
+  // ~ 1.3 us, a split's part of all rows 8 bytes an element at 8 TB/s and 0.05 us of the join (65 rows of 4 heads
+  // on 2999 keys: 24 splits 13.8 us, 47 splits 15.2).
   const int64_t all = cdiv(prefix_cap, p.keys);
-  const double part_us = (double)(B * H * D) * 8 / 4e6;
-  const int64_t most = std::max<int64_t>(1, (int64_t)std::sqrt(2.5 * (double)all / part_us));
-  p.S = std::min({all, most, std::max<int64_t>(1, 2 * num_cus() / (Hkv * p.tiles))});
+  const double part_us = (double)(B * H * D) * 1e-6 + 0.05;
+  const int64_t most = std::max<int64_t>(1, (int64_t)std::sqrt(1.3 * (double)all / part_us));
+  p.S = std::min({all, most, std::max<int64_t>(1, num_cus() / (Hkv * p.tiles))});
 
   AttnPlan& o = p.own;
   o.DP = p.DP;
@@ -529,8 +531,10 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
   o.wpb = 4;
   o.R = (int)std::min<int64_t>(G, own_rows(p.DP));
   o.RG = (int)cdiv(G, o.R);
-  o.unit = cdiv(cap, kTile) <= 4 * o.wpb && B * Hkv * o.RG <= num_cus();
-  o.blocks = o.unit ? B * Hkv * o.RG : num_cus();
+  // (a block a unit as long as that is a few tiles a wave: 64 sequences of up to 512 keys, 8 heads, behind 8192: 41.0
+  // and 45.1 us; very many short units are joined to runs)
+  o.unit = cdiv(cap, kTile) <= 4 * o.wpb && B * Hkv * o.RG <= 4 * num_cus();
+  o.blocks = o.unit ? B * Hkv * o.RG : 2 * num_cus();
   o.stat = align_up((size_t)o.blocks * 2 * o.R * (size_t)D * 4, 256);
   o.desc = o.bytes = o.unit ? 0 : o.stat + align_up((size_t)o.blocks * 2 * o.R * 2 * 4, 256);
   p.part = o.bytes;

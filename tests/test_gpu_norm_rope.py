@@ -227,3 +227,27 @@ def test_graph(dev):
         want = step(b, dys)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+def test_no_second_derivatives(dev):
+    """create_graph gives the same gradients; differentiating them raises."""
+    a = inputs(dev, 1, 9, 4, 2, 64, 32)
+    leaves = [t.detach().requires_grad_() for t in a[:4]]
+    dys = (torch.ones_like(a[0]), torch.ones_like(a[1]))
+    want = torch.autograd.grad(tbf16.autograd.qk_norm_rope(*leaves, *a[4:]), leaves, dys)
+    got = torch.autograd.grad(tbf16.autograd.qk_norm_rope(*leaves, *a[4:]), leaves, dys, create_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    with pytest.raises(RuntimeError):
+        got[0].sum().backward()
+
+
+def test_saved_tensors_moved_by_hooks(dev):
+    """Saved inputs that come back from the host in another layout."""
+    a = inputs(dev, 2, 30, 4, 2, 64, 32)
+    dys = (torch.ones_like(a[0]), torch.ones_like(a[1]))
+    leaves = [t.detach().requires_grad_() for t in a[:4]]
+    want = torch.autograd.grad(tbf16.autograd.qk_norm_rope(*leaves, *a[4:]), leaves, dys)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+        y = tbf16.autograd.qk_norm_rope(*leaves, *a[4:])
+    got = torch.autograd.grad(y, leaves, dys)
+    assert all(torch.equal(x, w) for x, w in zip(got, want))

@@ -26,7 +26,7 @@ namespace {
 struct AdvanceArgs {
   int32_t* table;
   int64_t t_sb;
-  int B, cap;  // cap: positions a table row covers
+  int B, n, cap;  // cap: positions the n entries of a table row cover
   int32_t* lengths;
   const int32_t* counts;
   int32_t* free;
@@ -90,11 +90,13 @@ __device__ __forceinline__ void token(const AdvanceArgs& a, int t, const int32_t
     const int b = last_upto(starts, a.B, t), from = base[b];
     if (from >= 0) {
       const int j = from + t - starts[b], p = j / a.page, r = j - p * a.page, kept = pages_of(a, from);
-      int id;
-      if (p < kept) {
+      const int at = top - 1 - first[b] - (p - kept);
+      int id = -1;
+      // (the bounds hold unless another stream writes lengths or counts meanwhile)
+      if (p < min(kept, a.n)) {
         id = a.table[b * a.t_sb + p];
-      } else {
-        id = a.free[top - 1 - first[b] - (p - kept)];
+      } else if (p < a.n && (uint32_t)at < (uint32_t)a.P) {
+        id = a.free[at];
         if (r == 0) a.table[b * a.t_sb + p] = id;
       }
       if ((uint32_t)id < (uint32_t)a.P) slot = id * a.page + r;
@@ -228,7 +230,7 @@ extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t
                                    int64_t tokens, const int32_t* prefix, int32_t* slots, int32_t* positions,
                                    int32_t* starts, void* ws, int64_t ws_bytes, void* stream) {
   const int64_t top31 = (int64_t)1 << 31;
-  TB_CHECK(B >= 0 && B < top31 - 1 && max_pages >= 0 && max_pages < top31 && (double)B * (double)max_pages < 2147483648.0,
+  TB_CHECK(B >= 0 && B < top31 / 2 && max_pages >= 0 && max_pages < top31 && (double)B * (double)max_pages < 2147483648.0,
            "paged_advance: bad table shape");
   TB_CHECK(B <= 1 || table_stride >= max_pages, "paged_advance: table rows overlap");
   TB_CHECK(page > 0 && page < top31 && pages >= 0 && (double)pages * (double)page < 2147483647.0,
@@ -248,6 +250,7 @@ extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t
   a.table = table;
   a.t_sb = table_stride;
   a.B = (int)B;
+  a.n = (int)max_pages;
   a.cap = (int)std::min<int64_t>(max_pages * page, INT32_MAX);
   a.lengths = lengths;
   a.counts = counts;

@@ -440,9 +440,15 @@ class QKNormRopeFn(torch.autograd.Function):
         return norm_rope.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
+        if torch.is_grad_enabled():  # create_graph: the gradients have none of their own
+            return QKNormRopeFn._once(ctx, dyq, dyk)
         return (*norm_rope.backward(*ctx.saved_tensors, *ctx.how, dyq, dyk, ctx.needs_input_grad[:4]), None, None, None, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def _once(ctx, dyq, dyk):
+        return QKNormRopeFn.backward(ctx, dyq, dyk)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):

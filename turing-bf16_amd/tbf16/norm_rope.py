@@ -110,23 +110,41 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interl
     return yq, yk
 
 
+# tbf16_qk_norm_rope_bwd's workspace bytes per (device, B, S, D): its blocks are counted by the device's
+# CUs, so it is asked on the tensors' device, once
+_WS_BYTES: dict = {}
+
+
+def _ws_bytes(dev: int, *sizes: int) -> int:
+    key = (dev, sizes)
+    n = _WS_BYTES.get(key)
+    if n is None:
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        with torch.cuda.device(dev):
+            n = _WS_BYTES[key] = int(lib().tbf16_qk_norm_rope_bwd_ws_bytes(*sizes))
+    return n
+
+
 def backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dyq, dyk, wanted):
     """Gradients of q, k and both weights (None where wanted says so) from those of the outputs."""
     sizes, tail, kept = _checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    _device(q, dyq, dyk)
-    if dyq.shape != q.shape or dyk.shape != k.shape:
-        raise ValueError(f"tbf16.qk_norm_rope: gradients {tuple(dyq.shape)} and {tuple(dyk.shape)}")
-    grads = [torch.empty_like(t, memory_format=_CONTIGUOUS) if want else None
-             for t, want in zip((q, k, kept[0], kept[1]), wanted)]
+    dev = _device(q, dyq, dyk)
+    if dyq.shape != q.shape or dyk.shape != k.shape or dyq.dtype is not torch.bfloat16 or dyk.dtype is not torch.bfloat16:
+        raise ValueError(f"tbf16.qk_norm_rope: gradients {tuple(dyq.shape)} {dyq.dtype} and {tuple(dyk.shape)} {dyk.dtype}")
+    want_q, want_k, want_wq, want_wk = wanted
+    dq = torch.empty_like(q, memory_format=_CONTIGUOUS) if want_q else None
+    dk = torch.empty_like(k, memory_format=_CONTIGUOUS) if want_k else None
+    dwq = torch.empty_like(kept[0]) if want_wq else None
+    dwk = torch.empty_like(kept[1]) if want_wk else None
+    ws, wsb = None, 0
+    if want_wq or want_wk:
+        wsb = _ws_bytes(dev, sizes[0], sizes[1], sizes[4])
+        ws = q.new_empty(wsb, dtype=torch.uint8)
     q, at_q, q_st = _heads(q)
     k, at_k, k_st = _heads(k)
-    dyq, at_dyq, dyq_st = _heads(dyq.to(torch.bfloat16))
-    dyk, at_dyk, dyk_st = _heads(dyk.to(torch.bfloat16))
-    ws, wsb = None, 0
-    if wanted[2] or wanted[3]:
-        with torch.cuda.device(q.device):
-            wsb = lib().tbf16_qk_norm_rope_bwd_ws_bytes(sizes[0], sizes[1], sizes[4])
-        ws = q.new_empty(wsb, dtype=torch.uint8)
+    dyq, at_dyq, dyq_st = _heads(dyq)
+    dyk, at_dyk, dyk_st = _heads(dyk)
     launch("tbf16_qk_norm_rope_bwd", q, at_q, at_k, at_dyq, at_dyk, *sizes, *q_st, *k_st, *dyq_st, *dyk_st, *tail,
-           *map(ptr, grads), ptr(ws), wsb)
-    return grads
+           ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(ws), wsb)
+    return dq, dk, dwq, dwk

@@ -136,7 +136,7 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     pages, page, tokens = sizes[2], int(page), int(tokens)
     if page < 1 or pages * page >= 2 ** 31 - 1:
         raise ValueError(f"tbf16.paged_advance: {pages} pages of {page} positions")
-    if not 0 <= tokens < 2 ** 31 - 1024 or B * n >= 2 ** 31:
+    if not 0 <= tokens < 2 ** 31 - 1024 or B * max(n, 2) >= 2 ** 31:
         raise ValueError(f"tbf16.paged_advance: room for {tokens} tokens, page_table {tuple(shape)}")
     torch.autograd.graph.increment_version((page_table, lengths, free_pages, n_free))
     slots, positions, starts = page_table.new_empty(tokens), page_table.new_empty(tokens), page_table.new_empty(B + 1)

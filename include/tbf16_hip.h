@@ -340,14 +340,14 @@ int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int64_t Hkv, in
  * position give zeros, of positions from `rows` on NaN. yq, yk bf16 contiguous.
  * The gradient: dq, dk, bf16 contiguous, dwq, dwk (D,) in the weights' type, each may be NULL, from dyq,
  * dyk with strides of their own; sums over tokens in a fixed order. ws:
- * tbf16_qk_norm_rope_bwd_ws_bytes(B, S, D) bytes (asked with the stream's device current), this call's
+ * tbf16_qk_norm_rope_bwd_ws_bytes(B, S, H, Hkv, D) bytes (asked with the stream's device current), this call's
  * alone until it has run; not used without dwq and dwk. No counterpart in the reference. */
 int tbf16_qk_norm_rope(const void* q, const void* k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D,
                        int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* wq,
                        const void* wk, int w_f32, const float* cos, const float* sin, int64_t rows, int64_t R,
                        const int32_t* pos, int64_t p_sb, int64_t p_ss, float eps, int interleaved, void* yq, void* yk,
                        void* stream);
-size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t D);
+size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D);
 int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, int64_t B, int64_t S, int64_t H,
                            int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t k_sb, int64_t k_ss,
                            int64_t k_sh, int64_t dyq_sb, int64_t dyq_ss, int64_t dyq_sh, int64_t dyk_sb, int64_t dyk_ss,

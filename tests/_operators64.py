@@ -94,7 +94,8 @@ def norm_rope64(x, w, cos, sin, pos, eps=1e-6, near=False, dy=None):
     dx = r * (du - u * (du * u).mean(-1, keepdim=True))
     spread = r * (A * w.abs() + u.abs() * (A * (w * u).abs()).mean(-1, keepdim=True))
     tokens, H = pos.numel(), x.shape[-2]
-    sums = -(-H // (64 // (4 if D <= 64 else 8 if D <= 128 else 16))) * -(-tokens // 4096) + 90
+    # (up to 8 times as many heads of the other kind: 256 waves at least take these, or one a token)
+    sums = -(-H // (64 // (4 if D <= 64 else 8 if D <= 128 else 16))) * -(-tokens // 256) + 90
     flat = lambda t: t.flatten(0, -2)  # noqa: E731
     dw, dw_bound = flat(dz * u).sum(0), (22 + sums) * U24 * flat(A * u.abs()).sum(0)
     return (*out, dx, 2.0 ** -8 * dx.abs() + 80 * U24 * spread, dw, dw_bound)

@@ -168,7 +168,7 @@ def test_norm_rope_abi_refusals():
     assert bwd() == -3 and "workspace" in err()
     assert bwd(ws=None, wsb=1 << 30) == -3
     assert fwd(B=0) == 0 and fwd(S=0) == 0 and bwd(S=0, dwq=None) == 0
-    assert L.tbf16_qk_norm_rope_bwd_ws_bytes(2, 100, 64) > 0 == L.tbf16_qk_norm_rope_bwd_ws_bytes(0, 100, 64)
+    assert L.tbf16_qk_norm_rope_bwd_ws_bytes(2, 100, 4, 2, 64) > 0 == L.tbf16_qk_norm_rope_bwd_ws_bytes(0, 100, 4, 2, 64)
 
 
 @pytest.mark.parametrize("near", [False, True])

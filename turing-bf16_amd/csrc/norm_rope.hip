@@ -37,7 +37,8 @@ struct NormArgs {
   float eps, inv_d;
   int T, S, H, Hkv, D, R;
   uint16_t *yq, *yk;  // outputs, or dx of both
-  float* part;        // [block][2][D], the blocks' shares of the weights' gradients
+  int q_blocks;       // gradient: the first blocks take query heads, the others key heads
+  float* part;        // [block][D], the blocks' shares of the weights' gradients
 };
 
 // Sum over the L lanes of a head, in each of them (DPP quad_perm, row_half_mirror, row_mirror).
@@ -152,23 +153,31 @@ __device__ __forceinline__ void load_turn(const NormArgs& a, const Item<NEAR>& i
 template <int L, bool NEAR, bool W32, bool BACK>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
   constexpr int HPW = 64 / L, U = BACK ? 2 : 4;
-  __shared__ float s_dw[BACK ? 4 : 1][2][BACK ? 16 * L : 1];
+  __shared__ float s_dw[BACK ? 4 : 1][BACK ? 16 * L : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane % L, hl = lane / L;
   const Item<NEAR> it(i, a.D, a.R);
-  float w[2][16], dw[BACK ? 2 : 1][16];
-  load_weights<NEAR, W32>(a.wq, it, w[0]);
-  load_weights<NEAR, W32>(a.wk, it, w[1]);
-  if constexpr (BACK)
+  // Forward: query heads, then key heads, in steps of HPW. Gradient: one kind a block, whose registers then
+  // hold one set of weights and of their gradients (189 -> 153 registers, three waves a SIMD instead of two).
+  const int sq = (a.H + HPW - 1) / HPW, sk = (a.Hkv + HPW - 1) / HPW;
+  const bool key_block = BACK && (int)blockIdx.x >= a.q_blocks;
+  const int begin = key_block ? sq : 0, steps = BACK && !key_block ? sq : sq + sk;
+  float w[BACK ? 1 : 2][16], dw[16];
+  load_weights<NEAR, W32>(key_block ? a.wk : a.wq, it, w[0]);
+  if constexpr (BACK) {
 #pragma unroll
-    for (int p = 0; p < 16; ++p) dw[0][p] = dw[1][p] = 0.f;
-  const int sq = (a.H + HPW - 1) / HPW, steps = sq + (a.Hkv + HPW - 1) / HPW;
-  for (int64_t tt = (int64_t)blockIdx.x * 4 + wave; tt < a.T; tt += (int64_t)gridDim.x * 4) {
+    for (int p = 0; p < 16; ++p) dw[p] = 0.f;
+  } else {
+    load_weights<NEAR, W32>(a.wk, it, w[1]);
+  }
+  const int block = key_block ? blockIdx.x - a.q_blocks : blockIdx.x;
+  const int blocks = !BACK ? gridDim.x : key_block ? gridDim.x - a.q_blocks : a.q_blocks;
+  for (int64_t tt = (int64_t)block * 4 + wave; tt < a.T; tt += (int64_t)blocks * 4) {
     const int t = (int)tt, b = t / a.S, s = t - b * a.S;
     const int pos = __builtin_amdgcn_readfirstlane(a.pos[b * a.p_sb + s * a.p_ss]);
     Turn turn;
     if (pos >= 0) load_turn<NEAR>(a, it, i, pos, turn);
-    for (int st0 = 0; st0 < steps; st0 += U) {
+    for (int st0 = begin; st0 < steps; st0 += U) {
       uint4 xv[U][2], gv[BACK ? U : 1][2];
       auto head_of = [&](int st) { return (st < sq ? st : st - sq) * HPW + hl; };
       auto valid = [&](int st) { return it.there && st < steps && head_of(st) < (st < sq ? a.H : a.Hkv); };
@@ -195,7 +204,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
       for (int u = 0; u < U; ++u) {
         const int st = st0 + u;
         if (st >= steps) break;
-        const bool is_k = st >= sq;
+        const bool is_k = BACK ? key_block : st >= sq;
+        const float* const ws = w[BACK ? 0 : is_k];
         uint16_t* out = is_k ? a.yk : a.yq;
         if (out) out += ((int64_t)t * (is_k ? a.Hkv : a.H) + head_of(st)) * a.D;
         float x[16];
@@ -212,7 +222,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
           float y[16];
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            const float za = x[p] * w[is_k][p], zb = x[8 + p] * w[is_k][8 + p];
+            const float za = x[p] * ws[p], zb = x[8 + p] * ws[8 + p];
             y[p] = za * turn.c[p] - zb * turn.s[p];
             y[8 + p] = zb * turn.c[p] + za * turn.s[p];
           }
@@ -228,10 +238,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
           const bool mine = valid(st);  // (elsewhere x r may be NaN: zeros without an eps)
 #pragma unroll
           for (int p = 0; p < 16; ++p) {
-            const float part = mine ? d[p] * x[p] : 0.f;
-            if (is_k) dw[1][p] += part;
-            else dw[0][p] += part;
-            d[p] *= w[is_k][p];
+            dw[p] += mine ? d[p] * x[p] : 0.f;
+            d[p] *= ws[p];
             dot = fmaf(d[p], x[p], dot);
           }
           dot = sum_head<L>(dot) * a.inv_d;
@@ -245,48 +253,52 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
   if constexpr (BACK) {
     if (a.part == nullptr) return;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int p = 0; p < 16; ++p) {
+      float v = dw[p];
 #pragma unroll
-      for (int p = 0; p < 16; ++p) {
-        float v = dw[n][p];
-#pragma unroll
-        for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-        if (hl == 0 && it.there) s_dw[wave][n][it.at(p)] = v;
-      }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 2 * a.D; e += 256) {
-      const int n = e >= a.D, d = e - n * a.D;
-      a.part[(int64_t)blockIdx.x * 2 * a.D + e] = s_dw[0][n][d] + s_dw[1][n][d] + s_dw[2][n][d] + s_dw[3][n][d];
+      for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+      if (hl == 0 && it.there) s_dw[wave][it.at(p)] = v;
     }
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < a.D) a.part[(int64_t)blockIdx.x * a.D + d] = s_dw[0][d] + s_dw[1][d] + s_dw[2][d] + s_dw[3][d];
   }
 }
 
-// The blocks' shares of the weights' gradients, added in an order of their own: 16 columns a block, 64
-// threads each.
+// The blocks' shares of the weights' gradients, added in an order of their own: 16 columns of one kind a
+// block, 64 threads each.
 template <bool W32>
-__global__ __launch_bounds__(1024) void norm_rope_weights_kernel(const float* part, int blocks, int D, void* dwq, void* dwk) {
+__global__ __launch_bounds__(1024) void norm_rope_weights_kernel(const float* part, int q_blocks, int blocks, int D, void* dwq,
+                                                                 void* dwk) {
   __shared__ float s[64][17];
-  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
+  const bool key = blockIdx.y;
+  void* out = key ? dwk : dwq;
+  if (out == nullptr) return;
   float v = 0.f;
 #pragma unroll 4
-  for (int b = g; b < blocks; b += 64) v += part[(int64_t)b * 2 * D + e];
+  for (int b = (key ? q_blocks : 0) + g; b < (key ? blocks : q_blocks); b += 64) v += part[(int64_t)b * D + d];
   s[g][c] = v;
   __syncthreads();
   if (g == 0) {
     v = 0.f;
 #pragma unroll
     for (int i = 0; i < 64; ++i) v += s[i][c];
-    void* out = e < D ? dwq : dwk;
-    const int d = e < D ? e : e - D;
-    if (out) {
-      if constexpr (W32) static_cast<float*>(out)[d] = v;
-      else static_cast<uint16_t*>(out)[d] = (uint16_t)pack_bf16(v, 0.f);
-    }
+    if constexpr (W32) static_cast<float*>(out)[d] = v;
+    else static_cast<uint16_t*>(out)[d] = (uint16_t)pack_bf16(v, 0.f);
   }
 }
 
-int64_t grid_of(int64_t T, bool back) {
-  return std::min<int64_t>(cdiv(T, 4), num_cus() * (back ? 4 : 8));
+// Blocks of four waves, a token a wave at a time.
+int64_t forward_blocks(int64_t T) { return std::min<int64_t>(cdiv(T, 4), num_cus() * 8); }
+// As many as run at once, by the kinds' shares of the work.
+struct BackBlocks {
+  int64_t q, k;
+};
+BackBlocks backward_blocks(int64_t T, int64_t H, int64_t Hkv) {
+  const int64_t all = 3 * num_cus(), most = cdiv(T, 4);
+  const int64_t q = std::min(std::max<int64_t>(1, all * H / (H + Hkv)), all - 1);
+  return {std::min(q, most), std::min(all - q, most)};
 }
 
 template <bool BACK>
@@ -357,13 +369,15 @@ extern "C" int tbf16_qk_norm_rope(const void* q, const void* k, int64_t B, int64
   a.yk = (uint16_t*)yk;
   if (int rc = check_norm("qk_norm_rope", a, B, S, H, Hkv, D, R)) return rc;
   if (a.T == 0) return 0;
-  launch_norm<false>(a, grid_of(a.T, false), interleaved, w_f32, as_stream(stream));
+  launch_norm<false>(a, forward_blocks(a.T), interleaved, w_f32, as_stream(stream));
   TB_LAUNCH_CHECK("qk_norm_rope");
   return 0;
 }
 
-extern "C" size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t D) {
-  return B > 0 && S > 0 && D > 0 && (double)B * (double)S < 2147483648.0 ? (size_t)grid_of(B * S, true) * 2 * (size_t)D * 4 : 0;
+extern "C" size_t tbf16_qk_norm_rope_bwd_ws_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D) {
+  if (B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || (double)B * (double)S >= 2147483648.0) return 0;
+  const BackBlocks n = backward_blocks(B * S, H, Hkv);
+  return (size_t)(n.q + n.k) * (size_t)D * 4;
 }
 
 extern "C" int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const void* dyk, int64_t B, int64_t S,
@@ -383,21 +397,23 @@ extern "C" int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* 
   a.part = weights ? (float*)ws : nullptr;
   if (int rc = check_norm("qk_norm_rope_bwd", a, B, S, H, Hkv, D, R)) return rc;
   TB_CHECK(aligned4(dwq) && aligned4(dwk), "qk_norm_rope_bwd: misaligned pointer");
-  const int64_t blocks = grid_of(a.T, true);
-  if (weights && blocks > 0 && (ws == nullptr || ws_bytes < (int64_t)tbf16_qk_norm_rope_bwd_ws_bytes(B, S, D))) {
-    set_error("qk_norm_rope_bwd: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes,
-              tbf16_qk_norm_rope_bwd_ws_bytes(B, S, D));
+  const BackBlocks n = a.T > 0 ? backward_blocks(a.T, H, Hkv) : BackBlocks{0, 0};
+  const size_t need = tbf16_qk_norm_rope_bwd_ws_bytes(B, S, H, Hkv, D);
+  if (weights && need && (ws == nullptr || ws_bytes < (int64_t)need)) {
+    set_error("qk_norm_rope_bwd: workspace too small (%lld bytes, needs %zu)", (long long)ws_bytes, need);
     return TBF16_EWS;
   }
+  a.q_blocks = (int)n.q;
   const hipStream_t st = as_stream(stream);
   if (a.T > 0) {
-    launch_norm<true>(a, blocks, interleaved, w_f32, st);
+    launch_norm<true>(a, n.q + n.k, interleaved, w_f32, st);
     TB_LAUNCH_CHECK("qk_norm_rope_bwd");
   }
   if (weights) {  // (without tokens: zeros)
-    const unsigned grid = (unsigned)(2 * D / 16);
-    if (w_f32) norm_rope_weights_kernel<true><<<grid, 1024, 0, st>>>(a.part, (int)blocks, (int)D, dwq, dwk);
-    else norm_rope_weights_kernel<false><<<grid, 1024, 0, st>>>(a.part, (int)blocks, (int)D, dwq, dwk);
+    const dim3 grid((unsigned)(D / 16), 2);
+    const int blocks = (int)(n.q + n.k);
+    if (w_f32) norm_rope_weights_kernel<true><<<grid, 1024, 0, st>>>(a.part, a.q_blocks, blocks, (int)D, dwq, dwk);
+    else norm_rope_weights_kernel<false><<<grid, 1024, 0, st>>>(a.part, a.q_blocks, blocks, (int)D, dwq, dwk);
     TB_LAUNCH_CHECK("qk_norm_rope_bwd weights");
   }
   return 0;

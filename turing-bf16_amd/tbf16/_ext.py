@@ -67,7 +67,7 @@ _SIGS = {
     "tbf16_linear_i8_ws_bytes": (SZ, [I64, I64, I64]),
     "tbf16_linear_i8": (I, [P, I64, I64, I64, P, I64, I64, P, P, P, I64, P, I64, P]),
     "tbf16_qk_norm_rope": (I, [P, P] + [I64] * 11 + [P, P, I, P, P, I64, I64, P, I64, I64, F, I, P, P, P]),
-    "tbf16_qk_norm_rope_bwd_ws_bytes": (SZ, [I64] * 3),
+    "tbf16_qk_norm_rope_bwd_ws_bytes": (SZ, [I64] * 5),
     "tbf16_qk_norm_rope_bwd": (I, [P] * 4 + [I64] * 17 + [P, P, I, P, P, I64, I64, P, I64, I64, F, I] + [P] * 5 + [I64, P]),
     "tbf16_paged_write": (I, [P, P] + [I64] * 7 + [P, P, P] + [I64] * 8 + [P]),
     "tbf16_paged_advance_ws_bytes": (SZ, [I64] * 2),

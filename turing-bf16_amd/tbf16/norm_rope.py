@@ -110,7 +110,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interl
     return yq, yk
 
 
-# tbf16_qk_norm_rope_bwd's workspace bytes per (device, B, S, D): its blocks are counted by the device's
+# tbf16_qk_norm_rope_bwd's workspace bytes per (device, B, S, H, Hkv, D): its blocks are counted by the device's
 # CUs, so it is asked on the tensors' device, once
 _WS_BYTES: dict = {}
 
@@ -139,7 +139,7 @@ def backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dy
     dwk = torch.empty_like(kept[1]) if want_wk else None
     ws, wsb = None, 0
     if want_wq or want_wk:
-        wsb = _ws_bytes(dev, sizes[0], sizes[1], sizes[4])
+        wsb = _ws_bytes(dev, *sizes)
         ws = q.new_empty(wsb, dtype=torch.uint8)
     q, at_q, q_st = _heads(q)
     k, at_k, k_st = _heads(k)

@@ -50,7 +50,7 @@ def check(dev, table, lengths, counts, stack, n_free, page, tokens, prefix=None,
 
 @pytest.mark.parametrize("B,n,page,tokens", [(1, 1, 1, 3), (1, 5, 16, 40), (5, 4, 3, 30), (64, 10, 16, 70), (70, 3, 1, 100),
                                              (1030, 4, 16, 2500), (2048, 3, 48, 6000), (2049, 3, 48, 4096), (3000, 2, 16, 5000),
-                                             (33, 300, 16, 9000)])
+                                             (33, 300, 16, 9000), (2500, 2, 16, 1500)])
 @pytest.mark.parametrize("spare", [0, 7, 10 ** 4])
 def test_steps(dev, B, n, page, tokens, spare):
     """Several steps of mixed counts: growth, shrinking, ends, idle ones; too few pages and rows."""
@@ -62,7 +62,7 @@ def test_steps(dev, B, n, page, tokens, spare):
         n_free = check(dev, table, lengths, counts, stack, n_free, page, tokens, step * 100 if step else None, n, wide=step % 2 * 3)
 
 
-@pytest.mark.parametrize("B,most,tokens", [(1, 3000, 3000), (40, 200, 9000), (1500, 9, 9000), (2500, 3, 9000), (300, 13, 4096)])
+@pytest.mark.parametrize("B,most,tokens", [(1, 3000, 3000), (1, 2000, 2000), (1, 70000, 70000), (40, 200, 9000), (1500, 9, 9000), (2500, 3, 9000), (300, 13, 4096)])
 def test_back_again(dev, B, most, tokens):
     r = random.Random(B)
     table, lengths, stack, n_free = state(r, B, -(-(2000 + most) // 16), 16, B * (most // 16 + 2), longest=2000)
@@ -123,9 +123,9 @@ def test_large_batch(dev):
 
 def test_graph_of_steps(dev):
     """Captured once, replayed with other counts; both forms (in one launch, in two)."""
-    for B, tokens in ((20, 300), (20, 5000)):
+    for B, tokens in ((20, 300), (20, 5000), (2100, 600)):
         r = random.Random(3)
-        table, lengths, stack, n_free = state(r, B, 8, 16, 60)
+        table, lengths, stack, n_free = state(r, B, 8, 16, 60 * B)
         t, ln, fr, nf = put(dev, table, lengths, stack, n_free, 8)
         c = torch.zeros(B, dtype=torch.int32, device=dev)
         s = torch.cuda.Stream()

@@ -13,9 +13,10 @@
 // token finds its page there by itself, and the page's first token writes the table entry.
 //
 // Nothing here is bound by memory or arithmetic: a chain of dependent steps (lengths, sums over the
-// batch, search, page id) of about a microsecond each, 3.4 us in all for 64 sequences; prompts of 65536 tokens in
-// all take 9.8.
+// batch, search, page id) of about a microsecond each, 3.5 us in all for 64 sequences; 32 prompts of 65536 tokens
+// together take 9.9.
 #include <algorithm>
+#include <type_traits>
 
 #include "abi_util.h"
 #include "common.h"
@@ -83,7 +84,8 @@ __device__ __forceinline__ Want want(const AdvanceArgs& a, int b) {
   return w;
 }
 
-// Slot and position of token t, with starts, base and first wherever they are.
+// Slot and position of token t, with starts, base and first wherever they are. (Several tokens a thread with
+// their loads under way together were 0.7 us slower at 2000 and at 4000 tokens.)
 __device__ __forceinline__ void token(const AdvanceArgs& a, int t, const int32_t* starts, const int32_t* base,
                                       const int32_t* first, int top, int prefix) {
   int slot = -1, pos = -1;
@@ -111,13 +113,15 @@ __device__ __forceinline__ void token(const AdvanceArgs& a, int t, const int32_t
 __device__ __forceinline__ int prefix_of(const AdvanceArgs& a) { return a.prefix ? max(*a.prefix, 0) : 0; }
 
 // One block does everything but, with TOKENS false, the tokens: up to kInside of them cost it no more than a second
-// launch does (2000 tokens: 6.7 us, in a launch of their own 7.6; 4000: 7.9 and 7.8; 8000: 10.3 and 7.8). HERE: the
-// batch's sums are kept in LDS (2000 sequences: 9.0 us, in memory 10.5), as far as it goes.
-constexpr int kHere = 2048, kInside = 4096;
+// launch does (device time of a call and of taking its tokens back, the mean: 2000 tokens 6.2 us, in a launch of
+// their own 6.8; 4000: 7.4 and 6.8; 8000: 9.8 and 6.9). HERE: the batch's sums are kept in LDS (2000 sequences:
+// 9.0 us, in memory 10.5), as far as it goes.
+constexpr int kHere = 2048, kInside = 2048;
 template <bool HERE, bool TOKENS>
 __global__ __launch_bounds__(1024) void paged_advance_kernel(AdvanceArgs a) {
   __shared__ int32_t s_mem[HERE ? 4 * kHere + 4 : 1];
   __shared__ uint32_t s_wave[3][16];
+  __shared__ uint32_t s_real[4][16];
   __shared__ uint32_t s_taken;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
   int32_t* const starts = HERE ? s_mem : a.starts;
@@ -166,28 +170,45 @@ __global__ __launch_bounds__(1024) void paged_advance_kernel(AdvanceArgs a) {
   // entries given back, from the last one on
   if (sum_rel) {
     uint32_t pushed = 0;
-    for (uint32_t i0 = 0; i0 < sum_rel; i0 += nt) {
-      const uint32_t i = i0 + tid;
-      int id = -1;
-      if (i < sum_rel) {
-        const int at = (int)(sum_rel - 1 - i), b = last_upto(rel, a.B, at);
-        int32_t* entry = a.table + b * a.t_sb + pages_of(a, base[b]) + (at - rel[b]);
-        id = *entry;
-        *entry = -1;
+    // (entries a thread has under way: one for few; four where ~4000 pages come and go, 10.4 -> 9.7 us as above)
+    auto give_back = [&](auto under_way) {
+      constexpr int U = decltype(under_way)::value;
+      for (uint32_t i0 = 0; i0 < sum_rel; i0 += U * nt) {
+        int id[U];
+        int32_t* entry[U];
+        uint64_t real[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t i = i0 + u * nt + tid;
+          id[u] = -1;
+          entry[u] = nullptr;
+          if (i >= sum_rel) continue;
+          const int at = (int)(sum_rel - 1 - i), b = last_upto(rel, a.B, at);
+          entry[u] = a.table + b * a.t_sb + pages_of(a, base[b]) + (at - rel[b]);
+          id[u] = *entry[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (entry[u]) *entry[u] = -1;
+          real[u] = __ballot((uint32_t)id[u] < (uint32_t)a.P);
+          if (lane == 0) s_real[u][wave] = __popcll(real[u]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          uint32_t before = pushed;
+          for (int v = 0; v < waves; ++v) {
+            if (v < wave) before += s_real[u][v];
+            pushed += s_real[u][v];
+          }
+          const uint32_t at = top + before + __popcll(real[u] & ((1ull << lane) - 1));
+          if ((real[u] >> lane & 1) && at < (uint32_t)a.P) a.free[at] = id[u];
+        }
+        __syncthreads();
       }
-      const bool real = (uint32_t)id < (uint32_t)a.P;
-      const uint64_t all = __ballot(real);
-      if (lane == 0) s_wave[0][wave] = __popcll(all);
-      __syncthreads();
-      uint32_t before = pushed;
-      for (int v = 0; v < waves; ++v) {
-        if (v < wave) before += s_wave[0][v];
-        pushed += s_wave[0][v];
-      }
-      const uint32_t at = top + before + __popcll(all & ((1ull << lane) - 1));
-      if (real && at < (uint32_t)a.P) a.free[at] = id;
-      __syncthreads();
-    }
+    };
+    if (sum_rel <= (uint32_t)nt) give_back(std::integral_constant<int, 1>());
+    else give_back(std::integral_constant<int, 4>());
     top = (int)min((uint32_t)top + pushed, (uint32_t)a.P);
   }
 
@@ -274,10 +295,9 @@ extern "C" int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t
   }
   const hipStream_t st = as_stream(stream);
   const bool here = B <= kHere, inside = tokens <= kInside;
-  // Few waves meet sooner at barriers (device time of a call and of taking its tokens back, the mean: 64 sequences, 6
-  // tokens: 256 threads 3.4 us, 1024 4.2; 512 sequences, a token each: 512 threads 4.9, 1024 5.6, 256 7.1).
-  const int64_t most = std::max(B, inside ? tokens : INT32_MAX);
-  const int nt = most <= 256 ? 256 : most <= 1024 ? 512 : 1024;
+  // Few waves meet sooner at barriers (as above; 64 sequences, 6 tokens: 512 threads 3.5 us, 1024 4.2; 512 sequences,
+  // a token each: 4.9 and 5.7; 2000: 10.9 and 9.0).
+  const int nt = std::max(B, inside ? tokens : 0) <= 1024 ? 512 : 1024;
   if (here && inside) paged_advance_kernel<true, true><<<1, nt, 0, st>>>(a);
   else if (here) paged_advance_kernel<true, false><<<1, nt, 0, st>>>(a);
   else if (inside) paged_advance_kernel<false, true><<<1, nt, 0, st>>>(a);

@@ -102,7 +102,7 @@ def test_layouts(dev):
     dq = torch.randn(B, H, S, D, generator=gen(1)).to(BF).to(dev).transpose(1, 2)
     dk = torch.ones((), dtype=BF, device=dev).expand(B, S, Hkv, D)
     want = check((q, k, wq, wk, cos, sin, pos), dys=(dq, dk))
-    for a in ((swap(q), swap(k), wq, wk, cos, sin, pos), (odd, thin, w2, wk, c2, s2, pos),
+    for a in ((swap(q), swap(k), wq, wk, cos, sin, pos), (odd, thin, w2, torch.cat((wk[:1], wk))[1:], c2, s2, pos),
               (q, k, wq, wk, cos, sin, pos.t().contiguous().t())):
         got = check(a, dys=(dq, dk))
         assert all(torch.equal(x, y) for u, v in zip(got, want) for x, y in zip(u, v))

@@ -84,7 +84,7 @@ def _checked(q, k, wq, wk, cos, sin, positions, eps, interleaved):
     if B * S >= 2 ** 31:
         raise ValueError(f"tbf16.qk_norm_rope: {B * S} tokens")
     _device(q, k, wq, wk, cos, sin, positions)
-    wq, wk, cos, sin = wq.contiguous(), wk.contiguous(), _table(cos), _table(sin)
+    wq, wk, cos, sin = _table(wq), _table(wk), _table(cos), _table(sin)
     return ((B, S, shape[-2], kshape[-2], D),
             (wq.data_ptr(), wk.data_ptr(), wide, cos.data_ptr(), sin.data_ptr(), table[0], R, positions.data_ptr(), *p_st, eps,
              bool(interleaved)), (wq, wk, cos, sin))

@@ -10,6 +10,9 @@
 // chunks of 8 elements of a head, chosen so that a pair's elements are in one lane; L lanes
 // make a head, whose sums go through DPP; a wave takes a token's heads, 64 / L at a time, so that
 // cos and sin are read once for all of them and the weights once per wave.
+// 8192 tokens of 40 heads of 128: 34.3 us, 5.0 TB/s; gradient of 8192 tokens of 32 heads: 41 us, 4.9 TB/s, and 4 us
+// for the sums of the weights' (a copy reaches 4.9). 16 tokens: 5.9 us, the position, its angles and the store after
+// one another.
 #include <float.h>
 
 #include <algorithm>
@@ -164,7 +167,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormArgs a) {
   const int i = lane % L, hl = lane / L;
   const Item<NEAR> it(i, a.D, a.R);
   // Forward: query heads, then key heads, in steps of HPW. Gradient: one kind a block, whose registers then
-  // hold one set of weights and of their gradients (189 -> 153 registers, three waves a SIMD instead of two).
+  // hold one set of weights and of their gradients (189 -> 151 registers, three waves a SIMD instead of two: 56 -> 41
+  // us for 8192 tokens of 32 heads).
   const int sq = (a.H + HPW - 1) / HPW, sk = (a.Hkv + HPW - 1) / HPW;
   const bool key_block = BACK && (int)blockIdx.x >= a.q_blocks;
   int begin = key_block ? sq : 0, steps = BACK && !key_block ? sq : sq + sk;

@@ -4,8 +4,9 @@
 // o = softmax of the logits of prefix keys and own keys together, times their values. Any split of the keys into
 // parts gives (m, l, o) with o = sum_j 2^(x_j - m) v_j and l = sum_j 2^(x_j - m), and parts join as
 //   m = max m_i,   l = sum l_i 2^(m_i - m),   o = sum o_i 2^(m_i - m).
-// Two launches: the prefix beside the sequences' own keys (prefix_kernel: blocks of either kind, the latter
-// attn_block of paged_attn.h, which leaves sums instead of outputs), and the join of all parts of a row.
+// Two launches: the prefix and behind it, in blocks of the same launch, the sequences' own keys (prefix_kernel; the
+// latter attn_block of paged_attn.h, which leaves sums instead of outputs), and the join of all parts of a row.
+// (The prefix's blocks first: in turns with the others they share CUs unevenly, 101 -> 136 us alone.)
 #include <cmath>
 #include <type_traits>
 
@@ -53,6 +54,14 @@ __device__ __forceinline__ int prefix_len(const int32_t* length, int cap) { retu
 // row's weights refer to follows its largest logit only in steps of 2^8 (weights then reach 2^8 of the last
 // step's; they carry 2^-16, so that sums have the room that paged_attn.h's have). Weights go into the second product as
 // the sum of two bf16: 8 bits, and the next 9 rounded to nearest.
+//
+// Bound by its instructions where the batch is large: 64 keys and 32 rows of D = 128 are 96 MFMAs, ~ 290 vector
+// instructions and 32 exponentials a wave, two units that overlap in part. 128 sequences of 32 heads on 8 key heads,
+// 32768 keys: 101 us alone with two blocks a CU (680 TFLOPS of the two products as defined, 1020 with the weights'
+// second part), 117 with one, which leaves half of the CU to the own keys' blocks: with up to 1024 of those a sequence
+// a call takes 150 us, with two blocks a CU 160. Where it is small, by a chain: length, page ids, keys, products,
+// parts (4 sequences of 16 heads on 700 keys: 6.7 us). Eight waves on 256 rows in one block were as fast (98 us alone,
+// more with own keys). One bf16 a weight: 168 -> 149 us a call, for outputs with twice the squared error.
 //
 // LDS: chunk c of 16 bytes of row r lies at chunk c ^ f(r) of its row, so that the 16 rows that a read of
 // K takes at one chunk lie in all 64 banks, and so do the two chunks of 8 rows that a transposed read takes.
@@ -429,7 +438,8 @@ struct JoinArgs {
   uint16_t* o;
 };
 
-// 64 groups of 4 outputs a block; its waves take a row's parts in turns and meet in LDS.
+// 64 groups of 4 outputs a block; its waves take a row's parts in turns and meet in LDS (16 parts of 4096 rows:
+// eight waves 15.4 us, four 13.2, two 12.7; 5 to 11 parts of few rows 4.2 to 4.5 us either way).
 constexpr int kMeet = 4;
 __global__ __launch_bounds__(kMeet * 64) void prefix_join_kernel(JoinArgs j) {
   __shared__ float4 so[kMeet][64];

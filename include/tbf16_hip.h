@@ -318,8 +318,8 @@ int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D
 
 /* tbf16_paged_attn where all sequences begin with the same tokens: keys are positions j <
  * *prefix_length of prefix_table int32 (prefix_pages,) and then positions j < lengths[b] of the
- * sequence's own table, in one softmax. The prefix is read once for the batch. B * H below 1e9. Other
- * arguments and limits as tbf16_paged_attn's; the size query takes prefix_pages * page and max_pages
+ * sequence's own table, in one softmax. The prefix is read once for the batch. B * H below 1e9,
+ * B * H * D below 2^32 - 256. Other arguments and limits as tbf16_paged_attn's; the size query takes prefix_pages * page and max_pages
  * * page. Weights of prefix keys below 2^-80 of the row's largest may count as zero. No counterpart in
  * the reference. */
 size_t tbf16_paged_attn_prefix_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_positions,

@@ -248,3 +248,14 @@ def test_prefix_abi_refusals():
     assert call(B=0) == 0
     small, large = (L.tbf16_paged_attn_prefix_ws_bytes(B, 32, 8, 128, 4096, 512) for B in (1, 64))
     assert 0 < small < large and L.tbf16_paged_attn_prefix_ws_bytes(0, 32, 8, 128, 4096, 512) == 0
+
+
+def test_prefix_abi_more_outputs_than_a_launch_counts():
+    """The join has 256 threads for 64 groups of four outputs, and a launch fewer than 2^32 threads."""
+    L = _ext.lib()
+    for B, H, D in ((2 ** 29 // 256, 256, 8), (2 ** 25 // 4, 4, 128), (2 ** 24 // 2, 2, 256)):
+        assert L.tbf16_paged_attn_prefix_ws_bytes(B - 1, H, H, D, 64, 64) > 0
+        assert L.tbf16_paged_attn_prefix_ws_bytes(B, H, H, D, 64, 64) == 0
+        assert L.tbf16_paged_attn_prefix(16, B, H, H, D, H * D, D, 16, 16, 4, 16, 16 * H * D, 16 * D, D, 16 * H * D, 16 * D, D,
+                                         16, 4, 16, 16, 4, 4, 16, 1.0, 16, 16, 1 << 60, None) == -1
+        assert "large" in L.tbf16_last_error().decode()

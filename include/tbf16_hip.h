@@ -319,9 +319,9 @@ int tbf16_paged_attn(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D
 /* tbf16_paged_attn where all sequences begin with the same tokens: keys are positions j <
  * *prefix_length of prefix_table int32 (prefix_pages,) and then positions j < lengths[b] of the
  * sequence's own table, in one softmax. The prefix is read once for the batch. B * H below 1e9,
- * B * H * D below 2^32 - 256. Other arguments and limits as tbf16_paged_attn's; the size query takes prefix_pages * page and max_pages
- * * page. Weights of prefix keys below 2^-80 of the row's largest may count as zero. No counterpart in
- * the reference. */
+ * B * H * D at most 2^32 - 256. Other arguments and limits as tbf16_paged_attn's; the size query takes
+ * prefix_pages * page and max_pages * page. Weights of prefix keys below 2^-80 of the row's largest may
+ * count as zero. No counterpart in the reference. */
 size_t tbf16_paged_attn_prefix_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_positions,
                                         int64_t positions);
 int tbf16_paged_attn_prefix(const void* q, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t q_sb, int64_t q_sh,
@@ -367,9 +367,9 @@ int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const 
  * tokens begin, at most tokens. slots, positions int32 (tokens,): page id * page + row, old length +
  * i + *prefix (0 if NULL), or -1 both for tokens that were not granted or are not there; a slot is -1
  * too where the table names no page. B * max_pages and pages * page below 2^31. No two arrays
- * overlap. ws: tbf16_paged_advance_ws_bytes(B, tokens) bytes, this call's alone until it has run (0 for
- * small batches, ws may then be NULL). No
- * counterpart in the reference. */
+ * overlap, and no two entries of table name one page (given back, it goes on the stack twice). ws:
+ * tbf16_paged_advance_ws_bytes(B, tokens) bytes, this call's alone until it has run (0 for small
+ * batches, ws may then be NULL). No counterpart in the reference. */
 size_t tbf16_paged_advance_ws_bytes(int64_t B, int64_t tokens);
 int tbf16_paged_advance(int32_t* table, int64_t table_stride, int64_t B, int64_t max_pages, int32_t* lengths,
                         const int32_t* counts, int32_t* free_pages, int64_t pages, int32_t* n_free, int64_t page,

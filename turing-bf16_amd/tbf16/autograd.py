@@ -454,7 +454,9 @@ class QKNormRopeFn(torch.autograd.Function):
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):
     """Differentiable tbf16.qk_norm_rope: gradients of q, k (bf16) and both weights (their own type), sums
     over tokens and heads in fp32 in a fixed order. Tokens of a negative position have no share in
-    any. cos, sin and positions are constants."""
+    any. cos, sin and positions are constants. Can be captured into a graph with its backward pass, as
+    long as no autograd graph made outside of the capture still holds the same leaves: torch would
+    add up their gradients on the stream that one came from."""
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("tbf16.autograd.qk_norm_rope: no gradients of cos and sin")
     return QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)

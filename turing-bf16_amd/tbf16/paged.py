@@ -84,7 +84,8 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     says where the new tokens belong: (slots, positions, starts), int32 (tokens,), (tokens,) and
     (B + 1,). All on the device, in place, without waiting for it:
 
-      page_table  int32 (B, n): sequence b's pages; lengths int32 (B,): its tokens so far
+      page_table  int32 (B, n): sequence b's pages, each of which no other entry names (a page that
+                  two entries give back goes on the stack twice); lengths int32 (B,): its tokens so far
       counts      int32 (B,): new tokens (0: none); negative: the last -counts[b] tokens are taken
                   back, all of them where there are fewer (a request that ends: -lengths[b])
       free_pages  int32 (pages,): a stack of the pages that nobody has, n_free int32 (1,) of them, the
@@ -254,7 +255,7 @@ def paged_sdpa_prefix(q, k_cache, v_cache, prefix_table, prefix_length, page_tab
     all of them ask about): positions j < prefix_length[0] of prefix_table int32 (m,), int32 (1,), come
     before each sequence's own positions j < lengths[b] of page_table. The prefix's keys and values
     are read once for the whole batch and multiplied with all its queries. One softmax over both:
-    the result is paged_sdpa's on tables that begin with prefix_table's pages.
+    the result is paged_sdpa's on sequences that hold the prefix's tokens before their own.
 
     Arguments, results and limits as paged_sdpa's; a sequence without any key gives zeros. Weights of
     prefix keys enter the second product with 16 bits, and below 2^-80 of the row's largest may count

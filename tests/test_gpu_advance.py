@@ -142,3 +142,35 @@ def test_graph_of_steps(dev):
             n_free, *want = advance_by_hand(table, lengths, counts, stack, n_free, 16, tokens)
             assert [x.tolist() for x in out] == want and nf.item() == n_free
             assert t.tolist() == table and ln.tolist() == lengths and fr.tolist() == stack
+
+
+def test_page_named_twice(dev):
+    """Two entries of one page, a page that is on the stack already: in bounds, each given back as it stands."""
+    check(dev, [[3, 3], [3, -1]], [8, 4], [-8, -4], [4, 0, 0, 0, 0], 1, 4, 5)
+    check(dev, [[1, 1, 1], [1, 1, 1]], [12, 12], [-12, -5], [0, 1, 2, 3], 2, 4, 5)
+    check(dev, [[1, 1, 1], [1, 1, 1], [2, -1, -1]], [12, 12, 1], [-12, -5, 11], [0, 0, 0, 0, 0], 1, 4, 12)
+
+
+def test_two_at_once(dev):
+    """Batches of their own on two streams, with and without a workspace."""
+    r = random.Random(8)
+    runs = []
+    for B, tokens in ((700, 1500), (2300, 9000)):
+        table, lengths, stack, n_free = state(r, B, 6, 16, 3 * B)
+        runs.append([put(dev, table, lengths, stack, n_free, 6), (table, lengths, stack), n_free, tokens, torch.cuda.Stream()])
+    for _ in range(6):
+        calls = []
+        for t, (table, lengths, stack), n_free, tokens, s in runs:
+            counts = [r.choice((0, 1, 5, -3, -200)) for _ in table]
+            calls.append((counts, torch.tensor(counts, dtype=torch.int32, device=dev)))
+        torch.cuda.synchronize()
+        outs = []
+        for (t, _, _, tokens, s), (_, c) in zip(runs, calls):
+            with torch.cuda.stream(s):
+                outs.append(tbf16.paged_advance(t[0], t[1], c, t[2], t[3], 16, tokens))
+        torch.cuda.synchronize()
+        for run, (counts, _), out in zip(runs, calls, outs):
+            t, by_hand, n_free, tokens, _ = run
+            run[2], *want = advance_by_hand(*by_hand[:2], counts, by_hand[2], n_free, 16, tokens)
+            assert [x.tolist() for x in out] == want and t[3].item() == run[2]
+            assert [x.tolist() for x in t[:3]] == list(by_hand)

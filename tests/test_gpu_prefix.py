@@ -274,3 +274,23 @@ def test_graph(dev, capacity):
         torch.cuda.synchronize()
         got = o.clone()
         assert torch.equal(got, check(a))
+
+
+def test_two_graphs_of_one_pool(dev):
+    """Graphs whose workspaces lie in the same memory, replayed in turns."""
+    both = [make(dev, 900, [b * 5 % 100 for b in range(20)], 8, 2, 128, 16, seed=15),
+            make(dev, 300, [b * 7 % 90 for b in range(33)], 16, 4, 64, 16, seed=16)]
+    want = [check(a) for a in both]
+    s = torch.cuda.Stream()
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for a in both:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s, pool=graphs[0].pool() if graphs else None):
+            outs.append(tbf16.paged_sdpa_prefix(*a))
+        graphs.append(g)
+    for _ in range(4):
+        for g, o, w, a in zip(graphs, outs, want, both):
+            o.zero_()
+            g.replay()
+            assert torch.equal(o, w) and torch.equal(tbf16.paged_sdpa_prefix(*a), w)

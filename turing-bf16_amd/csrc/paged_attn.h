@@ -96,6 +96,21 @@ __device__ __forceinline__ int seq_len(const AttnArgs& a, int b) { return min(ma
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Two weights as the sum of three bf16 each, packed: the leading 8 of their bits, the next ones and the last.
+__device__ __forceinline__ void weight_parts(float p0, float p1, uint32_t (&f)[3][4], int j) {
+#pragma unroll
+  for (int t = 0; t < 3; ++t) {
+    f[t][j] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
+    p0 -= bf16_hi(__float_as_uint(p0));
+    p1 -= bf16_hi(__float_as_uint(p1));
+  }
+  // 2^-28 of p in place of a part that is zero: an infinite value times it stays infinite
+  const ushort2v least = __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, f[0][j]), ushort2v{28 << 7, 28 << 7});
+#pragma unroll
+  for (int t = 1; t < 3; ++t)
+    f[t][j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, f[t][j]), least));
+}
+
 // A place in the list: tile `tile` of nt of a unit, the grp-th group of R rows of key/value head
 // `head` of sequence b.
 struct Cursor {
@@ -478,22 +493,12 @@ __device__ __forceinline__ void attn_block(const AttnArgs& a, Rows rows_of, floa
           acc.scale(r, ex2(acc.m[r] - mn));
           acc.m[r] = mn;
         }
-        uint32_t f[3][4];  // p's leading 8 bits, the next ones and the last
+        uint32_t f[3][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float p0 = ex2(x[2 * j] - acc.m[r]) * kWeight, p1 = ex2(x[2 * j + 1] - acc.m[r]) * kWeight;
+          const float p0 = ex2(x[2 * j] - acc.m[r]) * kWeight, p1 = ex2(x[2 * j + 1] - acc.m[r]) * kWeight;
           acc.l[r] += p0 + p1;
-#pragma unroll
-          for (int t = 0; t < 3; ++t) {
-            f[t][j] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
-            p0 -= bf16_hi(__float_as_uint(p0));
-            p1 -= bf16_hi(__float_as_uint(p1));
-          }
-          // 2^-28 of p in place of a part that is zero: an infinite value times it stays infinite
-          const ushort2v least = __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, f[0][j]), ushort2v{28 << 7, 28 << 7});
-#pragma unroll
-          for (int t = 1; t < 3; ++t)
-            f[t][j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, f[t][j]), least));
+          weight_parts(p0, p1, f, j);
         }
 #pragma unroll
         for (int t = 0; t < 3; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));

@@ -52,16 +52,17 @@ __device__ __forceinline__ int prefix_len(const int32_t* length, int cap) { retu
 // S^T = K Q^T on v_mfma_f32_16x16x32_bf16: lane l gets keys 4 (l / 16) .. + 3 of each 16-key block for row l % 16,
 // which are its k slots of O^T = V^T P^T; V^T comes from the row-major tile by ds_read_b64_tr_b16. The maximum a
 // row's weights refer to follows its largest logit only in steps of 2^8 (weights then reach 2^8 of the last
-// step's; they carry 2^-16, so that sums have the room that paged_attn.h's have). Weights go into the second product as
-// the sum of two bf16: 8 bits, and the next 9 rounded to nearest.
+// step's; they carry 2^-16, so that sums have the room that paged_attn.h's have). Weights go into the second product with all
+// their 24 bits, as the sum of three bf16. (Two of them, 8 bits and the next ones rounded to 8, take 151 us where three
+// take 180, for 2012 of 524288 outputs rounded other than the exact value instead of 468; fp32 products: 1014.)
 //
-// Bound by its instructions where the batch is large: 64 keys and 32 rows of D = 128 are 96 MFMAs, ~ 290 vector
+// Bound by its instructions where the batch is large: 64 keys and 32 rows of D = 128 are 128 MFMAs, ~ 420 vector
 // instructions and 32 exponentials a wave, two units that overlap in part. 128 sequences of 32 heads on 8 key heads,
 // 32768 keys: 101 us alone with two blocks a CU (680 TFLOPS of the two products as defined, 1020 with the weights'
 // second part), 117 with one, which leaves half of the CU to the own keys' blocks: with up to 1024 of those a sequence
 // a call takes 150 us, with two blocks a CU 160. Where it is small, by a chain: length, page ids, keys, products,
 // parts (4 sequences of 16 heads on 700 keys: 6.7 us). Eight waves on 256 rows in one block were as fast (98 us alone,
-// more with own keys). One bf16 a weight: 168 -> 149 us a call, for outputs with twice the squared error.
+// more with own keys).
 //
 // LDS: chunk c of 16 bytes of row r lies at chunk c ^ f(r) of its row, so that the 16 rows that a read of
 // K takes at one chunk lie in all 64 banks, and so do the two chunks of 8 rows that a transposed read takes.
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
   typedef __attribute__((address_space(3))) v4s lds_v4s;
 
   typedef floatx4 Logits[2][RB];
-  typedef bf16x8 Weights[RB][2];
+  typedef bf16x8 Weights[RB][3];
   // 32 keys at a time: logits, ...
   auto logits = [&](const uint8_t* stage, int kl, int h, Logits& s) {
 #pragma unroll
@@ -220,19 +221,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const float mo = m[r] + 2 * kLag;
-      uint32_t f[2][4];
+      uint32_t f[3][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const floatx4& sv = s[j >> 1][r];
         const float p0 = ex2(fmaf(sv[2 * (j & 1)], cc, -mo)), p1 = ex2(fmaf(sv[2 * (j & 1) + 1], cc, -mo));
         l[r] += p0 + p1;
-        f[0][j] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
-        // the rest, and 2^-22 of p so that it is never zero: an infinite value times it stays infinite
-        f[1][j] = pack_bf16(fmaf(p0, 0x1.000004p0f, -bf16_hi(__float_as_uint(p0))),
-                            fmaf(p1, 0x1.000004p0f, -bf16_hi(__float_as_uint(p1))));
+        weight_parts(p0, p1, f, j);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));
+      for (int t = 0; t < 3; ++t) pf[r][t] = __builtin_bit_cast(bf16x8, make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]));
     }
   };
   // ... and outputs; live: the keys that there are
@@ -254,7 +252,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
 #pragma unroll
       for (int r = 0; r < RB; ++r)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][t], o[r][d], 0, 0, 0);
+        for (int t = 0; t < 3; ++t) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r][t], o[r][d], 0, 0, 0);
     }
   };
   // A whole tile, from a stage that the next loads must not go into yet. (They go out behind the first reads: where

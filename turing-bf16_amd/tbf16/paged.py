@@ -258,8 +258,7 @@ def paged_sdpa_prefix(q, k_cache, v_cache, prefix_table, prefix_length, page_tab
     the result is paged_sdpa's on sequences that hold the prefix's tokens before their own.
 
     Arguments, results and limits as paged_sdpa's; a sequence without any key gives zeros. Weights of
-    prefix keys enter the second product with 16 bits, and below 2^-80 of the row's largest may count
-    as zero (an infinite value then gives NaN)."""
+    prefix keys below 2^-80 of the row's largest may count as zero (an infinite value then gives NaN)."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa_prefix", k_cache, v_cache)
     _same_device("paged_sdpa_prefix", k_cache, v_cache, q, prefix_table, prefix_length, page_table, lengths)
     q, q_st, page_table, lengths = _queries("paged_sdpa_prefix", q, k_cache.shape, page_table, lengths)

@@ -117,3 +117,60 @@ def test_weights_keep_their_bits(dev, B, H, Hkv, D, n, first, second):
     ref = torch.tanh(-step / 2)[..., None].expand(B, H, D)
     assert (ref.abs() < 2.0 ** -13).all()
     assert ((o - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -19).all(), (o - ref).abs().max() * 2.0 ** 19
+
+
+def near_the_top(g, Hkv, n, sign):
+    """Of n logits most differ from the largest, 2^23, by up to 7, some are zero."""
+    z = sign * (2 ** 23 - 1 - torch.randint(0, 8, (Hkv, n), generator=g))
+    return torch.where(torch.rand(Hkv, n, generator=g) < 0.1, 0 if sign > 0 else -2 ** 23, z)
+
+
+@pytest.mark.parametrize("B,H,Hkv,D", FORMS)
+@pytest.mark.parametrize("power,scale", [(-16, 1.0), (-13, 0.7), (-10, 1.0), (-4, 1.0), (-1, 1.0), (0, 1.0), (3, 1.0), (4, 0.09), (5, 1.0),
+                                         (8, -1.0), (20, 1.0), (40, 0.125), (103, 1.0), (103, 1e-30), (0, 0.0)])
+def test_large_logits(dev, B, H, Hkv, D, power, scale):
+    """Logits up to 2^126 of which many are equal or neighbours, in the prefix and among the own keys: the same
+    weights wherever a key lies, as paged_sdpa gives on tables that hold all of them."""
+    g = gen(power + D)
+    sign = -1 if power == 4 else 1
+    far = near_the_top(g, Hkv, 208, sign)
+    own = [near_the_top(g, Hkv, b % 40, sign) for b in range(B)]
+    a = make(dev, far, own, H, D, 16, power, seed=D)
+    ref, bound = expected(a, far, own, power, scale)
+    close(tbf16.paged_sdpa_prefix(*a, scale=scale), ref, bound)
+    q, k, v, table, _, tables, lengths = a
+    close(tbf16.paged_sdpa(q, k, v, torch.cat((table.expand(B, -1), tables), 1), lengths + 208, scale=scale), ref, bound)
+
+
+@pytest.mark.parametrize("B,H,Hkv,D", FORMS)
+@pytest.mark.parametrize("step", [1, 16, 3 * 64, 40 * 64, 8000])
+@pytest.mark.parametrize("falling", [False, True])
+def test_maximum_that_moves(dev, B, H, Hkv, D, step, falling):
+    """Logits that grow or fall by 1/64 to 125 from key to key."""
+    j = torch.arange(1000).expand(Hkv, 1000)
+    far = (999 - j if falling else j) * step
+    own = [torch.randint(990 * step, 1001 * step, (Hkv, b % 7), generator=gen(b)) for b in range(B)]
+    a = make(dev, far, own, H, D, 16, power=-6, seed=step)
+    close(tbf16.paged_sdpa_prefix(*a, scale=1.0), *expected(a, far, own, -6, 1.0))
+
+
+@pytest.mark.parametrize("B,H,Hkv,D", FORMS)
+@pytest.mark.parametrize("power", [-16, 2, 6, 60])
+def test_largest_values_at_large_logits(dev, B, H, Hkv, D, power):
+    """Equal logits of any size with values near the type's largest: their sum has room."""
+    far = torch.full((Hkv, 150), 2 ** 23 - 1)
+    own = [torch.full((Hkv, b % 5), 2 ** 23 - 1) for b in range(B)]
+    a = make(dev, far, own, H, D, 16, power)
+    a[2].masked_fill_(~torch.isnan(a[2]), 3e38)
+    close(tbf16.paged_sdpa_prefix(*a, scale=1.0), *expected(a, far, own, power, 1.0))
+
+
+@pytest.mark.parametrize("B,H,Hkv,D", FORMS)
+def test_large_tables_of_small_logits_and_one_large(dev, B, H, Hkv, D):
+    """A key of 2^30 far behind 300 small ones, and before them."""
+    for at in (299, 64, 0):
+        far = torch.randint(0, 2 ** 10, (Hkv, 300), generator=gen(at))
+        far[:, at] = 2 ** 23 - 1
+        own = [torch.randint(0, 2 ** 10, (Hkv, b % 9), generator=gen(b)) for b in range(B)]
+        a = make(dev, far, own, H, D, 16, power=7)
+        close(tbf16.paged_sdpa_prefix(*a, scale=1.0), *expected(a, far, own, 7, 1.0))

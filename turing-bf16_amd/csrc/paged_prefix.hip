@@ -52,7 +52,11 @@ __device__ __forceinline__ int prefix_len(const int32_t* length, int cap) { retu
 // S^T = K Q^T on v_mfma_f32_16x16x32_bf16: lane l gets keys 4 (l / 16) .. + 3 of each 16-key block for row l % 16,
 // which are its k slots of O^T = V^T P^T; V^T comes from the row-major tile by ds_read_b64_tr_b16. The maximum a
 // row's weights refer to follows its largest logit only in steps of 2^8 (weights then reach 2^8 of the last
-// step's; they carry 2^-16, so that sums have the room that paged_attn.h's have). Weights go into the second product with all
+// step's; they carry 2^-16, so that sums have the room that paged_attn.h's have). It is a whole number, so that the
+// constants added to it and the factors between steps are exact; from 2^22 on it follows at once. Logits are rounded
+// products and 2^-16 a factor, as in paged_attn.h: a key has the same weight in the prefix and among the own ones however
+// large they are (the product, the difference and 2^-16 in one operation: 180 us a call below instead of 184, and from
+// logits of 2^27 on weights that are off by their size). Weights go into the second product with all
 // their 24 bits, as the sum of three bf16. (Two of them, 8 bits and the next ones rounded to 8, take 151 us where three
 // take 180, for 2012 of 524288 outputs rounded other than the exact value instead of 468; fp32 products: 1014.)
 //
@@ -75,11 +79,20 @@ __device__ __forceinline__ int swz(int row) {
 constexpr int kIds = 2048;  // page ids a block holds at a time
 // rows of a unit of own keys
 constexpr int own_rows(int DP) { return DP == 256 ? 8 : 16; }
-constexpr float kLag = 8.f;
+// A row's weights refer to a whole number that its logits pass by at most kLag; by nothing beyond kNear, up to where kLag
+// can be added to it exactly.
+constexpr float kLag = 8.f, kNear = 0x1p22f;
 
 typedef __attribute__((address_space(1))) void global_void;
 __device__ __forceinline__ void load16_lds(const void* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((global_void*)from, (lds_void*)to, 16, 0, 0);
+}
+
+// 2^(s c - m - 16), at most 2^(kLag - 16): the product is rounded before the difference, as the maximum's is.
+__device__ __forceinline__ float weight(float s, float c, float m) {
+#pragma clang fp contract(off)
+  const float x = s * c;
+  return ex2(x - m) * 0x1p-16f;
 }
 
 struct LaunchArgs {
@@ -129,11 +142,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
   const float c = fabsf(a.scale_log2);
   bf16x8 qf[RB][KI];
   floatx4 o[RB][DB];
-  float m[RB], l[RB];  // m: what the weights refer to
+  float m[RB], up[RB], l[RB];  // m: what the weights refer to, a whole number; up: the largest logit it serves
   bool fresh = true;
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
-    m[r] = kNone;
+    m[r] = up[r] = kNone;
     l[r] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[r][d] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -198,18 +211,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
     for (int r = 0; r < RB; ++r) {
       mx[r] = fmaxf(fmaxf(fmaxf(fmaxf(s[0][r][0], s[0][r][1]), fmaxf(s[0][r][2], s[0][r][3])), fmaxf(s[1][r][0], s[1][r][1])),
                     fmaxf(s[1][r][2], s[1][r][3])) * cc;
-      grown |= mx[r] > m[r] + kLag;
+      grown |= mx[r] > up[r];
     }
     if (__any(grown)) {
       fresh = false;
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        float mn = fmaxf(mx[r], kFew);
+        float mn = fmaxf(ceilf(mx[r]), kFew);
         mn = fmaxf(mn, __shfl_xor(mn, 16, kWave));
         mn = fmaxf(mn, __shfl_xor(mn, 32, kWave));
         mn = fmaxf(mn, m[r]);
         const float f = ex2(m[r] - mn);
         m[r] = mn;
+        up[r] = fabsf(mn) <= kNear ? mn + kLag : mn;
         l[r] *= f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[r][d] *= f;
@@ -220,12 +234,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
   auto weights = [&](const Logits& s, float cc, Weights& pf) {
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      const float mo = m[r] + 2 * kLag;
       uint32_t f[3][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const floatx4& sv = s[j >> 1][r];
-        const float p0 = ex2(fmaf(sv[2 * (j & 1)], cc, -mo)), p1 = ex2(fmaf(sv[2 * (j & 1) + 1], cc, -mo));
+        const float p0 = weight(sv[2 * (j & 1)], cc, m[r]), p1 = weight(sv[2 * (j & 1) + 1], cc, m[r]);
         l[r] += p0 + p1;
         weight_parts(p0, p1, f, j);
       }
@@ -415,13 +428,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     if (out[r] < 0) continue;
+    // In the terms of paged_attn.h, whose weights are 2^(x - m - 8): the other 2^-8 go to m where that is exact, else to
+    // the sums, whose weights are none above 2^-16 then.
+    const bool near = fabsf(m[r]) <= kNear;
+    const float f = near ? 1.f : 0x1p8f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
       const int at = 16 * d + 4 * g;
-      if (!PAD || at < a.D) *reinterpret_cast<floatx4*>(a.part + out[r] * a.D + at) = o[r][d];
+      if (!PAD || at < a.D) *reinterpret_cast<floatx4*>(a.part + out[r] * a.D + at) = o[r][d] * f;
     }
-    // (in the terms of paged_attn.h, whose weights are 2^(x - m - 8))
-    if (g == 0) *reinterpret_cast<float2*>(a.stat + out[r] * 2) = make_float2(m[r] == kNone ? kNone : m[r] + kLag, l[r]);
+    if (g == 0) *reinterpret_cast<float2*>(a.stat + out[r] * 2) = make_float2(near ? m[r] + kLag : m[r], l[r] * f);
   }
 }
 

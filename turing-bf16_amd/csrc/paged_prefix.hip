@@ -134,7 +134,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void prefix_kernel(LaunchAr
   const int wr = wave % WR, kg = wave / WR;
   // (blocks that read the same keys one behind the other, on one XCD where there are 8 heads)
   const int head = block % a.Hkv, rt = block / a.Hkv % a.tiles, split = block / a.Hkv / a.tiles;
-  const int length = prefix_len(a.length, a.cap);
+  // read once a block: were another stream to write it meanwhile, waves of several lengths would look up page ids that
+  // none of them has loaded
+  if (threadIdx.x == 0) s_flags[0] = prefix_len(a.length, a.cap);
+  __syncthreads();
+  const int length = uniform(s_flags[0]);
   const Splits sp = splits_of(length, KS, a.S);
   const int t0 = split * sp.each, tn = min(sp.each, sp.tiles - t0);
   if (tn <= 0) return;

@@ -205,23 +205,23 @@ def _ws_bytes(dev: int, name: str, *sizes: int) -> int:
     return n
 
 
-def _queries(fn, q, shape, page_table, lengths):
-    """The checked q, page_table and lengths of an attention over a cache of `shape`."""
-    _, Hkv, _, D = shape
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"tbf16.{fn}: q {tuple(q.shape)} is not (B, H, {D})")
+def _queries(fn, q, Hkv, D, page_table, lengths):
+    """(q, its strides, B, H, page_table, its entries a sequence, lengths), checked."""
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"tbf16.{fn}: q {tuple(shape)} is not (B, H, {D})")
     if q.dtype is not torch.bfloat16:
         raise TypeError(f"tbf16.{fn}: expected bf16 q")
-    B, H, _ = q.shape
+    B, H, _ = shape
     if H == 0 or H % Hkv:
         raise ValueError(f"tbf16.{fn}: {H} query heads over {Hkv} key/value heads")
     page_table = _index(fn, "page_table", page_table, 2)
     lengths = _index(fn, "lengths", lengths, 1)
-    rows = page_table.shape[0]
+    rows, n = page_table.shape
     if rows != B or lengths.shape[0] != B:
         raise ValueError(f"tbf16.{fn}: page_table for {rows} and lengths for {lengths.shape[0]} sequences, q has {B}")
     q, q_st = _rows(q)
-    return q, q_st, page_table, lengths
+    return q, q_st, B, H, page_table, n, lengths
 
 
 def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
@@ -237,8 +237,7 @@ def paged_sdpa(q, k_cache, v_cache, page_table, lengths, scale=None):
     is NaN."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa", k_cache, v_cache)
     _same_device("paged_sdpa", k_cache, v_cache, q, page_table, lengths)
-    q, q_st, page_table, lengths = _queries("paged_sdpa", q, k_cache.shape, page_table, lengths)
-    (B, H, _), n = q.shape, page_table.shape[1]
+    q, q_st, B, H, page_table, n, lengths = _queries("paged_sdpa", q, Hkv, D, page_table, lengths)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return o
@@ -261,11 +260,11 @@ def paged_sdpa_prefix(q, k_cache, v_cache, prefix_table, prefix_length, page_tab
     prefix keys below 2^-80 of the row's largest may count as zero (an infinite value then gives NaN)."""
     (pages, Hkv, page, D), k_st, kc, v_st, vc = _cache("paged_sdpa_prefix", k_cache, v_cache)
     _same_device("paged_sdpa_prefix", k_cache, v_cache, q, prefix_table, prefix_length, page_table, lengths)
-    q, q_st, page_table, lengths = _queries("paged_sdpa_prefix", q, k_cache.shape, page_table, lengths)
+    q, q_st, B, H, page_table, n, lengths = _queries("paged_sdpa_prefix", q, Hkv, D, page_table, lengths)
     prefix_table = _index("paged_sdpa_prefix", "prefix_table", prefix_table, 1)
     if prefix_length.dtype is not torch.int32 or prefix_length.numel() != 1:
         raise TypeError(f"tbf16.paged_sdpa_prefix: expected prefix_length as one int32, got {tuple(prefix_length.shape)}")
-    (B, H, _), m, n = q.shape, prefix_table.shape[0], page_table.shape[1]
+    m = prefix_table.shape[0]
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0:
         return o

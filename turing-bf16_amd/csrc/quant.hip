@@ -383,15 +383,6 @@ __global__ __launch_bounds__(256) void head_amax3_kernel(AmaxSegs segs, int64_t 
   head_amax_block<uint16_t>(g.x, bh, g.H, g.S, D, g.sb, g.sh, g.ss, g.rows, g.nch, blockIdx.y, g.partial);
 }
 
-__global__ void reduce_partials_kernel(const float* __restrict__ partial, int64_t n, int64_t nchunks,
-                                       float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float m = 0.f;
-  for (int64_t c = 0; c < nchunks; ++c) m = fmaxf(m, partial[i * nchunks + c]);
-  out[i] = m;
-}
-
 template <typename Tin, typename Tout>
 __device__ __forceinline__ uint4 scale_cast8(uint4 v, float sc);
 template <>

@@ -88,6 +88,17 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const uint16_t* __rest
   }
 }
 
+// ---- attention ----------------------------------------------------------------------
+
+template <int DP, int RT, int WPB, bool PAD, bool UNIT>
+__global__ __launch_bounds__(WPB * 64, DP == 256 ? 1 : DP == 64 && RT == 1 ? 4 : 2) void paged_attn_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) float lds[];
+  __shared__ int flags[WPB];
+  attn_block<DP, RT, WPB, PAD, UNIT, false>(
+      a, [&](int w) { return lds + w * a.R * (DP + 4); }, lds + WPB * a.R * (DP + 4), flags, blockIdx.x, gridDim.x, blockIdx.y,
+      blockIdx.z);
+}
+
 // The join between blocks: for the unit that block blockIdx.x of the list began and did not end,
 // 64 groups of 4 outputs a block; its waves take the parts in turns and meet in LDS.
 constexpr int kJoinWaves = 8;
@@ -135,6 +146,61 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnArgs a)
   const float f = m == kNone ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(unit_out(a, u.x, u.y, u.w - 1) + (int64_t)row * a.D + d) =
       make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
+}
+
+AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap) {
+  AttnPlan p;
+  const int64_t G = H / Hkv;
+  p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  p.RT = G <= 16 || p.DP == 256 ? 1 : G <= 32 || p.DP == 128 ? 2 : 4;
+  p.R = (int)std::min<int64_t>(G, 16 * p.RT);
+  p.RG = (int)cdiv(G, p.R);
+  p.wpb = p.DP == 256 || p.RT > 1 ? 4 : 8;
+  // Few short units: a launch less on the host and on the device (1 x 32 heads, 100 keys: 5.5 us, the
+  // list and its join 8.4); with more tiles a wave the list's finer split wins (700 keys of 16 heads, 3
+  // tiles a wave: 12.6 and 9.9 us on the device, 12.6 and 16.1 with the host; at 1000 keys, 4 tiles, by 2.3)
+  p.unit = cdiv(cap, kTile) <= 3 * p.wpb && B * Hkv * p.RG <= num_cus();
+  p.stat = p.desc = p.bytes = 0;
+  p.blocks = 0;
+  if (p.unit) return p;
+  // as many as run at once: by registers, 4 waves a SIMD of D = 64, 2 of D = 128, 1 of D = 256
+  p.blocks = num_cus() * (p.DP == 64 || (p.wpb == 4 && p.DP < 256) ? 2 : 1);
+  p.stat = align_up((size_t)p.blocks * 2 * p.R * (size_t)D * 4, 256);
+  p.desc = p.stat + align_up((size_t)p.blocks * 2 * p.R * 2 * 4, 256);
+  p.bytes = p.desc + align_up((size_t)p.blocks * 16, 256);
+  return p;
+}
+
+template <int DP, int RT, int WPB>
+void launch_rows(const AttnArgs& a, bool unit, int64_t blocks, hipStream_t st) {
+  const dim3 grid = unit ? dim3((unsigned)a.B, (unsigned)a.Hkv, (unsigned)a.RG) : dim3((unsigned)blocks);
+  const size_t lds = (size_t)WPB * a.R * (DP + 4 + 2) * 4;
+  const bool pad = a.D != DP;
+#define ATTN(PAD_, UNIT_) \
+  paged_attn_kernel<DP, RT, WPB, PAD_, UNIT_><<<grid, WPB * 64, lds, st>>>(a)
+  if (unit) {
+    if (pad) ATTN(true, true);
+    else ATTN(false, true);
+  } else {
+    if (pad) ATTN(true, false);
+    else ATTN(false, false);
+  }
+#undef ATTN
+}
+
+void launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+#define ATTN(DP_, RT_, WPB_) launch_rows<DP_, RT_, WPB_>(a, p.unit, p.blocks, st)
+  if (p.DP == 64) {
+    if (p.RT == 1) ATTN(64, 1, 8);
+    else if (p.RT == 2) ATTN(64, 2, 4);
+    else ATTN(64, 4, 4);
+  } else if (p.DP == 128) {
+    if (p.RT == 1) ATTN(128, 1, 8);
+    else ATTN(128, 2, 4);
+  } else {
+    ATTN(256, 1, 4);
+  }
+#undef ATTN
 }
 
 }  // namespace

@@ -144,6 +144,33 @@ def launch(name: str, where, *args) -> None:
         raise RuntimeError(f"tbf16: {msg}")
 
 
+def same_device(fn: str, first, *others) -> int:
+    """The device of `first` (its index), which the others have to be on too."""
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("tbf16: expected tensors on a ROCm (cuda) device")
+    for t in others:
+        if t.get_device() != dev:
+            raise ValueError(f"tbf16.{fn}: tensors on {t.device} and {first.device}")
+    return dev
+
+
+# workspace bytes per (device, entry point, its sizes): blocks are counted by the device's CUs, so it
+# is asked on the tensors' device, once
+_WS_BYTES: dict = {}
+
+
+def ws_bytes(dev: int, name: str, *sizes: int) -> int:
+    key = (dev, name, sizes)
+    n = _WS_BYTES.get(key)
+    if n is None:
+        if len(_WS_BYTES) > 4096:
+            _WS_BYTES.clear()
+        with torch.cuda.device(dev):
+            n = _WS_BYTES[key] = int(getattr(lib(), name)(*sizes))
+    return n
+
+
 def ptr(t) -> int | None:
     """Device pointer of a tensor (None for None)."""
     return None if t is None else t.data_ptr()

@@ -11,21 +11,10 @@ from __future__ import annotations
 
 import torch
 
-from ._ext import launch, lib, ptr
+from ._ext import launch, ptr, same_device, ws_bytes
 
 MAX_HEAD_DIM = 256
 _CONTIGUOUS = torch.contiguous_format
-
-
-def _device(x, *others) -> int:
-    """The device of x (its index), which the others have to be on too."""
-    dev = x.get_device()
-    if dev < 0:
-        raise ValueError("tbf16: expected tensors on a ROCm (cuda) device")
-    for t in others:
-        if t.get_device() != dev:
-            raise ValueError(f"tbf16.qk_norm_rope: tensors on {t.device} and {x.device}")
-    return dev
 
 
 def _heads(x):
@@ -83,7 +72,7 @@ def _checked(q, k, wq, wk, cos, sin, positions, eps, interleaved):
         raise ValueError(f"tbf16.qk_norm_rope: eps {eps}")
     if B * S >= 2 ** 31:
         raise ValueError(f"tbf16.qk_norm_rope: {B * S} tokens")
-    _device(q, k, wq, wk, cos, sin, positions)
+    same_device("qk_norm_rope", q, k, wq, wk, cos, sin, positions)
     wq, wk, cos, sin = _table(wq), _table(wk), _table(cos), _table(sin)
     return ((B, S, shape[-2], kshape[-2], D),
             (wq.data_ptr(), wk.data_ptr(), wide, cos.data_ptr(), sin.data_ptr(), table[0], R, positions.data_ptr(), *p_st, eps,
@@ -110,26 +99,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interl
     return yq, yk
 
 
-# tbf16_qk_norm_rope_bwd's workspace bytes per (device, B, S, H, Hkv, D): its blocks are counted by the device's
-# CUs, so it is asked on the tensors' device, once
-_WS_BYTES: dict = {}
-
-
-def _ws_bytes(dev: int, *sizes: int) -> int:
-    key = (dev, sizes)
-    n = _WS_BYTES.get(key)
-    if n is None:
-        if len(_WS_BYTES) > 4096:
-            _WS_BYTES.clear()
-        with torch.cuda.device(dev):
-            n = _WS_BYTES[key] = int(lib().tbf16_qk_norm_rope_bwd_ws_bytes(*sizes))
-    return n
-
-
 def backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dyq, dyk, wanted):
     """Gradients of q, k and both weights (None where wanted says so) from those of the outputs."""
     sizes, tail, kept = _checked(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    dev = _device(q, dyq, dyk)
+    dev = same_device("qk_norm_rope", q, dyq, dyk)
     if dyq.shape != q.shape or dyk.shape != k.shape or dyq.dtype is not torch.bfloat16 or dyk.dtype is not torch.bfloat16:
         raise ValueError(f"tbf16.qk_norm_rope: gradients {tuple(dyq.shape)} {dyq.dtype} and {tuple(dyk.shape)} {dyk.dtype}")
     want_q, want_k, want_wq, want_wk = wanted
@@ -139,7 +112,7 @@ def backward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dy
     dwk = torch.empty_like(kept[1]) if want_wk else None
     ws, wsb = None, 0
     if want_wq or want_wk:
-        wsb = _ws_bytes(dev, *sizes)
+        wsb = ws_bytes(dev, "tbf16_qk_norm_rope_bwd_ws_bytes", *sizes)
         ws = q.new_empty(wsb, dtype=torch.uint8)
     q, at_q, q_st = _heads(q)
     k, at_k, k_st = _heads(k)

@@ -22,6 +22,7 @@ from __future__ import annotations
 import torch
 
 from ._ext import launch, lib, ptr
+from ._ext import same_device as _same_device, ws_bytes as _ws_bytes
 
 MAX_HEAD_DIM = 256
 
@@ -45,15 +46,6 @@ def _cache(fn, k_cache, v_cache):
             or (kc | vc) & 15):
         raise ValueError(f"tbf16.{fn}: cache rows must be contiguous and 16-byte aligned (strides multiples of 8)")
     return shape, k_st, kc, v_st, vc
-
-
-def _same_device(fn, first, *others):
-    dev = first.get_device()
-    if dev < 0:
-        raise ValueError("tbf16: expected tensors on a ROCm (cuda) device")
-    for t in others:
-        if t.get_device() != dev:
-            raise ValueError(f"tbf16.{fn}: tensors on {t.device} and {first.device}")
 
 
 def _index(fn, name, t, dim):
@@ -187,22 +179,6 @@ def paged_write(k_cache, v_cache, k, v, slots) -> None:
     (k, k_st), (v, v_st) = _rows(k), _rows(v)
     launch("tbf16_paged_write", k_cache, k.data_ptr(), v.data_ptr(), T, Hkv, D, k_st[0], k_st[1], v_st[0], v_st[1],
            slots.data_ptr(), kc, vc, pages, page, kc_st[0], kc_st[1], kc_st[2], vc_st[0], vc_st[1], vc_st[2])
-
-
-# workspace bytes per (device, entry point, its sizes): blocks are counted by the device's CUs, so it
-# is asked on the tensors' device, once
-_WS_BYTES: dict = {}
-
-
-def _ws_bytes(dev: int, name: str, *sizes: int) -> int:
-    key = (dev, name, sizes)
-    n = _WS_BYTES.get(key)
-    if n is None:
-        if len(_WS_BYTES) > 4096:
-            _WS_BYTES.clear()
-        with torch.cuda.device(dev):
-            n = _WS_BYTES[key] = int(getattr(lib(), name)(*sizes))
-    return n
 
 
 def _queries(fn, q, Hkv, D, page_table, lengths):

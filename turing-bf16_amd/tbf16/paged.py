@@ -95,6 +95,12 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     the last one, have slot and position -1, which paged_write leaves out and qk_norm_rope gives
     zeros. Taking all granted tokens back leaves lengths, table and stack as they were.
 
+    The attentions' rows are sequences, not tokens. Where a step has at most one new token for each of them and none for
+    some, the tokens' slots and positions go into the order of sequences before anything is computed by them:
+
+        new, at = starts[1:] > starts[:-1], starts[:-1].clamp(max=tokens - 1)
+        slots, positions = torch.where(new, slots[at], -1), torch.where(new, positions[at], -1)
+
     Lengths outside [0, n * page] count as the nearest there is, n_free likewise."""
     shape, row = page_table.shape, page_table.stride()
     others = (lengths, counts, free_pages, n_free) if prefix_length is None else (lengths, counts, free_pages, n_free, prefix_length)

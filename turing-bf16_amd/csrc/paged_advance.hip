@@ -3,8 +3,9 @@
 //
 // With old lengths l, counts c, page the positions of a page, and e = max(0, l + min(c, 0)):
 //   given back   table entries ceil(e / page) .. ceil(l / page), the last sequence's last entry first, so
-//                that taking tokens back puts the stack as it was before they came; entries that name no
-//                page are left out;
+//                that taking tokens back puts the stack as it was before they came (ids on it that are no page
+//                aside, and table entries that were other than -1 past a sequence's pages); entries that name
+//                no page are left out;
 //   granted      sequence b with c > 0 where e + c fits its table row, the sum of c up to b is at most
 //                `tokens`, and it needs no page or the sum of needs up to b is at most the free pages. Needs
 //                of sequences that are not granted count as well, so the rule is two prefix sums.

@@ -93,7 +93,9 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     length on, plus prefix_length int32 (1,) where one is given (the tokens of a prefix that all
     sequences share, which the tables do not hold). Tokens that were not granted, and those past
     the last one, have slot and position -1, which paged_write leaves out and qk_norm_rope gives
-    zeros. Taking all granted tokens back leaves lengths, table and stack as they were.
+    zeros. Taking all granted tokens back leaves lengths, table and the stack's n_free pages as they
+    were, if lengths and n_free were in range, entries past a sequence's pages -1 and the stack's entries
+    pages of the cache (other entries become -1, and an id that is no page does not go back).
 
     The attentions' rows are sequences, not tokens. Where a step has at most one new token for each of them and none for
     some, the tokens' slots and positions go into the order of sequences before anything is computed by them:

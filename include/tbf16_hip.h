@@ -363,7 +363,8 @@ int tbf16_qk_norm_rope_bwd(const void* q, const void* k, const void* dyq, const 
  * become -1 and go on the stack (the last sequence's last one first; those outside [0, pages) are
  * left out). Then, with needs in pages, sequence b gets its counts[b] > 0 tokens if they fit its row,
  * the sum of positive counts up to b is at most tokens, and it needs no page or the sum of the needs
- * of sequences up to b that fit their rows is at most *n_free. starts int32 (B + 1,): where b's
+ * of sequences up to b that fit their rows is at most *n_free (granted or not: a prompt that finds too
+ * few pages leaves none for those behind it). starts int32 (B + 1,): where b's
  * tokens begin, at most tokens. slots, positions int32 (tokens,): page id * page + row, old length +
  * i + *prefix (0 if NULL), or -1 both for tokens that were not granted or are not there; a slot is -1
  * too where the table names no page. B * max_pages and pages * page below 2^31. No two arrays

@@ -93,17 +93,18 @@ __device__ __forceinline__ void token(const AdvanceArgs& a, int t, const int32_t
   if (a.B > 0 && t < starts[a.B]) {
     const int b = last_upto(starts, a.B, t), from = base[b];
     if (from >= 0) {
-      const int j = from + t - starts[b], p = j / a.page, r = j - p * a.page, kept = pages_of(a, from);
-      const int at = top - 1 - first[b] - (p - kept);
+      // (unsigned, and with bounds that hold by themselves unless another stream writes lengths or counts meanwhile:
+      // then from may be of one length and t - starts[b] of another's tokens, up to 2^32 together)
+      const uint32_t j = (uint32_t)from + (uint32_t)(t - starts[b]), p = j / (uint32_t)a.page, r = j - p * (uint32_t)a.page;
+      const uint32_t kept = (uint32_t)pages_of(a, from), at = (uint32_t)(top - 1 - first[b]) - (p - kept);
       int id = -1;
-      // (the bounds hold unless another stream writes lengths or counts meanwhile)
-      if (p < min(kept, a.n)) {
+      if (p < min(kept, (uint32_t)a.n)) {
         id = a.table[b * a.t_sb + p];
-      } else if (p < a.n && (uint32_t)at < (uint32_t)a.P) {
+      } else if (p < (uint32_t)a.n && at < (uint32_t)a.P) {
         id = a.free[at];
         if (r == 0) a.table[b * a.t_sb + p] = id;
       }
-      if ((uint32_t)id < (uint32_t)a.P) slot = id * a.page + r;
+      if ((uint32_t)id < (uint32_t)a.P) slot = id * a.page + (int)r;
       pos = (int)min((int64_t)j + prefix, (int64_t)INT32_MAX);
     }
   }

@@ -89,9 +89,9 @@ def paged_advance(page_table, lengths, counts, free_pages, n_free, page, tokens,
     get their new tokens in order of b. One whose tokens do not fit its table row or `tokens`, or
     that needs pages that are no longer there after what the sequences before it asked for, gets
     none: its length stays. (What one asked for and did not get counts too: behind a prompt that finds
-    too few pages nobody gets one. Sequences that decode belong before prompts in the batch.) The new tokens of all sequences lie one after the other, those of b
-    from starts[b] on (at most `tokens`): slots for paged_write, positions from the sequence's old
-    length on, plus prefix_length int32 (1,) where one is given (the tokens of a prefix that all
+    too few pages nobody gets one. Sequences that decode belong before prompts in the batch.) The new
+    tokens of all sequences lie one after the other, those of b from starts[b] on (at most `tokens`):
+    slots for paged_write, positions from the sequence's old length on, plus prefix_length int32 (1,) where one is given (the tokens of a prefix that all
     sequences share, which the tables do not hold). Tokens that were not granted, and those past
     the last one, have slot and position -1, which paged_write leaves out and qk_norm_rope gives
     zeros. Taking all granted tokens back leaves lengths, table and the stack's n_free pages as they

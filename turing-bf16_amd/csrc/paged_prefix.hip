@@ -539,17 +539,21 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
   PrefixPlan p;
   const int64_t G = H / Hkv, n = B * G;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  // Blocks of 64 rows, two groups of waves on different keys, or of 128: the former where the rows are few, or leave
-  // a fifth and more of 128 empty (192 rows on 16384 keys 38.9 and 42.8 us; 128 rows on 4096: 28.1 and 24.5).
-  p.few = p.DP < 256 && 5 * cdiv(n, 128) * 128 >= 6 * cdiv(n, 64) * 64;
-  p.rows = p.DP == 256 || p.few ? 64 : 128;
   p.keys = p.DP == 256 ? 32 : 64;
+  const int64_t all = cdiv(prefix_cap, p.keys);
+  // Blocks of 64 rows, two groups of waves on different keys, or of 128, which read the keys half as often: the former
+  // where a CU would get up to 8 tiles of the latter, or the rows leave a fifth and more of 128 empty (8 heads, 64 and 128:
+  // 128 rows on 4096 keys 21.9 and 25.5 us, 256 rows 26.2 and 26.7, 512 rows 36.1 and 36.0, 256 rows on 32768 keys 96.9 and
+  // 90.1, 160 rows 80.6 and 88.2; one head, 256 rows on 4096: 15.9 and 19.1. Against it: 4 heads of 80, 65 rows on 2999
+  // keys: 15.5 and 14.9; of 64, 800 rows on 512: 15.0 and 14.1).
+  p.few = p.DP < 256 && ((double)(Hkv * cdiv(n, 128)) * (double)all <= 8.0 * (double)num_cus() ||
+                         5 * cdiv(n, 128) * 128 >= 6 * cdiv(n, 64) * 64);
+  p.rows = p.DP == 256 || p.few ? 64 : 128;
   p.tiles = cdiv(n, p.rows);
   // Splits: a block a CU, which leaves half of its room to the own keys' blocks (256 rows of 8 heads on 8192 keys:
   // 16 splits 35.2 us, two blocks a CU 47.5), but no more than pays for the parts they leave: a tile takes a block
   // ~ 1.3 us, a split's part of all rows 8 bytes an element at 8 TB/s and 0.05 us of the join (65 rows of 4 heads
   // on 2999 keys: 24 splits 13.8 us, 47 splits 15.2).
-  const int64_t all = cdiv(prefix_cap, p.keys);
   const double part_us = (double)(B * H * D) * 1e-6 + 0.05;
   const int64_t most = std::max<int64_t>(1, (int64_t)std::sqrt(1.3 * (double)all / part_us));
   p.S = std::min({all, most, std::max<int64_t>(1, num_cus() / (Hkv * p.tiles))});

@@ -6,7 +6,7 @@
 //   m = max m_i,   l = sum l_i 2^(m_i - m),   o = sum o_i 2^(m_i - m).
 // Two launches: the prefix and behind it, in blocks of the same launch, the sequences' own keys (prefix_kernel; the
 // latter attn_block of paged_attn.h, which leaves sums instead of outputs), and the join of all parts of a row.
-// (The prefix's blocks first: in turns with the others they share CUs unevenly, and take 136 us where alone they take 101.)
+// (The prefix's blocks first: in turns with the others they share CUs unevenly, and took 136 us where alone they took 101.)
 #include <cmath>
 #include <type_traits>
 
@@ -62,11 +62,11 @@ __device__ __forceinline__ int prefix_len(const int32_t* length, int cap) { retu
 //
 // Bound by its instructions where the batch is large: 64 keys and 32 rows of D = 128 are 128 MFMAs, ~ 420 vector
 // instructions and 32 exponentials a wave, two units that overlap in part. 128 sequences of 32 heads on 8 key heads,
-// 32768 keys: 101 us alone with two blocks a CU (680 TFLOPS of the two products as defined, 1020 with the weights'
-// second part), 117 with one, which leaves half of the CU to the own keys' blocks: with up to 1024 of those a sequence
-// a call takes 150 us, with two blocks a CU 160. Where it is small, by a chain: length, page ids, keys, products,
-// parts (4 sequences of 16 heads on 700 keys: 6.7 us). Eight waves on 256 rows in one block were as fast (98 us alone,
-// more with own keys).
+// 32768 keys and none of their own: 144 us a call with two blocks a CU (477 TFLOPS of the two products as defined, 954 with
+// the weights' parts), 162 with one, which leaves half of the CU to the own keys' blocks: with up to 1024 of those a
+// sequence a call takes 177 us, with two blocks a CU 186. Where it is small, by a chain: length, page ids, keys, products,
+// parts (4 sequences of 16 heads on 700 keys: 7.2 us). (Eight waves on 256 rows in one block were as fast, and slower beside
+// own keys.)
 //
 // LDS: chunk c of 16 bytes of row r lies at chunk c ^ f(r) of its row, so that the 16 rows that a read of
 // K takes at one chunk lie in all 64 banks, and so do the two chunks of 8 rows that a transposed read takes.
@@ -550,10 +550,10 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
                          5 * cdiv(n, 128) * 128 >= 6 * cdiv(n, 64) * 64);
   p.rows = p.DP == 256 || p.few ? 64 : 128;
   p.tiles = cdiv(n, p.rows);
-  // Splits: a block a CU, which leaves half of its room to the own keys' blocks (256 rows of 8 heads on 8192 keys:
-  // 16 splits 35.2 us, two blocks a CU 47.5), but no more than pays for the parts they leave: a tile takes a block
-  // ~ 1.3 us, a split's part of all rows 8 bytes an element at 8 TB/s and 0.05 us of the join (65 rows of 4 heads
-  // on 2999 keys: 24 splits 13.8 us, 47 splits 15.2).
+  // Splits: a block a CU, which leaves half of its room to the own keys' blocks (256 rows of 8 heads on 8192 keys
+  // and up to 512 own ones a sequence: 37.1 us, two blocks a CU 45.2; without own ones 34.2 and 32.5), but no more than
+  // pays for the parts they leave: a tile takes a block ~ 1.3 us, a split's part of all rows 8 bytes an element at 8 TB/s and
+  // 0.05 us of the join (65 rows of 4 heads of 80 on 2999 keys: 15.5 us, with up to twice as many splits 15.9).
   const double part_us = (double)(B * H * D) * 1e-6 + 0.05;
   const int64_t most = std::max<int64_t>(1, (int64_t)std::sqrt(1.3 * (double)all / part_us));
   p.S = std::min({all, most, std::max<int64_t>(1, num_cus() / (Hkv * p.tiles))});
@@ -564,8 +564,8 @@ PrefixPlan prefix_plan(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t pre
   o.wpb = 4;
   o.R = (int)std::min<int64_t>(G, own_rows(p.DP));
   o.RG = (int)cdiv(G, o.R);
-  // (a block a unit as long as that is a few tiles a wave: 64 sequences of up to 512 keys, 8 heads, behind 8192: 41.0
-  // and 45.1 us; very many short units are joined to runs)
+  // (a block a unit as long as that is a few tiles a wave: 32 sequences of up to 512 keys, 8 heads, behind 4096:
+  // 22.2 us, as a list 27.7; 64 behind 8192: 37.1 and 38.0; very many short units are joined to runs)
   o.unit = cdiv(cap, kTile) <= 4 * o.wpb && B * Hkv * o.RG <= 4 * num_cus();
   o.blocks = o.unit ? B * Hkv * o.RG : 2 * num_cus();
   o.stat = align_up((size_t)o.blocks * 2 * o.R * (size_t)D * 4, 256);

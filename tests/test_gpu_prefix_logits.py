@@ -174,3 +174,26 @@ def test_large_tables_of_small_logits_and_one_large(dev, B, H, Hkv, D):
         own = [torch.randint(0, 2 ** 10, (Hkv, b % 9), generator=gen(b)) for b in range(B)]
         a = make(dev, far, own, H, D, 16, power=7)
         close(tbf16.paged_sdpa_prefix(*a, scale=1.0), *expected(a, far, own, 7, 1.0))
+
+
+def expected_of_rows(a, far, own, power, scale):
+    """expected() with a power of its own for each query, (B, H)."""
+    ref, bound = torch.empty(a[0].shape, dtype=torch.float64), torch.empty(a[0].shape, dtype=torch.float64)
+    for t in power.unique().tolist():
+        r, e = expected(a, far, own, t, scale)
+        ref[power == t], bound[power == t] = r[power == t], e[power == t]
+    return ref, bound
+
+
+@pytest.mark.parametrize("B,H,Hkv,D", FORMS)
+@pytest.mark.parametrize("most", [12, 30, 100])
+def test_rows_of_every_size_side_by_side(dev, B, H, Hkv, D, most):
+    """Queries of a power of two each, so that one wave has small logits, large ones, and some around where the maximum
+    follows at once."""
+    g = gen(most + D)
+    far, own = near_the_top(g, Hkv, 208, 1), [near_the_top(g, Hkv, b % 40, 1) for b in range(B)]
+    a = make(dev, far, own, H, D, 16, power=-16, seed=D)
+    up = torch.randint(0, most, (B, H), generator=g)
+    a[0].mul_(torch.exp2(up.float())[..., None].to(dev))
+    for scale in (1.0, -1.0):
+        close(tbf16.paged_sdpa_prefix(*a, scale=scale), *expected_of_rows(a, far, own, up - 16, scale))
